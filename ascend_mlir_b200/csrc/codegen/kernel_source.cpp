@@ -600,6 +600,9 @@ GeneratedKernel generateKernelSource(const LaunchDescriptor &d) {
   case KernelClass::Gather: return generateGatherRows(d);
   case KernelClass::Transpose: out.whyNot = "a bare permutation has no body to generate: it runs on the prebuilt transpose kernel"; return out;
   case KernelClass::Matmul: out.whyNot = "the matmul group is the hand-written tcgen05 kernel of the library"; return out;
+  case KernelClass::BlockNorm:
+  case KernelClass::Checkpoint:
+  case KernelClass::CheckpointGrad: out.whyNot = "a hand-written kernel of the library"; return out;
   }
   out.whyNot = "unknown kernel class";
   return out;

@@ -1,0 +1,256 @@
+// Host side of the row passes: which team and kernel a launch takes, how the gradient's rows are split, and the kernel
+// that adds the teams' column sums.
+#include "kernels/block_norm.h"
+
+#include <algorithm>
+
+#include "kernels/block_norm_kernels.h"
+#include "kernels/launch_util.h"
+
+namespace afir {
+namespace kernels {
+namespace {
+
+// ---- the column sums --------------------------------------------------------------------------------------------
+struct FinishParams {
+  int layer, elemType, paramType, gateForm, gateAct;
+  int64_t cols, groups, chunks, teams, sumsLd;
+  const float *sumsA, *sumsB;  // null = that norm is not part of the pass
+  const void *weight, *bias, *scale, *gate;
+  int64_t gateLd;
+  float *dweight, *dbias, *dscale, *nextWeight, *nextBias, *dgate;
+  int64_t dgateLd;
+};
+
+__device__ __forceinline__ float elemAt(const void *p, int type, int64_t at) {
+  if (type == kF32) return static_cast<const float *>(p)[at];
+  if (type == kF16) return __half2float(static_cast<const __half *>(p)[at]);
+  return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[at]);
+}
+
+constexpr int kFinishCols = 8, kFinishSlots = 64;
+
+// Adds one value per slot over `slots` neighbouring slots (a power of two); the first slot of each run gets the sum.
+__device__ __forceinline__ float slotSum(float v, float (*buf)[kFinishCols], int slots) {
+  const int c = threadIdx.x, s = threadIdx.y;
+  buf[s][c] = v;
+  __syncthreads();
+  for (int o = slots / 2; o > 0; o >>= 1) {
+    if ((s & (slots - 1)) < o) buf[s][c] += buf[s + o][c];
+    __syncthreads();
+  }
+  v = buf[s & ~(slots - 1)][c];
+  __syncthreads();
+  return v;
+}
+
+// 8 columns (one 32-byte sector of every row of sums) x 64 slots per CTA: the slots share the rows of sums, and the
+// order in which they are added depends on the sizes alone.
+__global__ void __launch_bounds__(kFinishCols *kFinishSlots) blockNormFinishKernel(const __grid_constant__ FinishParams p) {
+  gridDependencyPrologue();
+  __shared__ float buf[kFinishSlots][kFinishCols];
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * kFinishCols + threadIdx.x;
+  const bool live = col < p.cols;
+  const int slot = threadIdx.y;
+  const int values = p.layer ? 2 : 1;
+  if (p.sumsA) {
+    // slots as (groups at once) x (slots per group)
+    int atOnce = 1;
+    while (atOnce < p.groups && atOnce < kFinishSlots) atOnce *= 2;
+    const int perGroup = kFinishSlots / atOnce;
+    const float w = live ? elemAt(p.weight, p.paramType, col) : 0.0f;
+    const float b = live && p.layer ? elemAt(p.bias, p.paramType, col) : 0.0f;
+    const float scale = live && p.scale ? elemAt(p.scale, p.paramType, col) : 1.0f;
+    float total[2] = {0.0f, 0.0f};
+    for (int64_t g0 = 0; g0 < p.groups; g0 += atOnce) {
+      const int64_t group = g0 + slot / perGroup;
+      float s[2] = {0.0f, 0.0f};
+      if (live && group < p.groups)
+        for (int64_t c = slot & (perGroup - 1); c < p.chunks; c += perGroup)
+          for (int k = 0; k < values; ++k) s[k] += p.sumsA[((group * p.chunks + c) * values + k) * p.sumsLd + col];
+      if (perGroup > 1)
+        for (int k = 0; k < values; ++k) s[k] = slotSum(s[k], buf, perGroup);
+      if (live && group < p.groups && (slot & (perGroup - 1)) == 0) {
+        float a = 1.0f;
+        if (p.gateForm == kGateGroup) {
+          a = gateValue(elemAt(p.gate, p.elemType, group * p.gateLd + col), p.gateAct);
+          p.dgate[group * p.dgateLd + col] = scale * fmaf(w, s[0], b * s[1]) * gateSlope(a, p.gateAct);
+        }
+        total[0] = fmaf(a, s[0], total[0]);
+        total[1] = fmaf(a, s[1], total[1]);
+      }
+    }
+    for (int k = 0; k < values; ++k) total[k] = slotSum(total[k], buf, kFinishSlots);
+    if (live && slot == 0) {
+      p.dweight[col] = scale * total[0];
+      if (p.dbias) p.dbias[col] = scale * total[1];
+      if (p.dscale) p.dscale[col] = fmaf(w, total[0], b * total[1]);
+    }
+  }
+  if (p.sumsB) {
+    float s[2] = {0.0f, 0.0f};
+    if (live)
+      for (int64_t t = slot; t < p.teams; t += kFinishSlots)
+        for (int k = 0; k < values; ++k) s[k] += p.sumsB[(t * values + k) * p.sumsLd + col];
+    for (int k = 0; k < values; ++k) s[k] = slotSum(s[k], buf, kFinishSlots);
+    if (live && slot == 0) {
+      p.nextWeight[col] = s[0];
+      if (p.nextBias) p.nextBias[col] = s[1];
+    }
+  }
+}
+
+// ---- launch shape -----------------------------------------------------------------------------------------------
+struct TeamShape { bool vector; int nv, lanes, teamsPerCta; };
+
+// A team has at most 512 threads; a row that fits them with one vector each takes one (short rows: fewer threads, more
+// teams), a wider one takes 2, 4 or 8.
+TeamShape teamShape(int elemType, int64_t cols, bool vector) {
+  TeamShape s;
+  s.vector = vector;
+  const int vec = vector ? (elemType == kF32 ? 4 : 8) : 1;
+  if (vector) {
+    s.nv = 1;
+    while (static_cast<int64_t>(s.nv) * vec * 512 < cols) s.nv *= 2;
+  } else {
+    s.nv = cols <= kScalarSmall * 512 ? kScalarSmall : kScalarLarge;
+  }
+  const int64_t perThread = static_cast<int64_t>(s.nv) * vec;
+  const int64_t threads = (cols + perThread - 1) / perThread;
+  s.lanes = static_cast<int>((threads + 31) / 32 * 32);
+  s.teamsPerCta = std::max(1, 256 / s.lanes);
+  return s;
+}
+
+bool rowsAligned(const void *base, int64_t ld, int64_t elemBytes, int64_t bytes) {
+  return !base || ((reinterpret_cast<uintptr_t>(base) % static_cast<uintptr_t>(bytes)) == 0 && (ld * elemBytes) % bytes == 0);
+}
+bool vectorAligned(const void *base) { return (reinterpret_cast<uintptr_t>(base) & 15u) == 0; }
+
+GradPlan gradPlan(int gateForm, int64_t rows, int64_t cols, int64_t groupRows, int smCount) {
+  GradPlan plan = {};
+  const bool grouped = gateForm == kGateGroup;
+  plan.groupRows = grouped ? std::min(groupRows, std::max<int64_t>(rows, 1)) : std::max<int64_t>(rows, 1);
+  plan.groups = (rows + plan.groupRows - 1) / plan.groupRows;
+  if (!grouped) plan.groups = 1;
+  // About 8192 columns' worth of teams per SM: enough rows under way to cover a row's two sums, few enough that the
+  // teams' sums (f32, one or two rows each) stay small beside the row tensors.
+  const int64_t perSm = std::min<int64_t>(16, std::max<int64_t>(1, 8192 / cols));
+  const int64_t teams = std::max<int64_t>(1, std::min<int64_t>(rows, smCount * perSm));
+  const int64_t wanted = std::max<int64_t>(1, plan.groups ? teams / plan.groups : 1);
+  plan.chunkRows = (plan.groupRows + wanted - 1) / wanted;
+  plan.chunks = (plan.groupRows + plan.chunkRows - 1) / plan.chunkRows;
+  plan.teams = std::max<int64_t>(1, std::min<int64_t>(teams, plan.groups * plan.chunks));
+  plan.sumsLd = (cols + 3) / 4 * 4;
+  return plan;
+}
+
+int64_t sumsFloats(const GradPlan &plan, int pass, int kind) {
+  const int64_t values = kind == kLayerNorm ? 2 : 1;
+  return values * plan.sumsLd * ((pass != kPre ? plan.groups * plan.chunks : 0) + (pass != kPost ? plan.teams : 0));
+}
+
+} // namespace
+
+int launchBlockNorm(const BlockNormLaunch &l, cudaStream_t stream, int *launched) {
+  if (launched) *launched = 0;
+  if (l.rows == 0) return 0;
+  if (l.cols <= 0 || l.cols > kMaxNormCols) return cudaErrorInvalidValue;
+  const int64_t eb = elemBytes(l.elemType);
+  const int vec = static_cast<int>(16 / eb);
+  bool vector = l.cols % vec == 0;
+  for (const RowsIn &r : {l.x, l.y, l.gate}) vector = vector && rowsAligned(r.base, r.ld, eb, 16);
+  for (const RowsOut &r : {l.out, l.h}) vector = vector && rowsAligned(r.base, r.ld, eb, 16);
+  for (const void *v : {l.a.weight, l.a.bias, l.b.weight, l.b.bias, l.scale}) vector = vector && vectorAligned(v);
+  vector = vector && rowsAligned(l.checkpoint.codes, l.checkpoint.codesLd, 1, vec);
+  const TeamShape s = teamShape(l.elemType, l.cols, vector);
+  const ForwardKernel kernel = l.elemType == kF32   ? forwardKernel<kF32>(l.kind, l.pass, vector, s.nv)
+                               : l.elemType == kF16 ? forwardKernel<kF16>(l.kind, l.pass, vector, s.nv)
+                                                    : forwardKernel<kBF16>(l.kind, l.pass, vector, s.nv);
+  if (!kernel) return cudaErrorInvalidValue;
+  const int64_t ctas = (l.rows + s.teamsPerCta - 1) / s.teamsPerCta;
+  const unsigned int grid = static_cast<unsigned int>(std::min<int64_t>(ctas, 0x7fffffff));
+  // without vectors a block of 128 columns spans warps: the checkpoint is a launch of its own, and the first one, in
+  // case an output takes the place of the tensor it reads
+  if (l.checkpoint.codes && !vector) {
+    CheckpointPackLaunch c = {};
+    c.elemType = l.elemType;
+    c.rows = l.rows;
+    c.cols = l.cols;
+    c.x = l.pass == kPre ? l.x : l.y;
+    c.out = l.checkpoint;
+    if (const int rc = launchCheckpointPack(c, stream, launched); rc != 0) return rc;
+  }
+  const cudaError_t e = launchDependent(kernel, dim3(grid), dim3(static_cast<unsigned int>(s.lanes * s.teamsPerCta)), 0, stream, l, s.lanes);
+  if (e == cudaSuccess && launched) *launched += 1;
+  return e;
+}
+
+size_t blockNormGradWorkspaceBytes(int pass, int kind, int gateForm, int64_t rows, int64_t cols, int64_t groupRows, int smCount) {
+  return static_cast<size_t>(sumsFloats(gradPlan(gateForm, rows, cols, groupRows, smCount), pass, kind)) * sizeof(float);
+}
+
+int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *launched) {
+  if (launched) *launched = 0;
+  if (l.cols <= 0 || l.cols > kMaxNormCols) return cudaErrorInvalidValue;
+  int device = 0;
+  if (const cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return e;
+  GradPlan plan = gradPlan(l.gateForm, l.rows, l.cols, l.groupRows, deviceSmCount(device));
+  const size_t need = static_cast<size_t>(sumsFloats(plan, l.pass, l.kind)) * sizeof(float);
+  if (!l.workspace || l.workspaceBytes < need || !vectorAligned(l.workspace)) return cudaErrorInvalidValue;
+  const int64_t values = l.kind == kLayerNorm ? 2 : 1;
+  if (l.pass != kPre) plan.sumsA = static_cast<float *>(l.workspace);
+  if (l.pass != kPost) plan.sumsB = static_cast<float *>(l.workspace) + (l.pass != kPre ? plan.groups * plan.chunks * values * plan.sumsLd : 0);
+
+  if (l.rows > 0) {
+    const int64_t eb = elemBytes(l.elemType);
+    const int vec = static_cast<int>(16 / eb);
+    bool vector = l.cols % vec == 0;
+    for (const RowsIn &r : {l.dout, l.dh, l.source, l.y, l.gate}) vector = vector && rowsAligned(r.base, r.ld, eb, 16);
+    for (const RowsOut &r : {l.dx, l.dy}) vector = vector && rowsAligned(r.base, r.ld, eb, 16);
+    if (l.gateForm == kGateToken) vector = vector && rowsAligned(l.dgate.base, l.dgate.ld, eb, 16);
+    for (const void *v : {l.a.weight, l.a.bias, l.b.weight, l.scale}) vector = vector && vectorAligned(v);
+    vector = vector && rowsAligned(l.checkpoint.codes, l.checkpoint.codesLd, 1, vec);
+    const TeamShape s = teamShape(l.elemType, l.cols, vector);
+    const GradKernel kernel = l.elemType == kF32   ? gradKernel<kF32>(l.kind, l.pass, vector, s.nv)
+                              : l.elemType == kF16 ? gradKernel<kF16>(l.kind, l.pass, vector, s.nv)
+                                                   : gradKernel<kBF16>(l.kind, l.pass, vector, s.nv);
+    if (!kernel) return cudaErrorInvalidValue;
+    const unsigned int grid = static_cast<unsigned int>((plan.teams + s.teamsPerCta - 1) / s.teamsPerCta);
+    const cudaError_t e = launchDependent(kernel, dim3(grid), dim3(static_cast<unsigned int>(s.lanes * s.teamsPerCta)), 0, stream, l, plan, s.lanes);
+    if (e != cudaSuccess) return e;
+    if (launched) *launched += 1;
+  }
+  FinishParams f = {};
+  f.layer = l.kind == kLayerNorm;
+  f.elemType = l.elemType;
+  f.paramType = l.paramType;
+  f.gateForm = l.gateForm;
+  f.gateAct = l.gateAct;
+  f.cols = l.cols;
+  f.sumsLd = plan.sumsLd;
+  f.groups = plan.groups;
+  f.chunks = l.rows > 0 ? plan.chunks : 0;  // no rows: the gradients are sums of nothing
+  f.teams = l.rows > 0 ? plan.teams : 0;
+  f.sumsA = l.pass != kPre ? plan.sumsA : nullptr;
+  f.sumsB = l.pass != kPost ? plan.sumsB : nullptr;
+  f.weight = l.a.weight;
+  f.bias = l.a.bias;
+  f.scale = l.scale;
+  f.gate = l.gate.base;
+  f.gateLd = l.gate.ld;
+  f.dweight = l.da.weight;
+  f.dbias = l.da.bias;
+  f.dscale = l.dscale;
+  f.nextWeight = l.db.weight;
+  f.nextBias = l.db.bias;
+  f.dgate = static_cast<float *>(l.gateForm == kGateGroup ? l.dgate.base : nullptr);
+  f.dgateLd = l.dgate.ld;
+  const unsigned int grid = static_cast<unsigned int>((l.cols + kFinishCols - 1) / kFinishCols);
+  const cudaError_t e = launchDependent(blockNormFinishKernel, dim3(grid), dim3(kFinishCols, kFinishSlots), 0, stream, f);
+  if (e == cudaSuccess && launched) *launched += 1;
+  return e;
+}
+
+} // namespace kernels
+} // namespace afir

@@ -1,0 +1,160 @@
+// Forward row passes: h = normB(x); out = alpha*x + scale*act(gate)*(normA(y)*weight + bias); h = normB(out).
+//
+// One team of threads per row.  A row is read once and held in registers (f32) across its statistics, so every tensor
+// crosses HBM once; the mean and the variance of a layer norm are two sums over those registers, not one sum of
+// squares, so that a row far from zero loses nothing.  Statistics, the gate and the sums are f32; `out` and `h` are
+// rounded once each, and normB reads `out` as it was rounded, which is what the gradient pass will read.
+#pragma once
+
+#include "kernels/block_norm_device.cuh"
+
+namespace afir {
+namespace kernels {
+
+// Statistics of the row in v (columns at or beyond `cols` are not counted).
+template <int KIND, int NV, int VEC>
+__device__ __forceinline__ void rowStatistics(Team &team, const float (&v)[NV][VEC], int cols, float eps, float &mean, float &rstd) {
+  const float share = 1.0f / static_cast<float>(cols);
+  mean = 0.0f;
+  if constexpr (KIND == kLayerNorm) {
+    float s[1] = {0.0f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s[0] += v[i][e];  // zeros beyond the row
+    teamSum(team, s);
+    mean = s[0] * share;
+  }
+  float q[1] = {0.0f};
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if ((i * team.lanes + team.lane) * VEC >= cols) continue;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float d = v[i][e] - mean;
+      q[0] += d * d;
+    }
+  }
+  teamSum(team, q);
+  rstd = 1.0f / sqrtf(q[0] * share + eps);
+}
+
+template <int ELEM, int KIND, int NV, int VEC>
+__device__ __forceinline__ void storeNormed(const Team &team, const float (&v)[NV][VEC], int cols, float mean, float rstd,
+                                            const NormVectors &p, int paramType, void *base, int64_t rowAt) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int col = (i * team.lanes + team.lane) * VEC;
+    if (col >= cols) continue;
+    float w[VEC], r[VEC];
+    loadParam<ELEM, VEC>(p.weight, paramType, col, w);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) r[e] = (v[i][e] - mean) * rstd * w[e];
+    if constexpr (KIND == kLayerNorm) {
+      loadParam<ELEM, VEC>(p.bias, paramType, col, w);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) r[e] += w[e];
+    }
+    storeElems<ELEM, VEC>(base, rowAt + col, r);
+  }
+}
+
+__device__ __forceinline__ void storeStatistics(const Team &team, const NormStatsOut &s, int64_t row, float mean, float rstd) {
+  if (team.lane != 0) return;
+  if (s.rstd) s.rstd[row] = rstd;
+  if (s.mean) s.mean[row] = mean;
+}
+
+// The 8-bit checkpoint of the row in v.  128 columns are 128 / VEC neighbouring lanes: the largest magnitude is a
+// shuffle tree over them.
+template <int ELEM, int NV, int VEC>
+__device__ __forceinline__ void storeCheckpoint(const Team &team, const float (&v)[NV][VEC], int cols, const CheckpointOut &c, int64_t row) {
+  static_assert(VEC >= 4, "128 columns inside one warp");
+  constexpr int kGroup = kCheckpointBlock / VEC;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int col = (i * team.lanes + team.lane) * VEC;
+    float top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) top = fmaxf(top, finiteMagnitude(v[i][e]));
+#pragma unroll
+    for (int o = kGroup / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (col >= cols) continue;
+    const int e8 = checkpointExponent<ELEM>(top);
+    const CheckpointScale s = checkpointScale<ELEM>(e8);
+    float r[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) r[e] = scaledForCode(v[i][e], s);
+    storeCodes<VEC>(c.codes + row * c.codesLd + col, r);
+    if (col % kCheckpointBlock == 0) c.exps[row * c.expsLd + col / kCheckpointBlock] = static_cast<uint8_t>(e8);
+  }
+}
+
+template <int ELEM, int KIND, int PASS, int VEC, int NV>
+__global__ void __launch_bounds__(512) blockNormForwardKernel(const __grid_constant__ BlockNormLaunch p, int teamLanes) {
+  gridDependencyPrologue();
+  __shared__ float scratch[kTeamScratchFloats];
+  Team team = makeTeam(teamLanes, scratch);
+  const int cols = static_cast<int>(p.cols);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * team.count;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * team.count + team.index; row < p.rows; row += step) {
+    const RowsIn first = PASS == kPre ? p.x : p.y;
+    float v[NV][VEC];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int col = (i * team.lanes + team.lane) * VEC;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[i][e] = 0.0f;
+      if (col < cols) loadElems<ELEM, VEC>(first.base, row * first.ld + col, v[i]);
+    }
+    if constexpr (VEC > 1) {
+      if (p.checkpoint.codes) storeCheckpoint<ELEM, NV, VEC>(team, v, cols, p.checkpoint, row);
+    }
+    float mean, rstd;
+    rowStatistics<KIND, NV, VEC>(team, v, cols, PASS == kPre ? p.epsB : p.epsA, mean, rstd);
+    if constexpr (PASS == kPre) {
+      storeStatistics(team, p.statsB, row, mean, rstd);
+      storeNormed<ELEM, KIND, NV, VEC>(team, v, cols, mean, rstd, p.b, p.paramType, p.h.base, row * p.h.ld);
+    } else {
+      storeStatistics(team, p.statsA, row, mean, rstd);
+      const int64_t gateRow = p.gateForm == kGateGroup ? row / p.groupRows : row;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int col = (i * team.lanes + team.lane) * VEC;
+        if (col >= cols) continue;
+        float t[VEC];
+        loadParam<ELEM, VEC>(p.a.weight, p.paramType, col, t);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[i][e] = (v[i][e] - mean) * rstd * t[e];
+        if constexpr (KIND == kLayerNorm) {
+          loadParam<ELEM, VEC>(p.a.bias, p.paramType, col, t);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) v[i][e] += t[e];
+        }
+        if (p.gateForm != kGateNone) {
+          loadElems<ELEM, VEC>(p.gate.base, gateRow * p.gate.ld + col, t);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) v[i][e] *= gateValue(t[e], p.gateAct);
+        }
+        if (p.scale) {
+          loadParam<ELEM, VEC>(p.scale, p.paramType, col, t);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) v[i][e] *= t[e];
+        }
+        loadElems<ELEM, VEC>(p.x.base, row * p.x.ld + col, t);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)  // as it is stored
+          v[i][e] = ElemOf<ELEM>::widen(ElemOf<ELEM>::narrow(fmaf(p.alpha, t[e], v[i][e])));
+        storeElems<ELEM, VEC>(p.out.base, row * p.out.ld + col, v[i]);
+      }
+      if constexpr (PASS == kPostPre) {
+        rowStatistics<KIND, NV, VEC>(team, v, cols, p.epsB, mean, rstd);
+        storeStatistics(team, p.statsB, row, mean, rstd);
+        storeNormed<ELEM, KIND, NV, VEC>(team, v, cols, mean, rstd, p.b, p.paramType, p.h.base, row * p.h.ld);
+      }
+    }
+  }
+}
+
+} // namespace kernels
+} // namespace afir

@@ -1,0 +1,7 @@
+#include "kernels/block_norm_forward_pick.cuh"
+
+namespace afir {
+namespace kernels {
+template ForwardKernel forwardKernel<kF16>(int kind, int pass, bool vector, int nv);
+} // namespace kernels
+} // namespace afir

@@ -1,0 +1,32 @@
+// The instantiations of the forward row kernel for one element type (included by one file per type).
+#pragma once
+
+#include "kernels/block_norm_forward.cuh"
+#include "kernels/block_norm_kernels.h"
+
+namespace afir {
+namespace kernels {
+
+template <int ELEM, int KIND, int PASS> ForwardKernel forwardKernelOf(bool vector, int nv) {
+  constexpr int V = ElemOf<ELEM>::kVec;
+  if (!vector) return nv <= kScalarSmall ? blockNormForwardKernel<ELEM, KIND, PASS, 1, kScalarSmall> : blockNormForwardKernel<ELEM, KIND, PASS, 1, kScalarLarge>;
+  switch (nv) {
+  case 1: return blockNormForwardKernel<ELEM, KIND, PASS, V, 1>;
+  case 2: return blockNormForwardKernel<ELEM, KIND, PASS, V, 2>;
+  case 4: return blockNormForwardKernel<ELEM, KIND, PASS, V, 4>;
+  default:
+    if constexpr (ELEM == kF32) return blockNormForwardKernel<ELEM, KIND, PASS, V, 8>;
+    else return nullptr;
+  }
+}
+template <int ELEM, int KIND> ForwardKernel forwardKernelOf(int pass, bool vector, int nv) {
+  if (pass == kPre) return forwardKernelOf<ELEM, KIND, kPre>(vector, nv);
+  if (pass == kPost) return forwardKernelOf<ELEM, KIND, kPost>(vector, nv);
+  return forwardKernelOf<ELEM, KIND, kPostPre>(vector, nv);
+}
+template <int ELEM> ForwardKernel forwardKernel(int kind, int pass, bool vector, int nv) {
+  return kind == kLayerNorm ? forwardKernelOf<ELEM, kLayerNorm>(pass, vector, nv) : forwardKernelOf<ELEM, kRmsNorm>(pass, vector, nv);
+}
+
+} // namespace kernels
+} // namespace afir

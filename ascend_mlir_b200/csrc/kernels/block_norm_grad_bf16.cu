@@ -1,0 +1,7 @@
+#include "kernels/block_norm_grad_pick.cuh"
+
+namespace afir {
+namespace kernels {
+template GradKernel gradKernel<kBF16>(int kind, int pass, bool vector, int nv);
+} // namespace kernels
+} // namespace afir

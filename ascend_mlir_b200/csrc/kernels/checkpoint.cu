@@ -1,0 +1,147 @@
+// 8-bit activation checkpoints: pack (x -> codes and exponents) and restore (-> values in the type again).
+//
+// value = e4m3(code) * 2^(exp - 127), one power of two per row and 128 columns: the restored value is exact in the type
+// the tensor had, so what a checkpoint loses is the one rounding to four significant bits.  1 + 1/128 bytes per element
+// for 2 or 4.  Both are one pass over the data, bound by HBM.
+#include "kernels/block_norm.h"
+
+#include <algorithm>
+
+#include "kernels/block_norm_device.cuh"
+#include "kernels/launch_util.h"
+
+namespace afir {
+namespace kernels {
+namespace {
+
+constexpr int kThreads = 256;
+
+// 128 columns are 16 lanes (8 columns each, 16-bit types) or 32 lanes (4 each, f32); a thread's vectors are neighbouring
+// in a flat numbering of [rows, blocks of 128, lanes], so a warp reads whole lines and a row may end inside a block.
+template <int ELEM>
+__global__ void __launch_bounds__(kThreads) checkpointPackVectorKernel(const __grid_constant__ CheckpointPackLaunch p) {
+  gridDependencyPrologue();
+  constexpr int VEC = ElemOf<ELEM>::kVec;
+  constexpr int kLanes = kCheckpointBlock / VEC;
+  const int cols = static_cast<int>(p.cols);
+  const int64_t blocks = (cols + kCheckpointBlock - 1) / kCheckpointBlock;
+  const int64_t units = p.rows * blocks * kLanes;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+  // whole warps go round together: the bound is rounded up to a warp
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; u < (units + 31) / 32 * 32; u += step) {
+    const int64_t block = u / kLanes, row = block / blocks;
+    const int b = static_cast<int>(block - row * blocks);
+    const int col = b * kCheckpointBlock + static_cast<int>(u & (kLanes - 1)) * VEC;
+    const bool live = u < units && col < cols;
+    float v[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = 0.0f;
+    if (live) loadElems<ELEM, VEC>(p.x.base, row * p.x.ld + col, v);
+    float top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) top = fmaxf(top, finiteMagnitude(v[e]));
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (!live) continue;
+    const int e8 = checkpointExponent<ELEM>(top);
+    const CheckpointScale s = checkpointScale<ELEM>(e8);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = scaledForCode(v[e], s);
+    storeCodes<VEC>(p.out.codes + row * p.out.codesLd + col, v);
+    if ((u & (kLanes - 1)) == 0) p.out.exps[row * p.out.expsLd + b] = static_cast<uint8_t>(e8);
+  }
+}
+
+// Any width and alignment: a warp per block, four columns per lane.
+template <int ELEM>
+__global__ void __launch_bounds__(kThreads) checkpointPackScalarKernel(const __grid_constant__ CheckpointPackLaunch p) {
+  gridDependencyPrologue();
+  const int cols = static_cast<int>(p.cols), lane = threadIdx.x & 31;
+  const int64_t blocks = (cols + kCheckpointBlock - 1) / kCheckpointBlock;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / 32);
+  for (int64_t block = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); block < p.rows * blocks; block += step) {
+    const int64_t row = block / blocks;
+    const int b = static_cast<int>(block - row * blocks);
+    float v[4][1];
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int col = b * kCheckpointBlock + i * 32 + lane;
+      v[i][0] = 0.0f;
+      if (col < cols) loadElems<ELEM, 1>(p.x.base, row * p.x.ld + col, v[i]);
+      top = fmaxf(top, finiteMagnitude(v[i][0]));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const int e8 = checkpointExponent<ELEM>(top);
+    const CheckpointScale s = checkpointScale<ELEM>(e8);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int col = b * kCheckpointBlock + i * 32 + lane;
+      if (col >= cols) continue;
+      v[i][0] = scaledForCode(v[i][0], s);
+      storeCodes<1>(p.out.codes + row * p.out.codesLd + col, v[i]);
+    }
+    if (lane == 0) p.out.exps[row * p.out.expsLd + b] = static_cast<uint8_t>(e8);
+  }
+}
+
+template <int ELEM, int VEC>
+__global__ void __launch_bounds__(kThreads) checkpointRestoreKernel(const __grid_constant__ CheckpointRestoreLaunch p) {
+  gridDependencyPrologue();
+  const int64_t perRow = p.cols / VEC;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; u < p.rows * perRow; u += step) {
+    const int64_t row = u / perRow;
+    const int col = static_cast<int>(u - row * perRow) * VEC;
+    float v[VEC];
+    loadCheckpoint<VEC>(p.in, row, col, v);
+    storeElems<ELEM, VEC>(p.out.base, row * p.out.ld + col, v);
+  }
+}
+
+bool aligned(const void *base, int64_t rowBytes, int64_t bytes) {
+  return (reinterpret_cast<uintptr_t>(base) % static_cast<uintptr_t>(bytes)) == 0 && rowBytes % bytes == 0;
+}
+unsigned int gridFor(int64_t units, int64_t perCta) {
+  int device = 0;
+  cudaGetDevice(&device);
+  const int64_t ctas = (units + perCta - 1) / perCta;
+  return static_cast<unsigned int>(std::max<int64_t>(1, std::min<int64_t>(ctas, static_cast<int64_t>(deviceSmCount(device)) * 64)));
+}
+
+} // namespace
+
+int launchCheckpointPack(const CheckpointPackLaunch &l, cudaStream_t stream, int *launched) {
+  if (l.rows == 0) return 0;
+  if (l.cols <= 0 || l.cols > (1ll << 30)) return cudaErrorInvalidValue;
+  const int64_t eb = elemBytes(l.elemType), vec = 16 / eb;
+  const int64_t blocks = (l.cols + kCheckpointBlock - 1) / kCheckpointBlock;
+  const bool vector = l.cols % vec == 0 && aligned(l.x.base, l.x.ld * eb, 16) && aligned(l.out.codes, l.out.codesLd, vec);
+  cudaError_t e;
+  if (vector) {
+    const auto kernel = l.elemType == kF32 ? checkpointPackVectorKernel<kF32> : l.elemType == kF16 ? checkpointPackVectorKernel<kF16> : checkpointPackVectorKernel<kBF16>;
+    e = launchDependent(kernel, dim3(gridFor(l.rows * blocks * (kCheckpointBlock / vec), kThreads)), dim3(kThreads), 0, stream, l);
+  } else {
+    const auto kernel = l.elemType == kF32 ? checkpointPackScalarKernel<kF32> : l.elemType == kF16 ? checkpointPackScalarKernel<kF16> : checkpointPackScalarKernel<kBF16>;
+    e = launchDependent(kernel, dim3(gridFor(l.rows * blocks, kThreads / 32)), dim3(kThreads), 0, stream, l);
+  }
+  if (e == cudaSuccess && launched) *launched += 1;
+  return e;
+}
+
+int launchCheckpointRestore(const CheckpointRestoreLaunch &l, cudaStream_t stream, int *launched) {
+  if (l.rows == 0) return 0;
+  if (l.cols <= 0 || l.cols > (1ll << 30)) return cudaErrorInvalidValue;
+  const int64_t eb = elemBytes(l.elemType), vec = 16 / eb;
+  const bool vector = l.cols % vec == 0 && aligned(l.out.base, l.out.ld * eb, 16) && aligned(l.in.codes, l.in.codesLd, vec);
+  const auto kernel = l.elemType == kF32   ? (vector ? checkpointRestoreKernel<kF32, 4> : checkpointRestoreKernel<kF32, 1>)
+                      : l.elemType == kF16 ? (vector ? checkpointRestoreKernel<kF16, 8> : checkpointRestoreKernel<kF16, 1>)
+                                           : (vector ? checkpointRestoreKernel<kBF16, 8> : checkpointRestoreKernel<kBF16, 1>);
+  const cudaError_t e = launchDependent(kernel, dim3(gridFor(l.rows * (l.cols / (vector ? vec : 1)), kThreads)), dim3(kThreads), 0, stream, l);
+  if (e == cudaSuccess && launched) *launched += 1;
+  return e;
+}
+
+} // namespace kernels
+} // namespace afir

@@ -1,6 +1,8 @@
 #include "runtime/descriptor.h"
 
 #include <algorithm>
+#include <cmath>
+#include <initializer_list>
 
 #include <cstring>
 
@@ -48,8 +50,20 @@ const char *kernelClassName(KernelClass c) {
   case KernelClass::Gather: return "gather";
   case KernelClass::Transpose: return "transpose";
   case KernelClass::Matmul: return "matmul";
+  case KernelClass::BlockNorm: return "block_norm";
+  case KernelClass::Checkpoint: return "checkpoint";
+  case KernelClass::CheckpointGrad: return "checkpoint_grad";
   }
   return "?";
+}
+
+Status evalDim(const DimExpr &e, const std::map<std::string, int64_t> &tiling, int64_t &out) {
+  if (e.literal) { out = e.value; return Status::success(); }
+  auto it = tiling.find(e.field);
+  if (it == tiling.end()) return Status::error("tiling field '" + e.field + "' is not in the kernel's TilingData");
+  out = it->second;
+  if (out < 0) return Status::error("tiling field '" + e.field + "' is negative");
+  return Status::success();
 }
 
 size_t LaunchDescriptor::tilingBytes() const {
@@ -214,6 +228,64 @@ Status parseGroup(const json::Value &g, const LaunchDescriptor &d, GroupSpec &ou
   return Status::success();
 }
 
+// One of the words of `names`; the first is the default.
+Status parseChoice(const json::Value &v, const char *key, std::initializer_list<const char *> names, int &out) {
+  const std::string word = v.getString(key, *names.begin());
+  out = 0;
+  for (const char *n : names) {
+    if (word == n) return Status::success();
+    ++out;
+  }
+  return Status::error(std::string("operator: unknown ") + key + " '" + word + "'");
+}
+
+// 'operator': the sizes, the roles of the arguments and the choices of one operator kernel.
+Status parseOperator(const json::Value &root, LaunchDescriptor &out) {
+  const json::Value *o = root.find("operator");
+  if (!o || !o->isObject()) return Status::error(std::string(kernelClassName(out.kernelClass)) + " descriptors need an 'operator' object");
+  OperatorSpec &op = out.op;
+  auto dim = [&](const char *key, bool required, DimExpr &to) -> Status {
+    const json::Value *v = o->find(key);
+    if (!v) return required ? Status::error(std::string("operator needs '") + key + "'") : Status::success();
+    return parseDim(*v, to, key);
+  };
+  op.groupRows.value = 1;
+  if (Status s = dim("rows", true, op.rows); !s) return s;
+  if (Status s = dim("cols", true, op.cols); !s) return s;
+  if (Status s = dim("out_cols", out.kernelClass == KernelClass::CheckpointGrad, op.outCols); !s) return s;
+  if (Status s = dim("group_rows", false, op.groupRows); !s) return s;
+  int direction = 0;
+  if (Status s = parseChoice(*o, "direction", {"forward", "gradient"}, direction); !s) return s;
+  op.gradient = direction == 1;
+  if (Status s = parseChoice(*o, "pass", {"pre", "post", "post_pre"}, op.pass); !s) return s;
+  if (Status s = parseChoice(*o, "kind", {"rms", "layer"}, op.kind); !s) return s;
+  if (Status s = parseChoice(*o, "gate", {"none", "token", "group"}, op.gateForm); !s) return s;
+  if (Status s = parseChoice(*o, "gate_act", {"none", "sigmoid", "tanh"}, op.gateAct); !s) return s;
+  if (!parseDType(o->getString("param_dtype", dtypeName(out.dtype)), op.paramType) ||
+      !parseDType(o->getString("out_dtype", dtypeName(out.dtype)), op.outType))
+    return Status::error("operator: unknown dtype");
+  op.alpha = o->getDouble("alpha", 1.0);
+  op.eps = o->getDouble("eps", 0.0);
+  op.nextEps = o->getDouble("next_eps", op.eps);
+  if (!std::isfinite(static_cast<float>(op.alpha))) return Status::error("operator: alpha must be finite");
+  for (double e : {op.eps, op.nextEps})
+    if (!(e >= 0.0) || !std::isfinite(static_cast<float>(e))) return Status::error("operator: eps must be finite and not negative");
+  op.accumulate = o->getBool("accumulate", false);
+  const json::Value *roles = o->find("roles");
+  if (!roles || !roles->isObject()) return Status::error("operator needs a 'roles' object");
+  std::vector<char> taken(static_cast<size_t>(out.numInputs + out.numOutputs), 0);
+  for (const auto &entry : roles->asObject()) {
+    ViewSpec v;
+    if (Status s = parseView(entry.second, out.dtype, out.numInputs + out.numOutputs, 2, false, v, entry.first.c_str()); !s) return s;
+    if (v.shape.size() > 2) return Status::error("operator: role '" + entry.first + "' has more than two dims");
+    taken[static_cast<size_t>(v.arg)] = 1;
+    op.roles[entry.first] = std::move(v);
+  }
+  for (char t : taken)
+    if (!t) return Status::error("operator: every argument needs a role");
+  return Status::success();
+}
+
 } // namespace
 
 Status parseDescriptorJson(const json::Value &root, LaunchDescriptor &out) {
@@ -231,11 +303,17 @@ Status parseDescriptorJson(const json::Value &root, LaunchDescriptor &out) {
   else if (cls == "gather") out.kernelClass = KernelClass::Gather;
   else if (cls == "transpose") out.kernelClass = KernelClass::Transpose;
   else if (cls == "matmul") out.kernelClass = KernelClass::Matmul;
+  else if (cls == "block_norm") out.kernelClass = KernelClass::BlockNorm;
+  else if (cls == "checkpoint") out.kernelClass = KernelClass::Checkpoint;
+  else if (cls == "checkpoint_grad") out.kernelClass = KernelClass::CheckpointGrad;
   else return Status::error("unknown kernel_class '" + cls + "'");
+  const bool operatorClass = out.kernelClass == KernelClass::BlockNorm || out.kernelClass == KernelClass::Checkpoint ||
+                             out.kernelClass == KernelClass::CheckpointGrad;
   if (!parseDType(root.getString("dtype", "f32"), out.dtype)) return Status::error("unknown dtype");
   out.numInputs = static_cast<int>(root.getInt("num_inputs", -1));
   out.numOutputs = static_cast<int>(root.getInt("num_outputs", -1));
-  if (out.numInputs < 0 || out.numOutputs <= 0 || out.numInputs + out.numOutputs > 16)
+  if (out.numInputs < 0 || out.numOutputs <= 0 || out.numInputs > 32 || out.numOutputs > 32 ||
+      out.numInputs + out.numOutputs > (operatorClass ? 32 : 16))
     return Status::error("invalid num_inputs/num_outputs");
 
   if (const json::Value *t = root.find("tiling")) {
@@ -305,6 +383,8 @@ Status parseDescriptorJson(const json::Value &root, LaunchDescriptor &out) {
     if (Status s = parseDim(*dk, ms.k, "matmul.k"); !s) return s;
     return Status::success();
   }
+
+  if (operatorClass) return parseOperator(root, out);
 
   if (const json::Value *gs = root.find("groups")) {
     if (!gs->isArray() || gs->asArray().empty()) return Status::error("'groups' must be a non-empty array");

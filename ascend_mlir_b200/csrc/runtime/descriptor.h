@@ -21,7 +21,7 @@ const char *dtypeName(DType t);
 bool parseDType(const std::string &s, DType &out);
 size_t dtypeBytes(DType t);
 
-enum class KernelClass { Elementwise, RowReduce, Gather, Transpose, Matmul };
+enum class KernelClass { Elementwise, RowReduce, Gather, Transpose, Matmul, BlockNorm, Checkpoint, CheckpointGrad };
 const char *kernelClassName(KernelClass c);
 
 // A dimension: an integer literal or the name of a TilingData field.
@@ -59,6 +59,20 @@ struct MatmulSpec {
   bool transposeB = false;  // B is [N, K]: out = A x B^T
 };
 
+// The row passes of a residual block, activation checkpoints and the gradient that reads one (kernels/block_norm.h).
+// `roles` names the arguments: each is a 2-D argument [rows, row length] or a vector, seen from an optional offset, so
+// a role may be a column slice of a wider tensor.
+struct OperatorSpec {
+  std::map<std::string, ViewSpec> roles;
+  DimExpr rows, cols, outCols, groupRows;  // outCols: checkpoint_grad; groupRows: gate rows that serve several rows
+  int pass = 0;           // kernels::NormPass
+  bool gradient = false;  // block_norm: the backward direction; checkpoint: restore instead of pack
+  int kind = 0, gateForm = 0, gateAct = 0;
+  DType paramType = DType::F32, outType = DType::BF16;
+  double alpha = 1.0, eps = 0.0, nextEps = 0.0;
+  bool accumulate = false;  // checkpoint_grad: add to what the output holds
+};
+
 struct TilingField {
   std::string name;
   int bytes = 8;  // int64 (8) or int32 (4), little-endian
@@ -72,6 +86,7 @@ struct LaunchDescriptor {
   std::vector<TilingField> tiling;
   std::vector<GroupSpec> groups;
   MatmulSpec matmul;
+  OperatorSpec op;
   // names of the tiling fields carrying B200 launch parameters (empty = library default)
   std::string ctaThreadsField, unrollField, splitColsField, stagesField, teamLanesField, bulkCopyField, streamStagesField, streamChunkField,
       warpRowsField, ctasPerSmField, tileKernelField, tileOrderField, variantField, streamRowsField, streamWarpsField;
@@ -106,6 +121,9 @@ struct ContainerCode {
   size_t sourceLen = 0;
 };
 ContainerCode containerCode(const uint8_t *data, size_t len);
+
+// A dimension's value at these tiling values.
+Status evalDim(const DimExpr &e, const std::map<std::string, int64_t> &tiling, int64_t &out);
 
 // Decodes packed tiling bytes (schema order, little-endian) into named values.
 Status unpackTiling(const LaunchDescriptor &d, const uint8_t *bytes, size_t len, std::map<std::string, int64_t> &out);

@@ -3,6 +3,7 @@
 #include <cuda_runtime_api.h>
 
 #include "codegen/nvrtc_compile.h"
+#include "runtime/block_norm_launch.h"
 
 #include <algorithm>
 #include <cctype>
@@ -563,6 +564,11 @@ Status CudaExecutor::launchDevice(const RunRequest &req, void *workspace, size_t
   } else {
     size_t wsBytes = 0;
     if (Status s = requiredWorkspaceBytes(*desc, tiling, device_, wsBytes); !s) return s.withStage("cuda:bindings");
+    // Scratch of an operator kernel that one executor kept for all of its launches would be shared by launches on
+    // different streams and by captured graphs: the caller owns it.
+    if (isOperatorClass(desc->kernelClass) && wsBytes > kWorkspaceStatusBytes)
+      return Status::error("[cuda:memory] kernel '" + desc->kernel + "' needs a workspace of " + std::to_string(wsBytes) +
+                           " bytes from the caller at these sizes");
     if (Status s = ownWorkspace(wsBytes); !s) return s.withStage("cuda:memory");
     args.workspace = workspace_.ptr;
     args.workspaceBytes = workspace_.capacity;

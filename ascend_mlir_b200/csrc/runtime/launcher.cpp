@@ -1,20 +1,12 @@
 #include "runtime/launcher.h"
 #include "kernels/matmul_plan.h"
+#include "runtime/block_norm_launch.h"
 
 #include <algorithm>
 #include <cstring>
 
 namespace afir {
 namespace {
-
-Status evalDim(const DimExpr &e, const std::map<std::string, int64_t> &tiling, int64_t &out) {
-  if (e.literal) { out = e.value; return Status::success(); }
-  auto it = tiling.find(e.field);
-  if (it == tiling.end()) return Status::error("tiling field '" + e.field + "' is not in the kernel's TilingData");
-  out = it->second;
-  if (out < 0) return Status::error("tiling field '" + e.field + "' is negative");
-  return Status::success();
-}
 
 Status evalDims(const std::vector<DimExpr> &es, const std::map<std::string, int64_t> &tiling, std::vector<int64_t> &out) {
   out.resize(es.size());
@@ -505,6 +497,7 @@ Status launchMatmulDescriptor(const LaunchDescriptor &d, const std::map<std::str
 
 Status requiredWorkspaceBytes(const LaunchDescriptor &d, const std::map<std::string, int64_t> &tiling, int device, size_t &bytes) {
   bytes = kWorkspaceStatusBytes;
+  if (isOperatorClass(d.kernelClass)) return operatorWorkspaceBytes(d, tiling, device, bytes);
   if (d.kernelClass != KernelClass::RowReduce) return Status::success();
   for (const auto &g : d.groups) {
     std::vector<int64_t> domain;
@@ -531,6 +524,7 @@ Status launchDescriptor(const LaunchDescriptor &d, const std::map<std::string, i
   if (!args.tableShards.empty() && (d.kernelClass != KernelClass::Gather || d.groups.size() != 1))
     return Status::error("only a single gather group takes a sharded table");
   if (d.kernelClass == KernelClass::Matmul) return launchMatmulDescriptor(d, tiling, args, info);
+  if (isOperatorClass(d.kernelClass)) return launchOperator(d, tiling, args, info);
   for (const auto &g : d.groups) {
     Status s;
     switch (d.kernelClass) {

@@ -42,6 +42,7 @@ class KernelSpec:
     shape_keys: Dict[str, str] = field(default_factory=dict)  # tiling field -> shape key
     defaults: Dict[str, int] = field(default_factory=dict)    # tile-parameter defaults
     magic: int = 0x41415246
+    derived: Dict[str, object] = field(default_factory=dict)  # shape key -> its value from the other keys
 
     def __post_init__(self):
         self.binary = container(self.descriptor)
@@ -51,7 +52,7 @@ class KernelSpec:
         values = dict(self.defaults)
         values.update(tile_params)
         for fname, key in self.shape_keys.items():
-            values[fname] = shape[key]
+            values[fname] = self.derived[key](shape) if key in self.derived and key not in shape else shape[key]
         return self.schema.pack(**values)
 
     def descriptor_json(self) -> str:
@@ -266,3 +267,247 @@ def matmul_bias_leakyrelu(in_dtype: str = "bf16", out_dtype: str = "bf16", bias_
     if transpose_b:
         body["matmul"]["transpose_b"] = True
     return _spec(name, "matmul", in_dtype, 3, 1, tile, dims, body, {"stages": "STAGES"})
+
+
+# ---- row passes of a residual block, activation checkpoints --------------------------------------------------------
+# No counterpart in the reference (it compiles inference groups).  Sizes: T rows (tokens), D columns, N output columns,
+# G rows per gate row and B = ceil(T / G) gate rows.  A tensor named in `strided` is a slice of a wider one: its size
+# keys are LD_<name> (row length) and OFF_<name> (first column), and its argument is the whole wide tensor.
+CHECKPOINT_BLOCK = 128  # columns that share one power of two
+
+
+class _Roles:
+    """Collects the arguments of an operator kernel in order: inputs, then outputs."""
+
+    def __init__(self, dtype: str, strided):
+        self.dtype, self.strided = dtype, tuple(strided)
+        self.inputs: List[tuple] = []
+        self.outputs: List[tuple] = []
+        self.dims: List[tuple] = []
+
+    def _add(self, side, role, dtype, shape):
+        side.append((role, {"dtype": dtype, "shape": list(shape)}))
+
+    def _row_shape(self, role, view):
+        if role in self.strided:
+            self.dims += [(f"ld_{role}", f"LD_{role}"), (f"off_{role}", f"OFF_{role}")]
+            view["shape"][1] = f"ld_{role}"
+            view["offset"] = [0, f"off_{role}"]
+
+    def rows(self, role, out=False, dtype=None, shape=("rows", "cols")):
+        side = self.outputs if out else self.inputs
+        self._add(side, role, dtype or self.dtype, shape)
+        self._row_shape(role, side[-1][1])
+        return self
+
+    def vector(self, role, dtype, out=False, n="cols"):
+        self._add(self.outputs if out else self.inputs, role, dtype, (n,))
+        return self
+
+    def checkpoint(self, out=False):
+        self.rows("codes", out, "u8")
+        return self.rows("exps", out, "u8", ("rows", "exp_cols"))
+
+    def spec(self, name, kernel_class, operator, dims) -> KernelSpec:
+        unknown = [s for s in self.strided if f"ld_{s}" not in [d[0] for d in self.dims]]
+        if unknown:
+            raise ValueError(f"{name}: no row tensor named {', '.join(unknown)}")
+        roles = {}
+        for i, (role, view) in enumerate(self.inputs + self.outputs):
+            roles[role] = dict(view, arg=i)
+        operator = dict(operator, rows="rows", cols="cols", roles=roles)
+        spec = _spec(name, kernel_class, self.dtype, len(self.inputs), len(self.outputs), [], list(dims) + self.dims,
+                     {"operator": operator}, {})
+        if any("exp_cols" in r["shape"] for r in roles.values()):
+            spec.derived = {"EXP_COLS": lambda shape: -(-shape["D"] // CHECKPOINT_BLOCK)}
+        return spec
+
+
+def _one_of(what, value, words):
+    if value not in words:
+        raise ValueError(f"{what} is one of {', '.join(words)}: got {value!r}")
+
+
+_ROW_DIMS = [("rows", "T"), ("cols", "D")]
+_EXP_DIMS = [("exp_cols", "EXP_COLS")]
+_FLOATS = ("f32", "f16", "bf16")
+
+
+def _block_operator(dtype, kind, param_dtype, direction, pass_, **more):
+    _one_of("dtype", dtype, _FLOATS)
+    _one_of("kind", kind, ("rms", "layer"))
+    _one_of("param_dtype", param_dtype or dtype, (dtype, "f32"))
+    return dict({"direction": direction, "pass": pass_, "kind": kind, "param_dtype": param_dtype or dtype}, **more)
+
+
+def block_norm(dtype: str = "bf16", kind: str = "rms", eps: float = 1e-6, checkpoint: bool = False, save_stats: bool = True,
+               param_dtype: Optional[str] = None, strided=(), name: str = "block_norm") -> KernelSpec:
+    """h = (x - mean) * rstd * weight [+ bias] over each row: rms (mean = 0, no bias) or layer norm.
+
+    Inputs: x [T, D], weight [D] (, bias [D]).  Outputs: h [T, D] (, rstd [T] f32 (, mean [T] f32)) (, codes [T, D] u8,
+    exps [T, ceil(D/128)] u8).  With `checkpoint` x is also kept in 8 bits, in the same pass; `save_stats` leaves the
+    statistics for block_norm_grad.  Statistics are f32.  D up to 16384."""
+    op_ = _block_operator(dtype, kind, param_dtype, "forward", "pre", eps=eps)
+    layer, pt = kind == "layer", param_dtype or dtype
+    r = _Roles(dtype, strided).rows("x").vector("weight", pt)
+    if layer:
+        r.vector("bias", pt)
+    r.rows("h", out=True)
+    if save_stats:
+        r.vector("rstd", "f32", True, "rows")
+        if layer:
+            r.vector("mean", "f32", True, "rows")
+    if checkpoint:
+        r.checkpoint(out=True)
+    return r.spec(name, "block_norm", op_, _ROW_DIMS + (_EXP_DIMS if checkpoint else []))
+
+
+def block_norm_grad(dtype: str = "bf16", kind: str = "rms", checkpoint: bool = False, residual_grad: bool = False,
+                    param_dtype: Optional[str] = None, strided=(), name: str = "block_norm_grad") -> KernelSpec:
+    """Gradients of block_norm from dh: dx = rstd*(dn - n*avg(dn*n) [- avg(dn)]) (+ dout), dn = dh*weight.
+
+    Inputs: dh [T, D], x [T, D] (with `checkpoint`: codes, exps instead), weight, rstd (, mean) (, dout [T, D]: with
+    `residual_grad`, the gradient of x's other uses, added to dx).  Outputs: dx [T, D], dweight [D] f32 (, dbias [D] f32).
+    Needs a workspace (workspace_bytes).  The sums over the rows are added in a fixed order."""
+    op_ = _block_operator(dtype, kind, param_dtype, "gradient", "pre")
+    layer, pt = kind == "layer", param_dtype or dtype
+    r = _Roles(dtype, strided).rows("dh")
+    r.checkpoint() if checkpoint else r.rows("x")
+    r.vector("weight", pt).vector("rstd", "f32", n="rows")
+    if layer:
+        r.vector("mean", "f32", n="rows")
+    if residual_grad:
+        r.rows("dout")
+    r.rows("dx", out=True).vector("dweight", "f32", True)
+    if layer:
+        r.vector("dbias", "f32", True)
+    return r.spec(name, "block_norm", op_, _ROW_DIMS + (_EXP_DIMS if checkpoint else []))
+
+
+_GATE_DIMS = [("group_rows", "G"), ("gate_rows", "B")]
+
+
+def _gate_fields(gate, gate_act, alpha):
+    _one_of("gate", gate, ("none", "token", "group"))
+    _one_of("gate_act", gate_act, ("none", "sigmoid", "tanh"))
+    fields = {"gate": gate, "gate_act": gate_act, "alpha": alpha}
+    if gate == "group":
+        fields["group_rows"] = "group_rows"
+    return fields, (_GATE_DIMS if gate == "group" else [])
+
+
+def gated_residual(dtype: str = "bf16", kind: str = "rms", eps: float = 1e-6, alpha: float = 1.0, gate: str = "none",
+                   gate_act: str = "none", scale: bool = True, next_norm: bool = False, next_eps: Optional[float] = None,
+                   checkpoint: bool = False, save_stats: bool = True, param_dtype: Optional[str] = None, strided=(),
+                   name: str = "gated_residual") -> KernelSpec:
+    """out = alpha*x + scale * act(gate) * (norm(y)*weight [+ bias]); with `next_norm` also h = norm(out)*next_weight [+ next_bias].
+
+    x is the residual stream, y a block's output.  gate: "token" a value per element [T, D]; "group" one row [B, D] for
+    every G rows (a sequence, say; the last group may be short).  Inputs: x, y, weight (, bias) (, gate) (, scale [D])
+    (, next_weight (, next_bias)).  Outputs: out (, rstd (, mean)) (, h (, next_rstd (, next_mean))) (, codes, exps of y).
+    The next norm reads `out` as it is stored.  `out` or `h` may take the place of x, y or a token gate."""
+    fields, gate_dims = _gate_fields(gate, gate_act, alpha)
+    op_ = _block_operator(dtype, kind, param_dtype, "forward", "post_pre" if next_norm else "post", eps=eps,
+                          next_eps=eps if next_eps is None else next_eps, **fields)
+    layer, pt = kind == "layer", param_dtype or dtype
+    r = _Roles(dtype, strided).rows("x").rows("y").vector("weight", pt)
+    if layer:
+        r.vector("bias", pt)
+    if gate != "none":
+        r.rows("gate", shape=("rows", "cols") if gate == "token" else ("gate_rows", "cols"))
+    if scale:
+        r.vector("scale", pt)
+    if next_norm:
+        r.vector("next_weight", pt)
+        if layer:
+            r.vector("next_bias", pt)
+    r.rows("out", out=True)
+    if save_stats:
+        r.vector("rstd", "f32", True, "rows")
+        if layer:
+            r.vector("mean", "f32", True, "rows")
+    if next_norm:
+        r.rows("h", out=True)
+        if save_stats:
+            r.vector("next_rstd", "f32", True, "rows")
+            if layer:
+                r.vector("next_mean", "f32", True, "rows")
+    if checkpoint:
+        r.checkpoint(out=True)
+    return r.spec(name, "block_norm", op_, _ROW_DIMS + gate_dims + (_EXP_DIMS if checkpoint else []))
+
+
+def gated_residual_grad(dtype: str = "bf16", kind: str = "rms", alpha: float = 1.0, gate: str = "none", gate_act: str = "none",
+                        scale: bool = True, next_norm: bool = False, checkpoint: bool = False, param_dtype: Optional[str] = None,
+                        strided=(), name: str = "gated_residual_grad") -> KernelSpec:
+    """Gradients of gated_residual from dout (the stream's later uses) and, with `next_norm`, dh.
+
+    Inputs: dout, y (with `checkpoint`: codes, exps), weight (, bias) (, gate) (, scale), rstd (, mean) (, dh, out,
+    next_weight, next_rstd (, next_mean)).  Outputs: dx, dy, dweight [D] f32 (, dbias f32) (, dgate: "token" [T, D], "group"
+    [B, D] f32) (, dscale f32) (, dnext_weight f32 (, dnext_bias f32)).  Needs a workspace (workspace_bytes)."""
+    fields, gate_dims = _gate_fields(gate, gate_act, alpha)
+    op_ = _block_operator(dtype, kind, param_dtype, "gradient", "post_pre" if next_norm else "post", **fields)
+    layer, pt = kind == "layer", param_dtype or dtype
+    gate_shape = ("rows", "cols") if gate == "token" else ("gate_rows", "cols")
+    r = _Roles(dtype, strided).rows("dout")
+    r.checkpoint() if checkpoint else r.rows("y")
+    r.vector("weight", pt)
+    if layer:
+        r.vector("bias", pt)
+    if gate != "none":
+        r.rows("gate", shape=gate_shape)
+    if scale:
+        r.vector("scale", pt)
+    r.vector("rstd", "f32", n="rows")
+    if layer:
+        r.vector("mean", "f32", n="rows")
+    if next_norm:
+        r.rows("dh").rows("out").vector("next_weight", pt).vector("next_rstd", "f32", n="rows")
+        if layer:
+            r.vector("next_mean", "f32", n="rows")
+    r.rows("dx", out=True).rows("dy", out=True).vector("dweight", "f32", True)
+    if layer:
+        r.vector("dbias", "f32", True)
+    if gate != "none":
+        r.rows("dgate", out=True, dtype=dtype if gate == "token" else "f32", shape=gate_shape)
+    if scale:
+        r.vector("dscale", "f32", True)
+    if next_norm:
+        r.vector("dnext_weight", "f32", True)
+        if layer:
+            r.vector("dnext_bias", "f32", True)
+    return r.spec(name, "block_norm", op_, _ROW_DIMS + gate_dims + (_EXP_DIMS if checkpoint else []))
+
+
+def checkpoint_pack(dtype: str = "bf16", strided=(), name: str = "checkpoint_pack") -> KernelSpec:
+    """An activation in 8 bits: value = e4m3(code) * 2^(exp - 127), one exponent per row and 128 columns.
+
+    Inputs: x [T, D].  Outputs: codes [T, D] u8, exps [T, ceil(D/128)] u8.  The power is the smallest that brings the
+    block's largest finite magnitude to 448 or less, kept where the restored value is exact in `dtype`; infinities and NaN
+    become NaN."""
+    _one_of("dtype", dtype, _FLOATS)
+    r = _Roles(dtype, strided).rows("x").checkpoint(out=True)
+    return r.spec(name, "checkpoint", {"direction": "forward"}, _ROW_DIMS + _EXP_DIMS)
+
+
+def checkpoint_restore(dtype: str = "bf16", strided=(), name: str = "checkpoint_restore") -> KernelSpec:
+    """The values of a checkpoint made from `dtype`.  Inputs: codes, exps.  Outputs: x [T, D]."""
+    _one_of("dtype", dtype, _FLOATS)
+    r = _Roles(dtype, strided).checkpoint().rows("x", out=True)
+    return r.spec(name, "checkpoint", {"direction": "gradient"}, _ROW_DIMS + _EXP_DIMS)
+
+
+def checkpoint_weight_grad(dtype: str = "bf16", out_dtype: Optional[str] = None, accumulate: bool = False, strided=(),
+                           name: str = "checkpoint_weight_grad") -> KernelSpec:
+    """dweight [D, N] = x^T dy of a linear layer y = x weight whose input x [T, D] was kept as a checkpoint.
+
+    Inputs: codes, exps (made from `dtype`), dy [T, N] in `dtype` (f16 or bf16).  Outputs: dweight in `out_dtype` (f32 or
+    `dtype`); with `accumulate` the product is added to what dweight holds.  The restored x is exact in `dtype`, products
+    are summed in f32.  Needs a workspace (workspace_bytes).  D a multiple of 16, N of 8, as are strided row lengths and
+    offsets."""
+    _one_of("dtype", dtype, ("f16", "bf16"))
+    _one_of("out_dtype", out_dtype or dtype, (dtype, "f32"))
+    r = _Roles(dtype, strided).checkpoint().rows("dy", shape=("rows", "out_cols"))
+    r.rows("dweight", out=True, dtype=out_dtype or dtype, shape=("cols", "out_cols"))
+    return r.spec(name, "checkpoint_grad", {"out_cols": "out_cols", "out_dtype": out_dtype or dtype, "accumulate": accumulate},
+                  _ROW_DIMS + [("out_cols", "N")] + _EXP_DIMS)
