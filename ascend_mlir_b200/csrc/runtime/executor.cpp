@@ -3,7 +3,6 @@
 #include <cuda_runtime_api.h>
 
 #include "codegen/nvrtc_compile.h"
-#include "runtime/block_norm_launch.h"
 
 #include <algorithm>
 #include <cctype>

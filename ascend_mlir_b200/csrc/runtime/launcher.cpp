@@ -1,6 +1,6 @@
 #include "runtime/launcher.h"
+#include "kernels/block_norm.h"
 #include "kernels/matmul_plan.h"
-#include "runtime/block_norm_launch.h"
 
 #include <algorithm>
 #include <cstring>
@@ -846,3 +846,5 @@ Status planRowPipeline(const LaunchDescriptor &d, const std::map<std::string, in
 }
 
 } // namespace afir
+
+#include "runtime/operator_launch.inc"

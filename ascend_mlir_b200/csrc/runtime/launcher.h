@@ -70,6 +70,13 @@ Status planRowPipeline(const LaunchDescriptor &d, const std::map<std::string, in
 Status launchDescriptor(const LaunchDescriptor &d, const std::map<std::string, int64_t> &tiling, const LaunchArgs &args,
                         LaunchInfo &info);
 
+// ---- operator kernels ------------------------------------------------------------------------------------------
+inline bool isOperatorClass(KernelClass c) {
+  return c == KernelClass::BlockNorm || c == KernelClass::Checkpoint || c == KernelClass::CheckpointGrad;
+}
+Status operatorWorkspaceBytes(const LaunchDescriptor &d, const std::map<std::string, int64_t> &tiling, int device, size_t &bytes);
+Status launchOperator(const LaunchDescriptor &d, const std::map<std::string, int64_t> &tiling, const LaunchArgs &args, LaunchInfo &info);
+
 // ---- generated kernels -------------------------------------------------------------------------------------------
 // The kernel generated for one descriptor (codegen/kernel_source), loaded on one device.
 struct GeneratedBinding {
