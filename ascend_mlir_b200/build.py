@@ -45,6 +45,7 @@ CU_SOURCES = {
     "kernels/block_norm_grad_f16.cu": [],
     "kernels/block_norm_grad_bf16.cu": [],
     "kernels/checkpoint.cu": [],
+    "kernels/checkpoint_grad_tcgen05.cu": [],
 }
 CPP_SOURCES = ["common/json.cpp", "kernels/matmul_plan.cpp", "kernels/body_match.cpp", "codegen/kernel_source.cpp",
                "codegen/nvrtc_compile.cpp", "codegen/embedded_headers.cpp", "runtime/device_module.cpp", "runtime/caller_device.cpp", "runtime/host_staging.cpp", "runtime/descriptor.cpp", "runtime/launcher.cpp", "runtime/executor.cpp",

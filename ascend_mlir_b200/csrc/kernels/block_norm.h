@@ -96,5 +96,21 @@ struct CheckpointRestoreLaunch {
 };
 int launchCheckpointRestore(const CheckpointRestoreLaunch &l, cudaStream_t stream, int *launched);
 
+// dweight[cols, outCols] = restore(in)[rows, cols]^T . dy[rows, outCols]  (checkpoint_grad_tcgen05.cu)
+struct CheckpointGradLaunch {
+  int elemType;                // of dy, and what the checkpoint was made from: kF16 or kBF16
+  int outType;                 // elemType or kF32
+  int64_t rows, cols, outCols;
+  CheckpointIn in;
+  RowsIn dy;
+  RowsOut out;
+  int accumulate;              // add to what `out` (f32) holds
+  unsigned int *status;        // device word for a pipeline wait that ran out
+  void *workspace;
+  size_t workspaceBytes;
+};
+size_t checkpointGradWorkspaceBytes(int64_t cols, int64_t outCols, int64_t rows, int smCount);
+int launchCheckpointGrad(const CheckpointGradLaunch &l, cudaStream_t stream, int *launched, char *errorText);
+
 } // namespace kernels
 } // namespace afir

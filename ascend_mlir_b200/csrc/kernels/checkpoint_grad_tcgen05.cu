@@ -1,0 +1,485 @@
+// Weight gradient from an 8-bit checkpoint, for sm_100a:
+//     dweight[D, N] = restore(codes, exps)[T, D]^T . dy[T, N]
+// The restored activation never exists in HBM: codes come in by TMA (one byte per element), are widened in the SM to the
+// 16-bit type of dy, which is exact (four significant bits times a power of two), and go to the tensor cores from shared
+// memory.
+//
+//   warp 0      TMA producer: codes [64 tokens x TM] and dy [64 tokens x 256] into a ring of stages;
+//   warp 1      MMA issuer: tcgen05.mma.cta_group::1.kind::f16, 128 x 256 x 16, both operands with their long side
+//               contiguous (tokens are the summed dimension and the rows of both tensors);
+//   warps 2..9  convert a stage's codes into the A operand (a ring of two tiles, 128-byte swizzle), and write the
+//               finished tile out: tcgen05.ld, convert, 16-byte stores that cover whole 128-byte lines.
+// TM = 128 * MB rows of dweight per CTA; MB = 2 halves what dy costs per flop.  One persistent CTA per SM.  Where the
+// tiles of dweight are fewer than the SMs the tokens are cut into slices whose partial tiles (f32) a second kernel adds in order.
+//
+// Every wait on an mbarrier is bounded, as in matmul_tcgen05.cu: after about 2 s a status word is set, every role leaves
+// its loop, copies in flight are waited for (bounded), tensor memory is freed and the kernel returns.
+#include <algorithm>
+#include <cstdio>
+
+#include "kernels/block_norm.h"
+#include "kernels/block_norm_device.cuh"
+#include "kernels/launch_util.h"
+#include "kernels/tcgen05_device.cuh"
+
+namespace afir {
+namespace kernels {
+namespace {
+
+constexpr int kTileN = 256;
+constexpr int kTokens = 64;                      // summed per stage
+constexpr int kCodeBoxBytes = kTokens * 128;     // 64 tokens x 128 columns of codes
+constexpr int kBlockBytes = kTokens * 64 * 2;    // 64 tokens x 64 columns of a 16-bit operand
+constexpr int kBStage = 4 * kBlockBytes;
+constexpr int kConvertWarps = 8;
+constexpr int kThreads = 64 + 32 * kConvertWarps;
+constexpr int kATiles = 2;
+
+template <int MB> struct GradShape {
+  static constexpr int kTileM = 128 * MB;
+  static constexpr int kCodeStage = MB * kCodeBoxBytes;
+  static constexpr int kStageBytes = kCodeStage + kBStage;
+  static constexpr int kStages = MB == 1 ? 4 : 3;
+  static constexpr int kATileBytes = MB * 2 * kBlockBytes;
+  static constexpr int kTmemCols = MB * kTileN;
+  static constexpr size_t kRing = static_cast<size_t>(kStages) * kStageBytes;
+  static_assert(kATiles * kATileBytes >= kConvertWarps * 4096, "the A tiles double as the staging area of the output");
+};
+template <int MB> struct GradControl {
+  unsigned long long full[GradShape<MB>::kStages], empty[GradShape<MB>::kStages];
+  unsigned long long aFull[kATiles], aEmpty[kATiles];
+  unsigned long long tileFull, tileEmpty;
+  unsigned int tmemBase;
+  AbortState abort;
+};
+template <int MB> constexpr size_t gradSmemBytes() { return 1024 + GradShape<MB>::kRing + kATiles * GradShape<MB>::kATileBytes + sizeof(GradControl<MB>); }
+
+struct GradParams {
+  int D, N, T;
+  int tilesM, tilesN, kBlocks, splits, kPerSplit, band;
+  const uint8_t *exps;
+  int64_t expsLd;
+  int expCols;
+  void *out;       // dweight, or the partial tiles [splits][D][N] f32
+  int64_t outLd;
+  int64_t splitStride;
+  int accumulate;
+  unsigned int idesc;
+  unsigned int *status;
+};
+
+// 16 codes -> 16 values of the operand type, times the power.
+template <int ELEM> __device__ __forceinline__ void widenCodes(const uint4 &raw, int exponent, uint4 (&out)[2]) {
+  const unsigned int w[4] = {raw.x, raw.y, raw.z, raw.w};
+  unsigned int r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const unsigned int pair = (w[i >> 1] >> ((i & 1) * 16)) & 0xffffu;
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(pair), __NV_E4M3);
+    const __half2 v = *reinterpret_cast<const __half2 *>(&h);
+    if constexpr (ELEM == kF16) {
+      // the power as f16: 2^-15 (a subnormal) to 2^8, exact, and so is the product
+      const __half p = __float2half_rn(powerOfExponent(exponent));
+      const __half2 m = __hmul2(v, __halves2half2(p, p));
+      r[i] = *reinterpret_cast<const unsigned int *>(&m);
+    } else {
+      const float p = powerOfExponent(exponent);
+      const float2 f = __half22float2(v);
+      const __nv_bfloat162 m = __floats2bfloat162_rn(f.x * p, f.y * p);
+      r[i] = *reinterpret_cast<const unsigned int *>(&m);
+    }
+  }
+  out[0] = make_uint4(r[0], r[1], r[2], r[3]);
+  out[1] = make_uint4(r[4], r[5], r[6], r[7]);
+}
+
+__device__ __forceinline__ uint4 addF32(const uint4 &a, const uint4 &b) {
+  return make_uint4(__float_as_uint(__uint_as_float(a.x) + __uint_as_float(b.x)), __float_as_uint(__uint_as_float(a.y) + __uint_as_float(b.y)),
+                    __float_as_uint(__uint_as_float(a.z) + __uint_as_float(b.z)), __float_as_uint(__uint_as_float(a.w) + __uint_as_float(b.w)));
+}
+
+template <int ELEM, int OUT, int MB>
+__global__ void __launch_bounds__(kThreads, 1)
+checkpointGradKernel(const __grid_constant__ CUtensorMap mapCodes, const __grid_constant__ CUtensorMap mapDy, const __grid_constant__ GradParams prm) {
+  using S = GradShape<MB>;
+  constexpr int STAGES = S::kStages;
+  extern __shared__ unsigned char smemRaw[];
+  unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smemRaw) + 1023) & ~uintptr_t(1023));
+  unsigned char *aTiles = smem + S::kRing;
+  GradControl<MB> *ctl = reinterpret_cast<GradControl<MB> *>(aTiles + kATiles * S::kATileBytes);
+  volatile AbortState *abortFlag = &ctl->abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tiles = prm.tilesM * prm.tilesN, units = tiles * prm.splits;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbarInit(smemAddr(&ctl->full[s]), 1);
+      mbarInit(smemAddr(&ctl->empty[s]), 1);
+    }
+    for (int a = 0; a < kATiles; ++a) {
+      mbarInit(smemAddr(&ctl->aFull[a]), kConvertWarps);
+      mbarInit(smemAddr(&ctl->aEmpty[a]), 1);
+    }
+    mbarInit(smemAddr(&ctl->tileFull), 1);
+    mbarInit(smemAddr(&ctl->tileEmpty), kConvertWarps);
+    ctl->abort.flag = 0;
+    ctl->abort.status = prm.status;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    prefetchTensorMap(&mapCodes);
+    prefetchTensorMap(&mapDy);
+  }
+  if (warp == 1) {
+    tmemAlloc(smemAddr(&ctl->tmemBase), S::kTmemCols);
+    tmemRelinquish();
+  }
+  tcgen05FenceBefore();
+  __syncthreads();
+  tcgen05FenceAfter();
+  const unsigned int tmemBase = ctl->tmemBase;
+
+  // Slices outermost; inside, bands of tile-rows with the rows fastest, so that CTAs running together share operands in L2.
+  auto unitCoords = [&](int u, int &tm, int &tn, int &k0, int &k1, int &split) {
+    split = u / tiles;
+    const int t = u - split * tiles;
+    const int bandTiles = prm.band * prm.tilesN;
+    const int band = t / bandTiles, within = t - band * bandTiles;
+    const int rowsInBand = min(prm.band, prm.tilesM - band * prm.band);
+    tm = band * prm.band + within % rowsInBand;
+    tn = within / rowsInBand;
+    k0 = split * prm.kPerSplit;
+    k1 = min(prm.kBlocks, k0 + prm.kPerSplit);
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      unsigned int it = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        int tm, tn, k0, k1, split;
+        unitCoords(u, tm, tn, k0, k1, split);
+        for (int kb = k0; kb < k1; ++kb, ++it) {
+          const int s = it % STAGES;
+          if (!mbarWait(smemAddr(&ctl->empty[s]), ((it / STAGES) & 1u) ^ 1u, abortFlag, 0)) { ok = false; break; }
+          const unsigned int full = smemAddr(&ctl->full[s]);
+          mbarExpectTx(full, S::kStageBytes);
+          unsigned char *stage = smem + static_cast<size_t>(s) * S::kStageBytes;
+#pragma unroll
+          for (int h = 0; h < MB; ++h) tmaLoad2d(smemAddr(stage + h * kCodeBoxBytes), &mapCodes, tm * S::kTileM + h * 128, kb * kTokens, full);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) tmaLoad2d(smemAddr(stage + S::kCodeStage + j * kBlockBytes), &mapDy, tn * kTileN + j * 64, kb * kTokens, full);
+        }
+      }
+      if (!ok) {
+        // loads already issued still land in this CTA's shared memory: give them time before leaving
+        for (int s = 0; s < STAGES; ++s) {
+          const unsigned long long t0 = globalTimerNs();
+          while (!mbarTryWait(smemAddr(&ctl->full[s]), 0) && !mbarTryWait(smemAddr(&ctl->full[s]), 1) && globalTimerNs() - t0 < 1000000ull) {
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      unsigned int it = 0, unit = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++unit) {
+        int tm, tn, k0, k1, split;
+        unitCoords(u, tm, tn, k0, k1, split);
+        if (!mbarWait(smemAddr(&ctl->tileEmpty), (unit & 1u) ^ 1u, abortFlag, 1)) break;
+        tcgen05FenceAfter();
+        for (int kb = k0; kb < k1; ++kb, ++it) {
+          const int s = it % STAGES, a = it % kATiles;
+          // dy's copy and the converted codes: each is waited for where it becomes visible to the tensor cores
+          if (!mbarWait(smemAddr(&ctl->full[s]), (it / STAGES) & 1u, abortFlag, 1) ||
+              !mbarWait(smemAddr(&ctl->aFull[a]), (it / kATiles) & 1u, abortFlag, 1)) { ok = false; break; }
+          tcgen05FenceAfter();
+          const unsigned int aBase = smemAddr(aTiles + a * S::kATileBytes);
+          const unsigned int bBase = smemAddr(smem + static_cast<size_t>(s) * S::kStageBytes + S::kCodeStage);
+#pragma unroll
+          for (int h = 0; h < MB; ++h) {
+            const unsigned int dTmem = tmemBase + static_cast<unsigned int>(h * kTileN);
+#pragma unroll
+            for (int k = 0; k < kTokens / 16; ++k) {
+              // 64-column blocks 8192 bytes apart (leading), groups of 8 tokens 1024 bytes apart (stride)
+              const unsigned long long aDesc = smemDesc(aBase + h * 2 * kBlockBytes + k * (16 * 128), kBlockBytes, 1024);
+              const unsigned long long bDesc = smemDesc(bBase + k * (16 * 128), kBlockBytes, 1024);
+              ummaF16(dTmem, aDesc, bDesc, prm.idesc, (kb > k0 || k > 0) ? 1u : 0u);
+            }
+          }
+          ummaCommit(smemAddr(&ctl->empty[s]));
+          ummaCommit(smemAddr(&ctl->aEmpty[a]));
+        }
+        if (!ok) break;
+        ummaCommit(smemAddr(&ctl->tileFull));
+      }
+    }
+  } else {
+    const int cw = warp - 2;
+    constexpr int kSteps = MB * (kTokens / 4) / kConvertWarps;  // 4 tokens x 128 columns per warp and step
+    const int half = MB == 2 ? cw & 1 : 0;                      // which 128 columns of the tile
+    const int tokenBase = (MB == 2 ? cw >> 1 : cw) * (kSteps * 4) + (lane >> 3);
+    const int piece = lane & 7;                                 // 16 columns of the 128
+    const int quarter = warp & 3;
+    unsigned int it = 0, unit = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++unit) {
+      int tm, tn, k0, k1, split;
+      unitCoords(u, tm, tn, k0, k1, split);
+      const int expCol = tm * MB + half;
+      const bool expLive = expCol < prm.expCols;
+      int exps[kSteps];
+      auto loadExps = [&](int kb) {
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+          const int token = kb * kTokens + tokenBase + j * 4;
+          exps[j] = expLive && token < prm.T ? __ldg(prm.exps + static_cast<int64_t>(token) * prm.expsLd + expCol) : 127;  // codes beyond are 0
+        }
+      };
+      loadExps(k0);
+      for (int kb = k0; kb < k1; ++kb, ++it) {
+        const int s = it % STAGES, a = it % kATiles;
+        const bool ready = mbarWait(smemAddr(&ctl->full[s]), (it / STAGES) & 1u, abortFlag, 3) &&
+                           mbarWait(smemAddr(&ctl->aEmpty[a]), ((it / kATiles) & 1u) ^ 1u, abortFlag, 3);
+        if (!__all_sync(0xffffffffu, ready)) { ok = false; break; }
+        const unsigned char *codes = smem + static_cast<size_t>(s) * S::kStageBytes + half * kCodeBoxBytes;
+        unsigned char *block = aTiles + a * S::kATileBytes + (half * 2 + (piece >> 2)) * kBlockBytes;
+        uint4 raw[kSteps];
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) raw[j] = *reinterpret_cast<const uint4 *>(codes + (tokenBase + j * 4) * 128 + piece * 16);
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+          const int token = tokenBase + j * 4;
+          uint4 v[2];
+          widenCodes<ELEM>(raw[j], exps[j], v);
+          // eight lanes write one token's 128 columns, two 64-column blocks: those of the second block write their upper
+          // half first, so that the eight 16-byte pieces of each store fall on different banks
+          const int first = piece >> 2, at = (piece & 3) * 2;
+          unsigned char *row = block + token * 128;
+          *reinterpret_cast<uint4 *>(row + (((at + first) ^ (token & 7)) << 4)) = first ? v[1] : v[0];
+          *reinterpret_cast<uint4 *>(row + (((at + 1 - first) ^ (token & 7)) << 4)) = first ? v[0] : v[1];
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbarArrive(smemAddr(&ctl->aFull[a]));
+        if (kb + 1 < k1) loadExps(kb + 1);
+      }
+      if (!ok) break;
+
+      // ---- the finished tile: warps 0..3 of the eight take the lower half (of its rows for MB = 2, of its columns for
+      // MB = 1), 4..7 the upper; the A tiles are free (every MMA has completed) and serve as staging
+      if (!__all_sync(0xffffffffu, mbarWait(smemAddr(&ctl->tileFull), unit & 1u, abortFlag, 2))) break;
+      tcgen05FenceAfter();
+      unsigned char *stg = aTiles + cw * 4096;
+      const int upper = cw >> 2;
+      const int rowBase = tm * S::kTileM + (MB == 2 ? upper * 128 : 0) + quarter * 32;
+      const int colBegin = MB == 2 ? 0 : upper * 128, colEnd = MB == 2 ? kTileN : colBegin + 128;
+      const unsigned int taddr = tmemBase + static_cast<unsigned int>(MB == 2 ? upper * kTileN : 0) + (static_cast<unsigned int>(quarter * 32) << 16);
+      constexpr int kColsPerSlice = 128 / OutPack<OUT>::kBytes;
+      unsigned char *out = static_cast<unsigned char *>(prm.out) + static_cast<size_t>(split) * prm.splitStride * OutPack<OUT>::kBytes;
+#pragma unroll 1
+      for (int c = colBegin; c < colEnd; c += kColsPerSlice) {
+        if (tn * kTileN + c >= prm.N) break;
+#pragma unroll
+        for (int part = 0; part < kColsPerSlice / 32; ++part) {
+          unsigned int r[32];
+          tmemLoad32(taddr + c + part * 32, r);
+          tmemLoadWait();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r[j * 8 + e]);
+            uint4 q[OutPack<OUT>::kPieces];
+            OutPack<OUT>::pack8(v, q);
+#pragma unroll
+            for (int p = 0; p < OutPack<OUT>::kPieces; ++p) {
+              const int at = (part * 4 + j) * OutPack<OUT>::kPieces + p;
+              *reinterpret_cast<uint4 *>(stg + lane * 128 + ((at ^ (lane & 7)) << 4)) = q[p];
+            }
+          }
+        }
+        __syncwarp();
+        const int col = tn * kTileN + c + piece * (16 / OutPack<OUT>::kBytes);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int rr = i * 4 + (lane >> 3), row = rowBase + rr;
+          uint4 val = *reinterpret_cast<const uint4 *>(stg + rr * 128 + ((piece ^ (rr & 7)) << 4));
+          if (row < prm.D && col < prm.N) {  // N is a multiple of 8: a 16-byte piece is wholly inside or outside
+            uint4 *to = reinterpret_cast<uint4 *>(out + (static_cast<size_t>(row) * prm.outLd + col) * OutPack<OUT>::kBytes);
+            if constexpr (OUT == kF32) {
+              if (prm.accumulate) val = addF32(*to, val);
+            }
+            *to = val;
+          }
+        }
+        __syncwarp();
+      }
+      tcgen05FenceBefore();
+      __syncwarp();
+      if (lane == 0) mbarArrive(smemAddr(&ctl->tileEmpty));
+      // nobody converts into the A tiles while another warp still reads its staging there
+      if (!__all_sync(0xffffffffu, mbarWait(smemAddr(&ctl->tileEmpty), unit & 1u, abortFlag, 3))) break;
+    }
+  }
+
+  tcgen05FenceBefore();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05FenceAfter();
+    tmemDealloc(tmemBase, S::kTmemCols);
+  }
+}
+
+// The slices' partial tiles, added in slice order; 4 columns per thread.
+template <int OUT>
+__global__ void __launch_bounds__(256) checkpointGradJoinKernel(const float *partial, int splits, int64_t rows, int cols, void *out, int64_t outLd, int accumulate) {
+  const int64_t perRow = cols / 4;
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < rows * perRow; u += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = u / perRow;
+    const int col = static_cast<int>(u - row * perRow) * 4;
+    float4 sum = *reinterpret_cast<const float4 *>(partial + row * cols + col);
+    for (int s = 1; s < splits; ++s) {
+      const float4 f = *reinterpret_cast<const float4 *>(partial + (s * rows + row) * cols + col);
+      sum.x += f.x;
+      sum.y += f.y;
+      sum.z += f.z;
+      sum.w += f.w;
+    }
+    if constexpr (OUT == kF32) {
+      float4 *to = reinterpret_cast<float4 *>(static_cast<float *>(out) + row * outLd + col);
+      if (accumulate) {
+        const float4 f = *to;
+        sum = make_float4(sum.x + f.x, sum.y + f.y, sum.z + f.z, sum.w + f.w);
+      }
+      *to = sum;
+    } else {
+      const float v[8] = {sum.x, sum.y, sum.z, sum.w, 0.f, 0.f, 0.f, 0.f};
+      uint4 q[1];
+      OutPack<OUT>::pack8(v, q);
+      *reinterpret_cast<uint2 *>(static_cast<unsigned short *>(out) + row * outLd + col) = make_uint2(q[0].x, q[0].y);
+    }
+  }
+}
+
+struct SplitPlan { int mb, tilesM, tilesN, kBlocks, splits, kPerSplit; };
+
+// 256-row tiles where they keep at least half of the SMs busy (each moves half of dy's bytes per flop), else 128-row
+// tiles; tokens cut into slices where the tiles leave SMs idle and a slice still has work for its ring.
+SplitPlan splitPlan(int64_t D, int64_t N, int64_t T, int smCount) {
+  SplitPlan p = {};
+  const int64_t tilesN = (N + kTileN - 1) / kTileN;
+  p.mb = 2 * ((D + 255) / 256) * tilesN >= smCount ? 2 : 1;
+  p.tilesM = static_cast<int>((D + 128 * p.mb - 1) / (128 * p.mb));
+  p.tilesN = static_cast<int>(tilesN);
+  p.kBlocks = static_cast<int>((T + kTokens - 1) / kTokens);
+  const int64_t tiles = static_cast<int64_t>(p.tilesM) * p.tilesN;
+  int64_t splits = std::max<int64_t>(1, std::min<int64_t>(smCount / std::max<int64_t>(1, tiles), p.kBlocks / 8));
+  p.kPerSplit = static_cast<int>((p.kBlocks + splits - 1) / splits);
+  p.splits = p.kPerSplit > 0 ? (p.kBlocks + p.kPerSplit - 1) / p.kPerSplit : 1;
+  return p;
+}
+
+void gradFail(char *errorText, const char *msg) {
+  if (errorText) std::snprintf(errorText, 256, "%s", msg);
+}
+
+template <int ELEM, int OUT, int MB>
+int launchGradVariant(const CUtensorMap &codes, const CUtensorMap &dy, const GradParams &p, int grid, cudaStream_t stream) {
+  auto kernel = checkpointGradKernel<ELEM, OUT, MB>;
+  static PerDeviceOnce reserved;
+  const cudaError_t e = reserved.run([&] {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(gradSmemBytes<MB>()));
+  });
+  if (e != cudaSuccess) return e;
+  return launchOrdinary(kernel, dim3(static_cast<unsigned int>(grid)), dim3(kThreads), gradSmemBytes<MB>(), stream, codes, dy, p);
+}
+template <int ELEM> int launchGradTyped(int out, int mb, const CUtensorMap &codes, const CUtensorMap &dy, const GradParams &p, int grid, cudaStream_t stream) {
+  if (out == kF32)
+    return mb == 2 ? launchGradVariant<ELEM, kF32, 2>(codes, dy, p, grid, stream) : launchGradVariant<ELEM, kF32, 1>(codes, dy, p, grid, stream);
+  return mb == 2 ? launchGradVariant<ELEM, ELEM, 2>(codes, dy, p, grid, stream) : launchGradVariant<ELEM, ELEM, 1>(codes, dy, p, grid, stream);
+}
+
+} // namespace
+
+size_t checkpointGradWorkspaceBytes(int64_t cols, int64_t outCols, int64_t rows, int smCount) {
+  const SplitPlan p = splitPlan(cols, outCols, rows, smCount);
+  return p.splits > 1 ? static_cast<size_t>(p.splits) * static_cast<size_t>(cols) * static_cast<size_t>(outCols) * sizeof(float) : 0;
+}
+
+int launchCheckpointGrad(const CheckpointGradLaunch &l, cudaStream_t stream, int *launched, char *errorText) {
+  if (launched) *launched = 0;
+  if (l.cols == 0 || l.outCols == 0) return 0;
+  const int64_t ob = l.outType == kF32 ? 4 : 2;
+  if (l.elemType != kF16 && l.elemType != kBF16) { gradFail(errorText, "checkpoint gradient: dy is f16 or bf16"); return 1; }
+  if (l.accumulate && l.outType != kF32) { gradFail(errorText, "checkpoint gradient: only an f32 output is added to"); return 1; }
+  if (l.cols % 16 || l.outCols % 8 || l.in.codesLd % 16 || (l.dy.ld * 2) % 16 || (l.out.ld * ob) % 16) {
+    gradFail(errorText, "checkpoint gradient: D a multiple of 16, N of 8, and 16-byte row lengths (TMA tensor maps)");
+    return 1;
+  }
+  if ((reinterpret_cast<uintptr_t>(l.in.codes) | reinterpret_cast<uintptr_t>(l.dy.base) | reinterpret_cast<uintptr_t>(l.out.base)) & 15u) {
+    gradFail(errorText, "checkpoint gradient: codes, dy and dweight must be 16-byte aligned");
+    return 1;
+  }
+  if (l.rows >= (1ll << 31) - kTokens || l.cols >= (1ll << 30) || l.outCols >= (1ll << 30)) { gradFail(errorText, "checkpoint gradient: dimension too large"); return 1; }
+  if (l.rows == 0) {  // a sum of nothing
+    if (l.accumulate) return 0;
+    return cudaMemset2DAsync(l.out.base, static_cast<size_t>(l.out.ld * ob), 0, static_cast<size_t>(l.outCols * ob), static_cast<size_t>(l.cols), stream);
+  }
+  int device = 0;
+  if (const cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return e;
+  const int sms = deviceSmCount(device);
+  const SplitPlan plan = splitPlan(l.cols, l.outCols, l.rows, sms);
+  if (static_cast<int64_t>(plan.tilesM) * plan.tilesN * plan.splits >= (1ll << 31)) { gradFail(errorText, "checkpoint gradient: dimension too large"); return 1; }
+  const size_t need = checkpointGradWorkspaceBytes(l.cols, l.outCols, l.rows, sms);
+  if (need && (!l.workspace || l.workspaceBytes < need)) { gradFail(errorText, "checkpoint gradient: workspace too small"); return 1; }
+
+  CUtensorMap mapCodes, mapDy;
+  const CUtensorMapDataType dt = l.elemType == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  if (!makeMap2d(&mapCodes, CU_TENSOR_MAP_DATA_TYPE_UINT8, l.in.codes, static_cast<uint64_t>(l.cols), static_cast<uint64_t>(l.rows),
+                 static_cast<uint64_t>(l.in.codesLd), 128, kTokens, CU_TENSOR_MAP_SWIZZLE_NONE) ||
+      !makeMap2d(&mapDy, dt, l.dy.base, static_cast<uint64_t>(l.outCols), static_cast<uint64_t>(l.rows), static_cast<uint64_t>(l.dy.ld) * 2, 64, kTokens)) {
+    gradFail(errorText, "checkpoint gradient: cuTensorMapEncodeTiled failed (driver entry point missing or bad operand layout)");
+    return 1;
+  }
+  GradParams p = {};
+  p.D = static_cast<int>(l.cols);
+  p.N = static_cast<int>(l.outCols);
+  p.T = static_cast<int>(l.rows);
+  p.tilesM = plan.tilesM;
+  p.tilesN = plan.tilesN;
+  p.kBlocks = plan.kBlocks;
+  p.splits = plan.splits;
+  p.kPerSplit = plan.kPerSplit;
+  p.band = 16;
+  p.exps = l.in.exps;
+  p.expsLd = l.in.expsLd;
+  p.expCols = static_cast<int>((l.cols + kCheckpointBlock - 1) / kCheckpointBlock);
+  p.status = l.status;
+  const bool joined = plan.splits > 1;
+  p.out = joined ? l.workspace : l.out.base;
+  p.outLd = joined ? l.outCols : l.out.ld;
+  p.splitStride = joined ? l.cols * l.outCols : 0;
+  p.accumulate = joined ? 0 : l.accumulate;
+  const unsigned int fmt = l.elemType == kF16 ? 0u : 1u;
+  // D f32, A and B of the same 16-bit type, both with the long side contiguous (bits 15 and 16), 128 x 256
+  p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (1u << 16) | ((kTileN >> 3) << 17) | ((128u >> 4) << 24);
+  const int grid = std::min(sms, plan.tilesM * plan.tilesN * plan.splits);
+  const int out = joined ? static_cast<int>(kF32) : l.outType;
+  int rc = l.elemType == kF16 ? launchGradTyped<kF16>(out, plan.mb, mapCodes, mapDy, p, grid, stream)
+                              : launchGradTyped<kBF16>(out, plan.mb, mapCodes, mapDy, p, grid, stream);
+  if (rc != 0) return rc;
+  if (launched) *launched += 1;
+  if (joined) {
+    const int64_t quads = l.cols * l.outCols / 4;
+    const unsigned int joinGrid = static_cast<unsigned int>(std::min<int64_t>((quads + 255) / 256, static_cast<int64_t>(sms) * 16));
+    const float *partial = static_cast<const float *>(l.workspace);
+    const auto kernel = l.outType == kF32 ? checkpointGradJoinKernel<kF32> : l.outType == kF16 ? checkpointGradJoinKernel<kF16> : checkpointGradJoinKernel<kBF16>;
+    rc = launchOrdinary(kernel, dim3(joinGrid), dim3(256), 0, stream, partial, plan.splits, l.cols, static_cast<int>(l.outCols), l.out.base, l.out.ld, l.accumulate);
+    if (rc == 0 && launched) *launched += 1;
+  }
+  return rc;
+}
+
+} // namespace kernels
+} // namespace afir

@@ -577,7 +577,8 @@ Status CudaExecutor::launchDevice(const RunRequest &req, void *workspace, size_t
   // The status words (bad gather indices, a staged reduction's time-out) accumulate over the launches queued since
   // the last synchronize: they are cleared only when nothing unread is pending on this workspace.
   const bool hasStatusWords = (desc->kernelClass == KernelClass::Gather || desc->kernelClass == KernelClass::RowReduce ||
-                               desc->kernelClass == KernelClass::Matmul || desc->kernelClass == KernelClass::Transpose) &&
+                               desc->kernelClass == KernelClass::Matmul || desc->kernelClass == KernelClass::Transpose ||
+                               desc->kernelClass == KernelClass::CheckpointGrad) &&
                               args.workspace && args.workspaceBytes >= kWorkspaceStatusBytes;
   if (hasStatusWords && !(statusPending_ && statusWorkspace_ == args.workspace)) {
     e = cudaMemsetAsync(args.workspace, 0, kWorkspaceStatusReadBytes, args.stream);
@@ -664,6 +665,13 @@ Status CudaExecutor::synchronize(void *stream) {
     }
     if (static_cast<unsigned int>(words[2] & 0xffffffffull) != 0)
       return Status::error("[cuda:kernel_launch] transpose: a wait for a staged tile ran out after 2 s");
+    if (const unsigned int cg = static_cast<unsigned int>(words[2] >> 32)) {
+      static const char *roles[] = {"TMA producer", "MMA issuer", "output", "conversion"};
+      char text[160];
+      std::snprintf(text, sizeof(text), "[cuda:kernel_launch] checkpoint gradient: %s gave up waiting on a pipeline barrier after 2 s (status 0x%x)",
+                    roles[std::min(3u, cg & 0xffu)], cg);
+      return Status::error(text);
+    }
     constexpr unsigned long long kGatherTimeoutFlag = 1ull << 62;  // set by the staged gather kernel when a stage wait ran out
     if (bad & kGatherTimeoutFlag) return Status::error("[cuda:kernel_launch] gather kernel gave up waiting for a staged copy");
     if (bad) return Status::error("[cuda:kernel_launch] gather index out of range (" + std::to_string(bad) + " indices)");
