@@ -3,6 +3,9 @@
 #include "kernels/block_norm.h"
 
 #include <algorithm>
+#include <mutex>
+#include <set>
+#include <utility>
 
 #include "kernels/block_norm_kernels.h"
 #include "kernels/launch_util.h"
@@ -103,23 +106,37 @@ __global__ void __launch_bounds__(kFinishCols *kFinishSlots) blockNormFinishKern
 // ---- launch shape -----------------------------------------------------------------------------------------------
 struct TeamShape { bool vector; int nv, lanes, teamsPerCta; };
 
-// A team has at most 512 threads; a row that fits them with one vector each takes one (short rows: fewer threads, more
-// teams), a wider one takes 2, 4 or 8.
-TeamShape teamShape(int elemType, int64_t cols, bool vector) {
+TeamShape shapeOf(int vec, int nv, int64_t cols) {
   TeamShape s;
-  s.vector = vector;
-  const int vec = vector ? (elemType == kF32 ? 4 : 8) : 1;
-  if (vector) {
-    s.nv = 1;
-    while (static_cast<int64_t>(s.nv) * vec * 512 < cols) s.nv *= 2;
-  } else {
-    s.nv = cols <= kScalarSmall * 512 ? kScalarSmall : kScalarLarge;
-  }
-  const int64_t perThread = static_cast<int64_t>(s.nv) * vec;
-  const int64_t threads = (cols + perThread - 1) / perThread;
-  s.lanes = static_cast<int>((threads + 31) / 32 * 32);
+  s.vector = vec > 1;
+  s.nv = nv;
+  const int64_t perThread = static_cast<int64_t>(nv) * vec;
+  s.lanes = static_cast<int>(((cols + perThread - 1) / perThread + 31) / 32 * 32);
   s.teamsPerCta = std::max(1, 256 / s.lanes);
   return s;
+}
+int scalarElements(int64_t cols) { return cols <= kScalarSmall * 512 ? kScalarSmall : kScalarLarge; }
+
+// A team has at most 512 threads; a row that fits them with one vector each takes one (short rows: fewer threads, more
+// teams), a wider one takes 2, 4 or 8.
+TeamShape forwardShape(int elemType, int64_t cols, bool vector) {
+  const int vec = vector ? (elemType == kF32 ? 4 : 8) : 1;
+  if (!vector) return shapeOf(1, scalarElements(cols), cols);
+  int nv = 1;
+  while (static_cast<int64_t>(nv) * vec * 512 < cols) nv *= 2;
+  return shapeOf(vec, nv, cols);
+}
+
+// Columns per thread of the gradient: 16 for an rms norm, 8 for a layer norm (which keeps twice the column sums) while
+// that leaves a team of at most 512 threads; beyond, what the width needs.
+TeamShape gradShape(int elemType, int kind, int64_t cols, bool vector) {
+  const int vec = vector ? (elemType == kF32 ? 4 : 8) : 1;
+  if (!vector) return shapeOf(1, scalarElements(cols), cols);
+  const int64_t perThread = kind == kLayerNorm ? 8 : 16;
+  int nv = 1;
+  while (nv * vec < perThread && static_cast<int64_t>(nv) * vec * 32 < cols) nv *= 2;
+  while (static_cast<int64_t>(nv) * vec * 512 < cols) nv *= 2;
+  return shapeOf(vec, nv, cols);
 }
 
 bool rowsAligned(const void *base, int64_t ld, int64_t elemBytes, int64_t bytes) {
@@ -127,35 +144,53 @@ bool rowsAligned(const void *base, int64_t ld, int64_t elemBytes, int64_t bytes)
 }
 bool vectorAligned(const void *base) { return (reinterpret_cast<uintptr_t>(base) & 15u) == 0; }
 
-GradPlan gradPlan(int gateForm, int64_t rows, int64_t cols, int64_t groupRows, int smCount) {
+int64_t gradTeamsPerSm(int kind, int64_t cols) {
+  return std::min<int64_t>(16, std::max<int64_t>(1, (kind == kLayerNorm ? 4096 : 8192) / cols));
+}
+
+GradPlan gradPlan(int kind, int gateForm, int64_t rows, int64_t cols, int64_t groupRows, int smCount) {
   GradPlan plan = {};
-  const bool grouped = gateForm == kGateGroup;
-  plan.groupRows = grouped ? std::min(groupRows, std::max<int64_t>(rows, 1)) : std::max<int64_t>(rows, 1);
-  plan.groups = (rows + plan.groupRows - 1) / plan.groupRows;
-  if (!grouped) plan.groups = 1;
-  // About 8192 columns' worth of teams per SM: enough rows under way to cover a row's two sums, few enough that the
-  // teams' sums (f32, one or two rows each) stay small beside the row tensors.
-  const int64_t perSm = std::min<int64_t>(16, std::max<int64_t>(1, 8192 / cols));
-  const int64_t teams = std::max<int64_t>(1, std::min<int64_t>(rows, smCount * perSm));
-  const int64_t wanted = std::max<int64_t>(1, plan.groups ? teams / plan.groups : 1);
-  plan.chunkRows = (plan.groupRows + wanted - 1) / wanted;
-  plan.chunks = (plan.groupRows + plan.chunkRows - 1) / plan.chunkRows;
-  plan.teams = std::max<int64_t>(1, std::min<int64_t>(teams, plan.groups * plan.chunks));
-  plan.sumsLd = (cols + 3) / 4 * 4;
+  const int64_t all = std::max<int64_t>(rows, 1);
+  const int64_t perGroup = gateForm == kGateGroup ? std::min(groupRows, all) : all;
+  const int64_t groups = gateForm == kGateGroup ? (rows + perGroup - 1) / perGroup : 1;
+  // 512 threads' worth of teams per SM (they have 128 registers each): enough rows under way to cover a row's two
+  // sums, few enough that the teams' sums (f32, one or two rows each) stay small beside the row tensors.
+  const int64_t teams = std::max<int64_t>(1, std::min<int64_t>(rows, smCount * gradTeamsPerSm(kind, cols)));
+  const int64_t wanted = std::max<int64_t>(1, groups ? teams / groups : 1);
+  const int64_t chunkRows = (perGroup + wanted - 1) / wanted;
+  const int64_t chunks = (perGroup + chunkRows - 1) / chunkRows;
+  plan.groups = static_cast<int>(groups);
+  plan.groupRows = static_cast<int>(perGroup);
+  plan.chunkRows = static_cast<int>(chunkRows);
+  plan.chunks = static_cast<int>(chunks);
+  plan.teams = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(teams, groups * chunks)));
+  plan.sumsLd = static_cast<int>((cols + 3) / 4 * 4);
   return plan;
 }
 
 int64_t sumsFloats(const GradPlan &plan, int pass, int kind) {
   const int64_t values = kind == kLayerNorm ? 2 : 1;
-  return values * plan.sumsLd * ((pass != kPre ? plan.groups * plan.chunks : 0) + (pass != kPost ? plan.teams : 0));
+  return values * plan.sumsLd * ((pass != kPre ? static_cast<int64_t>(plan.groups) * plan.chunks : 0) + (pass != kPost ? plan.teams : 0));
 }
 
 } // namespace
 
+cudaError_t reserveSharedMemory(const void *kernel, int bytes) {
+  static std::mutex mu;
+  static std::set<std::pair<const void *, int>> done;
+  int device = 0;
+  if (const cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  if (done.count({kernel, device})) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.insert({kernel, device});
+  return e;
+}
+
 int launchBlockNorm(const BlockNormLaunch &l, cudaStream_t stream, int *launched) {
   if (launched) *launched = 0;
   if (l.rows == 0) return 0;
-  if (l.cols <= 0 || l.cols > kMaxNormCols) return cudaErrorInvalidValue;
+  if (l.cols <= 0 || l.cols > kMaxNormCols || l.rows > kMaxNormRows) return cudaErrorInvalidValue;
   const int64_t eb = elemBytes(l.elemType);
   const int vec = static_cast<int>(16 / eb);
   bool vector = l.cols % vec == 0;
@@ -163,7 +198,7 @@ int launchBlockNorm(const BlockNormLaunch &l, cudaStream_t stream, int *launched
   for (const RowsOut &r : {l.out, l.h}) vector = vector && rowsAligned(r.base, r.ld, eb, 16);
   for (const void *v : {l.a.weight, l.a.bias, l.b.weight, l.b.bias, l.scale}) vector = vector && vectorAligned(v);
   vector = vector && rowsAligned(l.checkpoint.codes, l.checkpoint.codesLd, 1, vec);
-  const TeamShape s = teamShape(l.elemType, l.cols, vector);
+  const TeamShape s = forwardShape(l.elemType, l.cols, vector);
   const ForwardKernel kernel = l.elemType == kF32   ? forwardKernel<kF32>(l.kind, l.pass, vector, s.nv)
                                : l.elemType == kF16 ? forwardKernel<kF16>(l.kind, l.pass, vector, s.nv)
                                                     : forwardKernel<kBF16>(l.kind, l.pass, vector, s.nv);
@@ -187,20 +222,20 @@ int launchBlockNorm(const BlockNormLaunch &l, cudaStream_t stream, int *launched
 }
 
 size_t blockNormGradWorkspaceBytes(int pass, int kind, int gateForm, int64_t rows, int64_t cols, int64_t groupRows, int smCount) {
-  return static_cast<size_t>(sumsFloats(gradPlan(gateForm, rows, cols, groupRows, smCount), pass, kind)) * sizeof(float);
+  return static_cast<size_t>(sumsFloats(gradPlan(kind, gateForm, rows, cols, groupRows, smCount), pass, kind)) * sizeof(float);
 }
 
 int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *launched) {
   if (launched) *launched = 0;
-  if (l.cols <= 0 || l.cols > kMaxNormCols) return cudaErrorInvalidValue;
+  if (l.cols <= 0 || l.cols > kMaxNormCols || l.rows > kMaxNormRows) return cudaErrorInvalidValue;
   int device = 0;
   if (const cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return e;
-  GradPlan plan = gradPlan(l.gateForm, l.rows, l.cols, l.groupRows, deviceSmCount(device));
+  GradPlan plan = gradPlan(l.kind, l.gateForm, l.rows, l.cols, l.groupRows, deviceSmCount(device));
   const size_t need = static_cast<size_t>(sumsFloats(plan, l.pass, l.kind)) * sizeof(float);
   if (!l.workspace || l.workspaceBytes < need || !vectorAligned(l.workspace)) return cudaErrorInvalidValue;
   const int64_t values = l.kind == kLayerNorm ? 2 : 1;
   if (l.pass != kPre) plan.sumsA = static_cast<float *>(l.workspace);
-  if (l.pass != kPost) plan.sumsB = static_cast<float *>(l.workspace) + (l.pass != kPre ? plan.groups * plan.chunks * values * plan.sumsLd : 0);
+  if (l.pass != kPost) plan.sumsB = static_cast<float *>(l.workspace) + (l.pass != kPre ? static_cast<int64_t>(plan.groups) * plan.chunks * values * plan.sumsLd : 0);
 
   if (l.rows > 0) {
     const int64_t eb = elemBytes(l.elemType);
@@ -211,13 +246,32 @@ int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *
     if (l.gateForm == kGateToken) vector = vector && rowsAligned(l.dgate.base, l.dgate.ld, eb, 16);
     for (const void *v : {l.a.weight, l.a.bias, l.b.weight, l.scale}) vector = vector && vectorAligned(v);
     vector = vector && rowsAligned(l.checkpoint.codes, l.checkpoint.codesLd, 1, vec);
-    const TeamShape s = teamShape(l.elemType, l.cols, vector);
-    const GradKernel kernel = l.elemType == kF32   ? gradKernel<kF32>(l.kind, l.pass, vector, s.nv)
-                              : l.elemType == kF16 ? gradKernel<kF16>(l.kind, l.pass, vector, s.nv)
-                                                   : gradKernel<kBF16>(l.kind, l.pass, vector, s.nv);
-    if (!kernel) return cudaErrorInvalidValue;
-    const unsigned int grid = static_cast<unsigned int>((plan.teams + s.teamsPerCta - 1) / s.teamsPerCta);
-    const cudaError_t e = launchDependent(kernel, dim3(grid), dim3(static_cast<unsigned int>(s.lanes * s.teamsPerCta)), 0, stream, l, plan, s.lanes);
+    const TeamShape s = gradShape(l.elemType, l.kind, l.cols, vector);
+    const unsigned int threads = static_cast<unsigned int>(s.lanes * s.teamsPerCta);
+    const dim3 grid(static_cast<unsigned int>((plan.teams + s.teamsPerCta - 1) / s.teamsPerCta));
+    // rows fetched ahead: as many (2 to 4) as the teams of an SM have shared memory for; rows too wide for two take the
+    // kernel without
+    const int tensors = (l.pass != kPost ? 2 : 0) + (l.dout.base ? 1 : 0) + (l.pass != kPre ? 1 : 0) + (l.gateForm == kGateToken ? 1 : 0);
+    const size_t rowBytes = static_cast<size_t>(tensors) * static_cast<size_t>(s.nv) * 16;
+    const size_t threadsPerSm = std::max<size_t>(threads, static_cast<size_t>(gradTeamsPerSm(l.kind, l.cols)) * static_cast<size_t>(s.lanes));
+    constexpr size_t kAheadBytesPerSm = 200 * 1024, kAheadBytesPerCta = 220 * 1024;
+    const int stages = static_cast<int>(std::min<size_t>(4, std::max<size_t>(2, kAheadBytesPerSm / (rowBytes * threadsPerSm))));
+    const size_t slotBytes = static_cast<size_t>(stages) * rowBytes * threads;
+    const GradAheadKernel ahead = !vector || slotBytes > kAheadBytesPerCta ? nullptr
+                                  : l.elemType == kF32                      ? gradAheadKernel<kF32>(l.kind, l.pass, s.nv)
+                                  : l.elemType == kF16                      ? gradAheadKernel<kF16>(l.kind, l.pass, s.nv)
+                                                                            : gradAheadKernel<kBF16>(l.kind, l.pass, s.nv);
+    cudaError_t e;
+    if (ahead) {
+      if (e = reserveSharedMemory(reinterpret_cast<const void *>(ahead), static_cast<int>(kAheadBytesPerCta)); e != cudaSuccess) return e;
+      e = launchDependent(ahead, grid, dim3(threads), slotBytes, stream, l, plan, s.lanes, stages);
+    } else {
+      const GradKernel kernel = l.elemType == kF32   ? gradKernel<kF32>(l.kind, l.pass, vector, s.nv)
+                                : l.elemType == kF16 ? gradKernel<kF16>(l.kind, l.pass, vector, s.nv)
+                                                     : gradKernel<kBF16>(l.kind, l.pass, vector, s.nv);
+      if (!kernel) return cudaErrorInvalidValue;
+      e = launchDependent(kernel, grid, dim3(threads), 0, stream, l, plan, s.lanes);
+    }
     if (e != cudaSuccess) return e;
     if (launched) *launched += 1;
   }

@@ -18,6 +18,7 @@ namespace afir {
 namespace kernels {
 
 constexpr int64_t kMaxNormCols = 16384;  // a row stays in the registers of one team of at most 512 threads
+constexpr int64_t kMaxNormRows = 1ll << 30;  // rows, and rows of column sums, are counted in 32 bits
 constexpr int kCheckpointBlock = 128;    // columns that share one power of two
 
 enum NormPass : int { kPre = 0, kPost = 1, kPostPre = 2 };

@@ -23,12 +23,12 @@ namespace kernels {
 // How the rows are split over teams, and where their sums go.  Depends on sizes only, so that the workspace can be
 // sized before any pointer is known.
 struct GradPlan {
-  int64_t groups;         // gate groups whose sums are kept apart (1 unless kGateGroup)
-  int64_t groupRows;      // rows of a group (all rows unless kGateGroup)
-  int64_t chunks;         // runs of rows per group
-  int64_t chunkRows;      // rows of a run
-  int64_t teams;          // teams launched; each takes runs index, index + teams, ...
-  int64_t sumsLd;         // floats of one row of sums (cols, rounded up to 16 bytes)
+  int groups;             // gate groups whose sums are kept apart (1 unless kGateGroup)
+  int groupRows;          // rows of a group (all rows unless kGateGroup)
+  int chunks;             // runs of rows per group
+  int chunkRows;          // rows of a run
+  int teams;              // teams launched; each takes runs index, index + teams, ...
+  int sumsLd;             // floats of one row of sums (cols, rounded up to 16 bytes)
   float *sumsA, *sumsB;   // [groups*chunks][values][sumsLd], [teams][values][sumsLd]
 };
 
@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(512) blockNormGradKernel(const __grid_constant
   Team team = makeTeam(teamLanes, scratch);
   const int cols = static_cast<int>(p.cols);
   const float share = 1.0f / static_cast<float>(cols);
-  const int64_t teamIndex = static_cast<int64_t>(blockIdx.x) * team.count + team.index;
+  const int teamIndex = static_cast<int>(blockIdx.x) * team.count + team.index;
   if (teamIndex >= plan.teams) return;
 
   float sumB[kPrePart ? kValues : 1][NV][VEC];
@@ -62,11 +62,11 @@ __global__ void __launch_bounds__(512) blockNormGradKernel(const __grid_constant
 #pragma unroll
       for (int e = 0; e < VEC; ++e) sumB[k][i][e] = 0.0f;
 
-  for (int64_t run = teamIndex; run < plan.groups * plan.chunks; run += plan.teams) {
-    const int64_t group = run / plan.chunks, chunk = run - group * plan.chunks;
-    const int64_t groupEnd = min(p.rows, (group + 1) * plan.groupRows);
-    const int64_t begin = group * plan.groupRows + chunk * plan.chunkRows;
-    const int64_t end = min(groupEnd, begin + plan.chunkRows);
+  for (int run = teamIndex; run < plan.groups * plan.chunks; run += plan.teams) {
+    const int group = run / plan.chunks, chunk = run - group * plan.chunks;
+    const int64_t groupBegin = static_cast<int64_t>(group) * plan.groupRows;
+    const int64_t begin = groupBegin + static_cast<int64_t>(chunk) * plan.chunkRows;
+    const int64_t end = min(min(p.rows, groupBegin + plan.groupRows), begin + plan.chunkRows);
 
     float sumA[kPostPart ? kValues : 1][NV][VEC];
 #pragma unroll
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(512) blockNormGradKernel(const __grid_constant
         const int col = (i * team.lanes + team.lane) * VEC;
         if (col >= cols) continue;
 #pragma unroll
-        for (int k = 0; k < kValues; ++k) storeSums<VEC>(plan.sumsA + (run * kValues + k) * plan.sumsLd + col, sumA[k][i]);
+        for (int k = 0; k < kValues; ++k) storeSums<VEC>(plan.sumsA + (static_cast<int64_t>(run) * kValues + k) * plan.sumsLd + col, sumA[k][i]);
       }
     }
   }
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(512) blockNormGradKernel(const __grid_constant
       const int col = (i * team.lanes + team.lane) * VEC;
       if (col >= cols) continue;
 #pragma unroll
-      for (int k = 0; k < kValues; ++k) storeSums<VEC>(plan.sumsB + (teamIndex * kValues + k) * plan.sumsLd + col, sumB[k][i]);
+      for (int k = 0; k < kValues; ++k) storeSums<VEC>(plan.sumsB + (static_cast<int64_t>(teamIndex) * kValues + k) * plan.sumsLd + col, sumB[k][i]);
     }
   }
 }

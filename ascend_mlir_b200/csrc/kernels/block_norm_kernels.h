@@ -7,13 +7,16 @@
 namespace afir {
 namespace kernels {
 
-// VEC = 16-byte accesses; NV = vectors (or, without them, elements) per thread.
+// `vector`: 16-byte accesses; nv = vectors (or, without them, elements) per thread.
 constexpr int kScalarSmall = 8, kScalarLarge = 32;
 
 using ForwardKernel = void (*)(const BlockNormLaunch, int);
 using GradKernel = void (*)(const BlockNormGradLaunch, const GradPlan, int);
 template <int ELEM> ForwardKernel forwardKernel(int kind, int pass, bool vector, int nv);
 template <int ELEM> GradKernel gradKernel(int kind, int pass, bool vector, int nv);
+// With rows fetched ahead (block_norm_grad_vector.cuh); null where a thread would hold more than it has registers for.
+using GradAheadKernel = void (*)(const BlockNormGradLaunch, const GradPlan, int, int);
+template <int ELEM> GradAheadKernel gradAheadKernel(int kind, int pass, int nv);
 
 } // namespace kernels
 } // namespace afir

@@ -54,5 +54,9 @@ cudaError_t launchOrdinary(void (*kernel)(Params...), dim3 grid, dim3 block, siz
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
+// Lets `kernel` take up to `bytes` of dynamic shared memory on the current device; asked of the driver once per kernel
+// and device.
+cudaError_t reserveSharedMemory(const void *kernel, int bytes);
+
 } // namespace kernels
 } // namespace afir

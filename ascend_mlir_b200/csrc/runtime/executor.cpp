@@ -17,9 +17,17 @@ Status cudaFail(cudaError_t e, const char *what) {
   return Status::error(std::string(what) + ": " + cudaGetErrorString(e));
 }
 
+// FNV-1a over 8-byte words, then the rest bytewise: every launch hashes its kernel binary.
 uint64_t fnv1a(const uint8_t *p, size_t n) {
   uint64_t h = 1469598103934665603ull;
-  for (size_t i = 0; i < n; ++i) { h ^= p[i]; h *= 1099511628211ull; }
+  size_t i = 0;
+  for (; i + 8 <= n; i += 8) {
+    uint64_t w;
+    std::memcpy(&w, p + i, 8);
+    h = (h ^ w) * 1099511628211ull;
+    h ^= h >> 32;  // a word's high bits reach the low ones
+  }
+  for (; i < n; ++i) { h ^= p[i]; h *= 1099511628211ull; }
   return h ^ (static_cast<uint64_t>(n) << 1);
 }
 
