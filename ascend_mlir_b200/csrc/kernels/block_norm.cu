@@ -117,12 +117,15 @@ TeamShape shapeOf(int vec, int nv, int64_t cols) {
 }
 int scalarElements(int64_t cols) { return cols <= kScalarSmall * 512 ? kScalarSmall : kScalarLarge; }
 
-// A team has at most 512 threads; a row that fits them with one vector each takes one (short rows: fewer threads, more
-// teams), a wider one takes 2, 4 or 8.
-TeamShape forwardShape(int elemType, int64_t cols, bool vector) {
+// A team has at most 512 threads.  Few rows: one vector per thread while that is enough, for the shortest way through one
+// row.  Rows enough to fill the SMs: 16 columns per thread, which keeps more loads under way per thread and less
+// of the time in sums across warps.
+TeamShape forwardShape(int elemType, int64_t rows, int64_t cols, bool vector, int smCount) {
   const int vec = vector ? (elemType == kF32 ? 4 : 8) : 1;
   if (!vector) return shapeOf(1, scalarElements(cols), cols);
+  const int64_t perThread = rows >= smCount ? 16 : vec;
   int nv = 1;
+  while (nv * vec < perThread && static_cast<int64_t>(nv) * vec * 32 < cols) nv *= 2;
   while (static_cast<int64_t>(nv) * vec * 512 < cols) nv *= 2;
   return shapeOf(vec, nv, cols);
 }
@@ -198,7 +201,9 @@ int launchBlockNorm(const BlockNormLaunch &l, cudaStream_t stream, int *launched
   for (const RowsOut &r : {l.out, l.h}) vector = vector && rowsAligned(r.base, r.ld, eb, 16);
   for (const void *v : {l.a.weight, l.a.bias, l.b.weight, l.b.bias, l.scale}) vector = vector && vectorAligned(v);
   vector = vector && rowsAligned(l.checkpoint.codes, l.checkpoint.codesLd, 1, vec);
-  const TeamShape s = forwardShape(l.elemType, l.cols, vector);
+  int device = 0;
+  if (const cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return e;
+  const TeamShape s = forwardShape(l.elemType, l.rows, l.cols, vector, deviceSmCount(device));
   const ForwardKernel kernel = l.elemType == kF32   ? forwardKernel<kF32>(l.kind, l.pass, vector, s.nv)
                                : l.elemType == kF16 ? forwardKernel<kF16>(l.kind, l.pass, vector, s.nv)
                                                     : forwardKernel<kBF16>(l.kind, l.pass, vector, s.nv);

@@ -65,31 +65,7 @@ __device__ __forceinline__ void storeStatistics(const Team &team, const NormStat
   if (s.mean) s.mean[row] = mean;
 }
 
-// The 8-bit checkpoint of the row in v.  128 columns are 128 / VEC neighbouring lanes: the largest magnitude is a
-// shuffle tree over them.
-template <int ELEM, int NV, int VEC>
-__device__ __forceinline__ void storeCheckpoint(const Team &team, const float (&v)[NV][VEC], int cols, const CheckpointOut &c, int64_t row) {
-  static_assert(VEC >= 4, "128 columns inside one warp");
-  constexpr int kGroup = kCheckpointBlock / VEC;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int col = (i * team.lanes + team.lane) * VEC;
-    float top = 0.0f;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) top = fmaxf(top, finiteMagnitude(v[i][e]));
-#pragma unroll
-    for (int o = kGroup / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (col >= cols) continue;
-    const int e8 = checkpointExponent<ELEM>(top);
-    const CheckpointScale s = checkpointScale<ELEM>(e8);
-    float r[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) r[e] = scaledForCode(v[i][e], s);
-    storeCodes<VEC>(c.codes + row * c.codesLd + col, r);
-    if (col % kCheckpointBlock == 0) c.exps[row * c.expsLd + col / kCheckpointBlock] = static_cast<uint8_t>(e8);
-  }
-}
-
+// Any width and alignment, an element at a time.
 template <int ELEM, int KIND, int PASS, int VEC, int NV>
 __global__ void __launch_bounds__(512) blockNormForwardKernel(const __grid_constant__ BlockNormLaunch p, int teamLanes) {
   gridDependencyPrologue();
@@ -106,9 +82,6 @@ __global__ void __launch_bounds__(512) blockNormForwardKernel(const __grid_const
 #pragma unroll
       for (int e = 0; e < VEC; ++e) v[i][e] = 0.0f;
       if (col < cols) loadElems<ELEM, VEC>(first.base, row * first.ld + col, v[i]);
-    }
-    if constexpr (VEC > 1) {
-      if (p.checkpoint.codes) storeCheckpoint<ELEM, NV, VEC>(team, v, cols, p.checkpoint, row);
     }
     float mean, rstd;
     rowStatistics<KIND, NV, VEC>(team, v, cols, PASS == kPre ? p.epsB : p.epsA, mean, rstd);

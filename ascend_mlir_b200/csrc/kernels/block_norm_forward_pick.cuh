@@ -1,21 +1,21 @@
-// The instantiations of the forward row kernel for one element type (included by one file per type).
+// The instantiations of the forward row kernels for one element type (included by one file per type).
 #pragma once
 
 #include "kernels/block_norm_forward.cuh"
+#include "kernels/block_norm_forward_vector.cuh"
 #include "kernels/block_norm_kernels.h"
 
 namespace afir {
 namespace kernels {
 
 template <int ELEM, int KIND, int PASS> ForwardKernel forwardKernelOf(bool vector, int nv) {
-  constexpr int V = ElemOf<ELEM>::kVec;
   if (!vector) return nv <= kScalarSmall ? blockNormForwardKernel<ELEM, KIND, PASS, 1, kScalarSmall> : blockNormForwardKernel<ELEM, KIND, PASS, 1, kScalarLarge>;
   switch (nv) {
-  case 1: return blockNormForwardKernel<ELEM, KIND, PASS, V, 1>;
-  case 2: return blockNormForwardKernel<ELEM, KIND, PASS, V, 2>;
-  case 4: return blockNormForwardKernel<ELEM, KIND, PASS, V, 4>;
+  case 1: return blockNormForwardVectorKernel<ELEM, KIND, PASS, 1>;
+  case 2: return blockNormForwardVectorKernel<ELEM, KIND, PASS, 2>;
+  case 4: return blockNormForwardVectorKernel<ELEM, KIND, PASS, 4>;
   default:
-    if constexpr (ELEM == kF32) return blockNormForwardKernel<ELEM, KIND, PASS, V, 8>;
+    if constexpr (ELEM == kF32) return blockNormForwardVectorKernel<ELEM, KIND, PASS, 8>;
     else return nullptr;
   }
 }

@@ -1,0 +1,206 @@
+// The forward row kernel for rows in 16-byte vectors (formulas: block_norm_forward.cuh).
+//
+// A thread issues the loads of everything it will need of a row (y, x and a token's gate) before the first sum, so that
+// the sums wait for HBM once.  A layer norm's statistics take one barrier: each warp centres its own columns, and the
+// warps' sums of squares are joined with what their means differ by (Chan, Golub and LeVeque's update).
+#pragma once
+
+#include "kernels/block_norm_forward.cuh"
+#include "kernels/pairs.cuh"
+
+namespace afir {
+namespace kernels {
+
+// Mean and 1/sqrt(variance + eps) of the row in v; what lies beyond the row is zero in v and not counted.
+template <int ELEM, int KIND, int NV>
+__device__ __forceinline__ void pairStatistics(Team &team, const F2 (&v)[NV][kPairs<ELEM>], int cols, float eps, float &mean, float &rstd) {
+  constexpr int VEC = ElemOf<ELEM>::kVec, P = kPairs<ELEM>;
+  const float share = 1.0f / static_cast<float>(cols);
+  if constexpr (KIND == kRmsNorm) {
+    F2 q = splat(0.0f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < P; ++e) q = fma2(v[i][e], v[i][e], q);
+    float s[1] = {sumOf(q)};
+    teamSum(team, s);
+    mean = 0.0f;
+    rstd = 1.0f / sqrtf(s[0] * share + eps);
+  } else {
+    F2 sum = splat(0.0f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < P; ++e) sum = sum + v[i][e];
+    const float s = warpSum(sumOf(sum));
+    auto columnsOf = [&](int warp) {  // of the row, in this warp's lanes
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) n += max(0, min(32 * VEC, cols - (i * team.lanes + warp * 32) * VEC));
+      return static_cast<float>(n);
+    };
+    const float mine = columnsOf(team.lane >> 5);
+    const float centre = s / fmaxf(mine, 1.0f);
+    const F2 shift = splat(-centre);
+    F2 q = splat(0.0f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if ((i * team.lanes + team.lane) * VEC >= cols) continue;
+#pragma unroll
+      for (int e = 0; e < P; ++e) {
+        const F2 d = v[i][e] + shift;
+        q = fma2(d, d, q);
+      }
+    }
+    float squares = warpSum(sumOf(q));
+    if (team.lanes == 32) {
+      mean = centre;
+    } else {
+      float *buf = team.scratch + team.half * 32;
+      team.half ^= 1;
+      const int lane = threadIdx.x & 31, warps = team.lanes >> 5;
+      if (lane == 0) {
+        buf[team.lane >> 5] = s;
+        buf[16 + (team.lane >> 5)] = squares;
+      }
+      asm volatile("bar.sync %0, %1;" ::"r"(team.index + 1), "r"(team.lanes) : "memory");
+      const float n = lane < warps ? columnsOf(lane) : 0.0f;
+      const float sw = lane < warps ? buf[lane] : 0.0f, qw = lane < warps ? buf[16 + lane] : 0.0f;
+      float total = sw;
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      mean = __shfl_sync(0xffffffffu, total, 0) * share;
+      const float off = sw / fmaxf(n, 1.0f) - mean;
+      squares = n > 0.0f ? fmaf(n * off, off, qw) : 0.0f;
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
+      squares = __shfl_sync(0xffffffffu, squares, 0);
+    }
+    rstd = 1.0f / sqrtf(squares * share + eps);
+  }
+}
+
+// v normed, times weight, plus bias.
+template <int ELEM, int KIND>
+__device__ __forceinline__ void normPairs(F2 (&v)[kPairs<ELEM>], F2 shift, F2 rstd, const NormVectors &p, int paramType, int col) {
+  F2 w[kPairs<ELEM>];
+  loadParamPairs<ELEM>(p.weight, paramType, col, w);
+#pragma unroll
+  for (int e = 0; e < kPairs<ELEM>; ++e) v[e] = (KIND == kLayerNorm ? (v[e] + shift) * rstd : v[e] * rstd) * w[e];
+  if constexpr (KIND == kLayerNorm) {
+    loadParamPairs<ELEM>(p.bias, paramType, col, w);
+#pragma unroll
+    for (int e = 0; e < kPairs<ELEM>; ++e) v[e] = v[e] + w[e];
+  }
+}
+
+// The 8-bit checkpoint of a vector.  128 columns are 128 / VEC neighbouring lanes: the largest magnitude is a shuffle
+// tree over them.
+template <int ELEM>
+__device__ __forceinline__ void storeCheckpointVector(const F2 (&p)[kPairs<ELEM>], int col, int cols, const CheckpointOut &c, int64_t row) {
+  constexpr int VEC = ElemOf<ELEM>::kVec, kGroup = kCheckpointBlock / VEC;
+  float v[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC / 2; ++e) {
+    const float2 f = valuesOf(p[e]);
+    v[2 * e] = f.x;
+    v[2 * e + 1] = f.y;
+  }
+  float top = 0.0f;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) top = fmaxf(top, finiteMagnitude(v[e]));
+#pragma unroll
+  for (int o = kGroup / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (col >= cols) return;
+  const int e8 = checkpointExponent<ELEM>(top);
+  const CheckpointScale s = checkpointScale<ELEM>(e8);
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) v[e] = scaledForCode(v[e], s);
+  storeCodes<VEC>(c.codes + row * c.codesLd + col, v);
+  if (col % kCheckpointBlock == 0) c.exps[row * c.expsLd + col / kCheckpointBlock] = static_cast<uint8_t>(e8);
+}
+
+template <int ELEM, int KIND, int PASS, int NV>
+__global__ void __launch_bounds__(512) blockNormForwardVectorKernel(const __grid_constant__ BlockNormLaunch p, int teamLanes) {
+  gridDependencyPrologue();
+  constexpr int VEC = ElemOf<ELEM>::kVec, P = kPairs<ELEM>;
+  constexpr int kPostVectors = PASS == kPre ? 1 : NV;
+  __shared__ float scratch[kTeamScratchFloats];
+  Team team = makeTeam(teamLanes, scratch);
+  const int cols = static_cast<int>(p.cols);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * team.count;
+  auto colOf = [&](int i) { return (i * team.lanes + team.lane) * VEC; };
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * team.count + team.index; row < p.rows; row += step) {
+    const RowsIn first = PASS == kPre ? p.x : p.y;
+    auto raw = [&](const RowsIn &r, int64_t at, int i) {
+      return *reinterpret_cast<const uint4 *>(static_cast<const char *>(r.base) + (at * r.ld + colOf(i)) * (16 / VEC));
+    };
+    uint4 raw0[NV], rawX[kPostVectors], rawGate[kPostVectors];
+    const bool gated = PASS != kPre && p.gateForm != kGateNone;
+    const int64_t gateRow = p.gateForm == kGateGroup ? row / p.groupRows : row;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) raw0[i] = colOf(i) < cols ? raw(first, row, i) : make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (PASS != kPre) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (colOf(i) >= cols) continue;
+        rawX[i] = raw(p.x, row, i);
+        if (gated) rawGate[i] = raw(p.gate, gateRow, i);
+      }
+    }
+    F2 v[NV][P];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) widenPairs<ELEM>(raw0[i], v[i]);
+    if (p.checkpoint.codes) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) storeCheckpointVector<ELEM>(v[i], colOf(i), cols, p.checkpoint, row);
+    }
+    float mean, rstd;
+    pairStatistics<ELEM, KIND, NV>(team, v, cols, PASS == kPre ? p.epsB : p.epsA, mean, rstd);
+    storeStatistics(team, PASS == kPre ? p.statsB : p.statsA, row, mean, rstd);
+    if constexpr (PASS != kPre) {
+      const F2 shift = splat(-mean), r = splat(rstd), alpha = splat(p.alpha);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int col = colOf(i);
+        if (col >= cols) continue;
+        normPairs<ELEM, KIND>(v[i], shift, r, p.a, p.paramType, col);
+        F2 t[P];
+        if (gated) {
+          widenPairs<ELEM>(rawGate[i], t);
+          gatePairs(t, p.gateAct);
+#pragma unroll
+          for (int e = 0; e < P; ++e) v[i][e] = v[i][e] * t[e];
+        }
+        if (p.scale) {
+          loadParamPairs<ELEM>(p.scale, p.paramType, col, t);
+#pragma unroll
+          for (int e = 0; e < P; ++e) v[i][e] = v[i][e] * t[e];
+        }
+        widenPairs<ELEM>(rawX[i], t);
+#pragma unroll
+        for (int e = 0; e < P; ++e) v[i][e] = fma2(alpha, t[e], v[i][e]);
+        const uint4 stored = narrowPairs<ELEM>(v[i]);
+        *reinterpret_cast<uint4 *>(static_cast<char *>(p.out.base) + (row * p.out.ld + col) * (16 / VEC)) = stored;
+        if constexpr (PASS == kPostPre) widenPairs<ELEM>(stored, v[i]);  // as it is stored
+      }
+      if constexpr (PASS == kPostPre) {
+        pairStatistics<ELEM, KIND, NV>(team, v, cols, p.epsB, mean, rstd);
+        storeStatistics(team, p.statsB, row, mean, rstd);
+      }
+    }
+    if constexpr (PASS != kPost) {
+      const F2 shift = splat(-mean), r = splat(rstd);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int col = colOf(i);
+        if (col >= cols) continue;
+        normPairs<ELEM, KIND>(v[i], shift, r, p.b, p.paramType, col);
+        storePairs<ELEM>(p.h.base, row * p.h.ld + col, v[i]);
+      }
+    }
+  }
+}
+
+} // namespace kernels
+} // namespace afir

@@ -16,39 +16,52 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// 128 columns are 16 lanes (8 columns each, 16-bit types) or 32 lanes (4 each, f32); a thread's vectors are neighbouring
-// in a flat numbering of [rows, blocks of 128, lanes], so a warp reads whole lines and a row may end inside a block.
+// 128 columns are 16 lanes (8 columns each, 16-bit types) or 32 lanes (4 each, f32).  Threads are numbered through
+// [rows, blocks of 128, lanes] (a row may end inside a block), and each takes kAhead places a stride apart, all loaded
+// before the first is used.
+constexpr int kAhead = 4;
 template <int ELEM>
 __global__ void __launch_bounds__(kThreads) checkpointPackVectorKernel(const __grid_constant__ CheckpointPackLaunch p) {
   gridDependencyPrologue();
   constexpr int VEC = ElemOf<ELEM>::kVec;
   constexpr int kLanes = kCheckpointBlock / VEC;
   const int cols = static_cast<int>(p.cols);
-  const int64_t blocks = (cols + kCheckpointBlock - 1) / kCheckpointBlock;
+  const unsigned int blocks = static_cast<unsigned int>((cols + kCheckpointBlock - 1) / kCheckpointBlock);
   const int64_t units = p.rows * blocks * kLanes;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
   // whole warps go round together: the bound is rounded up to a warp
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; u < (units + 31) / 32 * 32; u += step) {
-    const int64_t block = u / kLanes, row = block / blocks;
-    const int b = static_cast<int>(block - row * blocks);
-    const int col = b * kCheckpointBlock + static_cast<int>(u & (kLanes - 1)) * VEC;
-    const bool live = u < units && col < cols;
-    float v[VEC];
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * (kThreads * kAhead) + threadIdx.x; base < (units + 31) / 32 * 32;
+       base += static_cast<int64_t>(gridDim.x) * (kThreads * kAhead)) {
+    uint4 raw[kAhead];
+    int64_t row[kAhead];
+    int col[kAhead];
+    bool live[kAhead];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = 0.0f;
-    if (live) loadElems<ELEM, VEC>(p.x.base, row * p.x.ld + col, v);
-    float top = 0.0f;
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t u = base + i * kThreads, block = u / kLanes;
+      // the division by the row's blocks in 32 bits where the count allows
+      row[i] = block <= 0xffffffffll ? static_cast<unsigned int>(block) / blocks : block / blocks;
+      col[i] = static_cast<int>(block - row[i] * blocks) * kCheckpointBlock + static_cast<int>(u & (kLanes - 1)) * VEC;
+      live[i] = u < units && col[i] < cols;
+      raw[i] = live[i] ? *reinterpret_cast<const uint4 *>(static_cast<const char *>(p.x.base) + (row[i] * p.x.ld + col[i]) * (16 / VEC))
+                       : make_uint4(0u, 0u, 0u, 0u);
+    }
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) top = fmaxf(top, finiteMagnitude(v[e]));
+    for (int i = 0; i < kAhead; ++i) {
+      float v[VEC];
+      unpack<ELEM, VEC>(raw[i], v);
+      float top = 0.0f;
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (!live) continue;
-    const int e8 = checkpointExponent<ELEM>(top);
-    const CheckpointScale s = checkpointScale<ELEM>(e8);
+      for (int e = 0; e < VEC; ++e) top = fmaxf(top, finiteMagnitude(v[e]));
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = scaledForCode(v[e], s);
-    storeCodes<VEC>(p.out.codes + row * p.out.codesLd + col, v);
-    if ((u & (kLanes - 1)) == 0) p.out.exps[row * p.out.expsLd + b] = static_cast<uint8_t>(e8);
+      for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (!live[i]) continue;
+      const int e8 = checkpointExponent<ELEM>(top);
+      const CheckpointScale s = checkpointScale<ELEM>(e8);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] = scaledForCode(v[e], s);
+      storeCodes<VEC>(p.out.codes + row[i] * p.out.codesLd + col[i], v);
+      if (col[i] % kCheckpointBlock == 0) p.out.exps[row[i] * p.out.expsLd + col[i] / kCheckpointBlock] = static_cast<uint8_t>(e8);
+    }
   }
 }
 
@@ -121,7 +134,7 @@ int launchCheckpointPack(const CheckpointPackLaunch &l, cudaStream_t stream, int
   cudaError_t e;
   if (vector) {
     const auto kernel = l.elemType == kF32 ? checkpointPackVectorKernel<kF32> : l.elemType == kF16 ? checkpointPackVectorKernel<kF16> : checkpointPackVectorKernel<kBF16>;
-    e = launchDependent(kernel, dim3(gridFor(l.rows * blocks * (kCheckpointBlock / vec), kThreads)), dim3(kThreads), 0, stream, l);
+    e = launchDependent(kernel, dim3(gridFor(l.rows * blocks * (kCheckpointBlock / vec), kThreads * kAhead)), dim3(kThreads), 0, stream, l);
   } else {
     const auto kernel = l.elemType == kF32 ? checkpointPackScalarKernel<kF32> : l.elemType == kF16 ? checkpointPackScalarKernel<kF16> : checkpointPackScalarKernel<kBF16>;
     e = launchDependent(kernel, dim3(gridFor(l.rows * blocks, kThreads / 32)), dim3(kThreads), 0, stream, l);
