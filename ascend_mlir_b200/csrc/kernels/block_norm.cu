@@ -142,6 +142,16 @@ TeamShape gradShape(int elemType, int kind, int64_t cols, bool vector) {
   return shapeOf(vec, nv, cols);
 }
 
+GradAheadKernel aheadKernel(int elemType, int kind, int pass, int gate, int nv) {
+  if (kind == kLayerNorm)
+    return elemType == kF32   ? gradAheadKernel<kF32, kLayerNorm>(pass, gate, nv)
+           : elemType == kF16 ? gradAheadKernel<kF16, kLayerNorm>(pass, gate, nv)
+                              : gradAheadKernel<kBF16, kLayerNorm>(pass, gate, nv);
+  return elemType == kF32   ? gradAheadKernel<kF32, kRmsNorm>(pass, gate, nv)
+         : elemType == kF16 ? gradAheadKernel<kF16, kRmsNorm>(pass, gate, nv)
+                            : gradAheadKernel<kBF16, kRmsNorm>(pass, gate, nv);
+}
+
 bool rowsAligned(const void *base, int64_t ld, int64_t elemBytes, int64_t bytes) {
   return !base || ((reinterpret_cast<uintptr_t>(base) % static_cast<uintptr_t>(bytes)) == 0 && (ld * elemBytes) % bytes == 0);
 }
@@ -262,10 +272,7 @@ int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *
     constexpr size_t kAheadBytesPerSm = 200 * 1024, kAheadBytesPerCta = 220 * 1024;
     const int stages = static_cast<int>(std::min<size_t>(4, std::max<size_t>(2, kAheadBytesPerSm / (rowBytes * threadsPerSm))));
     const size_t slotBytes = static_cast<size_t>(stages) * rowBytes * threads;
-    const GradAheadKernel ahead = !vector || slotBytes > kAheadBytesPerCta ? nullptr
-                                  : l.elemType == kF32                      ? gradAheadKernel<kF32>(l.kind, l.pass, s.nv)
-                                  : l.elemType == kF16                      ? gradAheadKernel<kF16>(l.kind, l.pass, s.nv)
-                                                                            : gradAheadKernel<kBF16>(l.kind, l.pass, s.nv);
+    const GradAheadKernel ahead = vector && slotBytes <= kAheadBytesPerCta ? aheadKernel(l.elemType, l.kind, l.pass, l.gateForm, s.nv) : nullptr;
     cudaError_t e;
     if (ahead) {
       if (e = reserveSharedMemory(reinterpret_cast<const void *>(ahead), static_cast<int>(kAheadBytesPerCta)); e != cudaSuccess) return e;

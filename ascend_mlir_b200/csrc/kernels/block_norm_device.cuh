@@ -188,18 +188,6 @@ __device__ __forceinline__ float2 valuePair(unsigned int codes, float power) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
   return make_float2(f.x * power, f.y * power);
 }
-template <int VEC> __device__ __forceinline__ void storeCodes(uint8_t *p, const float (&scaled)[VEC]) {
-  if constexpr (VEC == 1) {
-    *p = static_cast<uint8_t>(codePair(scaled[0], 0.0f) & 0xffu);
-  } else {
-    unsigned int w[VEC / 4];
-#pragma unroll
-    for (int i = 0; i < VEC / 4; ++i)
-      w[i] = codePair(scaled[4 * i], scaled[4 * i + 1]) | (codePair(scaled[4 * i + 2], scaled[4 * i + 3]) << 16);
-    if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
-    else *reinterpret_cast<unsigned int *>(p) = w[0];
-  }
-}
 template <int VEC> __device__ __forceinline__ void valuesOfCodes(const unsigned int (&w)[VEC / 4 > 0 ? VEC / 4 : 1], float power, float (&v)[VEC]) {
   if constexpr (VEC == 1) {
     v[0] = valuePair(w[0] & 0xffu, power).x;

@@ -94,32 +94,6 @@ __device__ __forceinline__ void normPairs(F2 (&v)[kPairs<ELEM>], F2 shift, F2 rs
   }
 }
 
-// The 8-bit checkpoint of a vector.  128 columns are 128 / VEC neighbouring lanes: the largest magnitude is a shuffle
-// tree over them.
-template <int ELEM>
-__device__ __forceinline__ void storeCheckpointVector(const F2 (&p)[kPairs<ELEM>], int col, int cols, const CheckpointOut &c, int64_t row) {
-  constexpr int VEC = ElemOf<ELEM>::kVec, kGroup = kCheckpointBlock / VEC;
-  float v[VEC];
-#pragma unroll
-  for (int e = 0; e < VEC / 2; ++e) {
-    const float2 f = valuesOf(p[e]);
-    v[2 * e] = f.x;
-    v[2 * e + 1] = f.y;
-  }
-  float top = 0.0f;
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) top = fmaxf(top, finiteMagnitude(v[e]));
-#pragma unroll
-  for (int o = kGroup / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (col >= cols) return;
-  const int e8 = checkpointExponent<ELEM>(top);
-  const CheckpointScale s = checkpointScale<ELEM>(e8);
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) v[e] = scaledForCode(v[e], s);
-  storeCodes<VEC>(c.codes + row * c.codesLd + col, v);
-  if (col % kCheckpointBlock == 0) c.exps[row * c.expsLd + col / kCheckpointBlock] = static_cast<uint8_t>(e8);
-}
-
 template <int ELEM, int KIND, int PASS, int NV>
 __global__ void __launch_bounds__(512) blockNormForwardVectorKernel(const __grid_constant__ BlockNormLaunch p, int teamLanes) {
   gridDependencyPrologue();
@@ -153,7 +127,7 @@ __global__ void __launch_bounds__(512) blockNormForwardVectorKernel(const __grid
     for (int i = 0; i < NV; ++i) widenPairs<ELEM>(raw0[i], v[i]);
     if (p.checkpoint.codes) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) storeCheckpointVector<ELEM>(v[i], colOf(i), cols, p.checkpoint, row);
+      for (int i = 0; i < NV; ++i) packVector<ELEM>(raw0[i], colOf(i) < cols, colOf(i), row, p.checkpoint);
     }
     float mean, rstd;
     pairStatistics<ELEM, KIND, NV>(team, v, cols, PASS == kPre ? p.epsB : p.epsA, mean, rstd);

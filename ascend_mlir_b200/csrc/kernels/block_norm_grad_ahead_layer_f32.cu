@@ -1,0 +1,7 @@
+#include "kernels/block_norm_grad_ahead_pick.cuh"
+
+namespace afir {
+namespace kernels {
+template GradAheadKernel gradAheadKernel<kF32, kLayerNorm>(int pass, int gate, int nv);
+} // namespace kernels
+} // namespace afir

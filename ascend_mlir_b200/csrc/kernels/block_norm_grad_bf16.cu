@@ -3,6 +3,5 @@
 namespace afir {
 namespace kernels {
 template GradKernel gradKernel<kBF16>(int kind, int pass, bool vector, int nv);
-template GradAheadKernel gradAheadKernel<kBF16>(int kind, int pass, int nv);
 } // namespace kernels
 } // namespace afir

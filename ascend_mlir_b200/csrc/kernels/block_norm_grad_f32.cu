@@ -3,6 +3,5 @@
 namespace afir {
 namespace kernels {
 template GradKernel gradKernel<kF32>(int kind, int pass, bool vector, int nv);
-template GradAheadKernel gradAheadKernel<kF32>(int kind, int pass, int nv);
 } // namespace kernels
 } // namespace afir

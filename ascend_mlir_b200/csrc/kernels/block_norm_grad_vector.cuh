@@ -37,14 +37,15 @@ struct RowCursor {
   }
 };
 
-template <int ELEM, int KIND, int PASS, int NV>
+// GATE: GateForm (kGateNone for kPre).
+template <int ELEM, int KIND, int PASS, int GATE, int NV>
 __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_constant__ BlockNormGradLaunch p, const __grid_constant__ GradPlan plan,
                                                                  int teamLanes, int stages) {
   gridDependencyPrologue();
   constexpr bool kLayer = KIND == kLayerNorm;
   constexpr int kValues = kLayer ? 2 : 1;
-  constexpr bool kPostPart = PASS != kPre, kPrePart = PASS != kPost;
-  constexpr int VEC = ElemOf<ELEM>::kVec, P = kPairs<ELEM>;
+  constexpr bool kPostPart = PASS != kPre, kPrePart = PASS != kPost, kToken = GATE == kGateToken;
+  constexpr int VEC = ElemOf<ELEM>::kVec, P = kPairs<ELEM>, EB = 16 / VEC;
   extern __shared__ uint4 slots[];  // [stages][tensors][NV][threads]
   __shared__ float scratch[kTeamScratchFloats];
   Team team = makeTeam(teamLanes, scratch);
@@ -53,49 +54,60 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
   const int teamIndex = static_cast<int>(blockIdx.x) * team.count + team.index, rows = static_cast<int>(p.rows);
   if (teamIndex >= plan.teams) return;
 
-  // which tensor has which slot
-  const bool packed = p.checkpoint.codes != nullptr;
-  const bool token = kPostPart && p.gateForm == kGateToken;
-  int tensors = 0;
-  const int slotDh = tensors;
-  if (kPrePart) ++tensors;
-  const int slotSource = tensors;
-  if (kPrePart) ++tensors;
-  const int slotDout = tensors;
-  if (p.dout.base) ++tensors;
-  const int slotY = tensors;
-  if (kPostPart) ++tensors;
-  const int slotGate = tensors;
-  if (token) ++tensors;
-  const int threads = static_cast<int>(blockDim.x);
-  auto slot = [&](int stage, int tensor, int i) -> uint4 * { return slots + ((stage * tensors + tensor) * NV + i) * threads + threadIdx.x; };
-  auto colOf = [&](int i) { return (i * team.lanes + team.lane) * VEC; };
-
-  auto fetch = [&](const RowCursor &c, int stage) {
-    if (c.live(plan)) {
+  // A thread's columns: VEC from col0, and again every `apart` columns.
+  const int col0 = team.lane * VEC, apart = team.lanes * VEC;
+  bool has[NV];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int col = colOf(i);
-        if (col >= cols) continue;
-        constexpr int eb = 16 / VEC;
-        auto vectors = [&](int tensor, const RowsIn &r) { copyAhead16(slot(stage, tensor, i), static_cast<const char *>(r.base) + (static_cast<int64_t>(c.row) * r.ld + col) * eb); };
-        auto codes = [&](int tensor) {
-          const uint8_t *from = p.checkpoint.codes + static_cast<int64_t>(c.row) * p.checkpoint.codesLd + col;
-          if constexpr (VEC == 8) copyAhead8(slot(stage, tensor, i), from);
-          else copyAhead4(slot(stage, tensor, i), from);
-        };
-        if constexpr (kPrePart) {
-          vectors(slotDh, p.dh);
-          if (PASS == kPre && packed) codes(slotSource);
-          else vectors(slotSource, p.source);
+  for (int i = 0; i < NV; ++i) has[i] = col0 + i * apart < cols;
+
+  // Slots by byte: tensors present get one each, in this order.
+  const bool packed = p.checkpoint.codes != nullptr, hasDout = p.dout.base != nullptr;
+  const unsigned int perTensor = NV * blockDim.x * 16, perVector = blockDim.x * 16;
+  unsigned int used = 0;
+  const unsigned int atDh = used;
+  if (kPrePart) used += perTensor;
+  const unsigned int atSource = used;
+  if (kPrePart) used += perTensor;
+  const unsigned int atDout = used;
+  if (hasDout) used += perTensor;
+  const unsigned int atY = used;
+  if (kPostPart) used += perTensor;
+  const unsigned int atGate = used;
+  if (kToken) used += perTensor;
+  const unsigned int slot0 = static_cast<unsigned int>(__cvta_generic_to_shared(slots)) + threadIdx.x * 16, slotEnd = slot0 + stages * used;
+
+  auto rowOf = [&](const RowsIn &r, int row) { return static_cast<const char *>(r.base) + (static_cast<int64_t>(row) * r.ld + col0) * EB; };
+  auto rowTo = [&](const RowsOut &r, int row) { return static_cast<char *>(r.base) + (static_cast<int64_t>(row) * r.ld + col0) * EB; };
+  auto store = [&](char *to, int i, const F2 (&v)[P]) { *reinterpret_cast<uint4 *>(to + i * apart * EB) = narrowPairs<ELEM>(v); };
+
+  auto fetch = [&](const RowCursor &c, unsigned int slot) {
+    if (c.live(plan)) {
+      auto vectors = [&](unsigned int at, const RowsIn &r) {
+        const char *from = rowOf(r, c.row);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (has[i]) copyAhead16(slot + at + i * perVector, from + i * apart * EB);
+      };
+      auto codes = [&](unsigned int at) {
+        const uint8_t *from = p.checkpoint.codes + static_cast<int64_t>(c.row) * p.checkpoint.codesLd + col0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          if (!has[i]) continue;
+          if constexpr (VEC == 8) copyAhead8(slot + at + i * perVector, from + i * apart);
+          else copyAhead4(slot + at + i * perVector, from + i * apart);
         }
-        if (p.dout.base) vectors(slotDout, p.dout);
-        if constexpr (kPostPart) {
-          if (packed) codes(slotY);
-          else vectors(slotY, p.y);
-        }
-        if (token) vectors(slotGate, p.gate);
+      };
+      if constexpr (kPrePart) {
+        vectors(atDh, p.dh);
+        if (PASS == kPre && packed) codes(atSource);
+        else vectors(atSource, p.source);
       }
+      if (hasDout) vectors(atDout, p.dout);
+      if constexpr (kPostPart) {
+        if (packed) codes(atY);
+        else vectors(atY, p.y);
+      }
+      if constexpr (kToken) vectors(atGate, p.gate);
     }
     copiesCommit();  // an empty group where there is no row: the count stays the number of rows ahead
   };
@@ -114,7 +126,7 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
     if (packed) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (colOf(i) < cols) s.exps[i] = __ldg(p.checkpoint.exps + static_cast<int64_t>(c.row) * p.checkpoint.expsLd + colOf(i) / kCheckpointBlock);
+        if (has[i]) s.exps[i] = __ldg(p.checkpoint.exps + static_cast<int64_t>(c.row) * p.checkpoint.expsLd + (col0 + i * apart) / kCheckpointBlock);
     }
   };
 
@@ -124,7 +136,7 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
   ahead = now;
   RowScalars next = {};
   fetchScalars(now, next);
-  for (int s = 0; s < stages; ++s) {
+  for (unsigned int s = slot0; s < slotEnd; s += used) {
     fetch(ahead, s);
     ahead.advance(plan, rows);
   }
@@ -147,20 +159,21 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
       reinterpret_cast<float4 *>(to)[e] = make_float4(a.x, a.y, b.x, b.y);
     }
   };
+  auto storeRunSums = [&](int run) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int k = 0; k < kValues; ++k)
+        if (has[i]) storeSumPairs(plan.sumsA + (static_cast<int64_t>(run) * kValues + k) * plan.sumsLd + col0 + i * apart, sumA[k][i]);
+  };
 
-  if constexpr (kPostPart) {  // runs without rows: sums of nothing
+  if constexpr (GATE == kGateGroup) {  // runs without rows, of a short last group: sums of nothing
     RowCursor c;
-    for (c.enter(plan, rows, teamIndex); c.live(plan); c.enter(plan, rows, c.run + plan.teams)) {
-      if (c.row < c.end) continue;
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int k = 0; k < kValues; ++k)
-          if (colOf(i) < cols) storeSumPairs(plan.sumsA + (static_cast<int64_t>(c.run) * kValues + k) * plan.sumsLd + colOf(i), sumA[k][i]);
-    }
+    for (c.enter(plan, rows, teamIndex); c.live(plan); c.enter(plan, rows, c.run + plan.teams))
+      if (c.row >= c.end) storeRunSums(c.run);
   }
 
-  int stage = 0;
+  unsigned int slot = slot0;
   while (now.live(plan)) {
     const RowScalars at = next;
     const int row = now.row, run = now.run, group = now.group;
@@ -176,12 +189,13 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
       for (int k = 0; k < kValues; ++k) s[k] = zero;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        if (colOf(i) >= cols) continue;
+        if (!has[i]) continue;
         F2 w[P];
-        if (PASS == kPre && packed) codePairs<ELEM>(*reinterpret_cast<const uint2 *>(slot(stage, slotSource, i)), at.exps[i], n[i]);
-        else widenPairs<ELEM>(*slot(stage, slotSource, i), n[i]);
-        widenPairs<ELEM>(*slot(stage, slotDh, i), dz[i]);
-        loadParamPairs<ELEM>(p.b.weight, p.paramType, colOf(i), w);
+        const uint4 raw = readSlot(slot + atSource + i * perVector);
+        if (PASS == kPre && packed) codePairs<ELEM>(make_uint2(raw.x, raw.y), at.exps[i], n[i]);
+        else widenPairs<ELEM>(raw, n[i]);
+        widenPairs<ELEM>(readSlot(slot + atDh + i * perVector), dz[i]);
+        loadParamPairs<ELEM>(p.b.weight, p.paramType, col0 + i * apart, w);
 #pragma unroll
         for (int e = 0; e < P; ++e) {
           n[i][e] = kLayer ? (n[i][e] + shift) * rstd : n[i][e] * rstd;
@@ -200,85 +214,94 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
       const F2 constant = splat(kLayer ? -total[kValues - 1] * share * at.rstdB : 0.0f);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        if (colOf(i) >= cols) continue;
-        F2 t[P];
-        if (p.dout.base) widenPairs<ELEM>(*slot(stage, slotDout, i), t);
-        else {
+        if (!has[i]) continue;
+        if (hasDout) {
+          F2 t[P];
+          widenPairs<ELEM>(readSlot(slot + atDout + i * perVector), t);
 #pragma unroll
-          for (int e = 0; e < P; ++e) t[e] = zero;
-        }
+          for (int e = 0; e < P; ++e) {
+            if constexpr (kLayer) t[e] = t[e] + constant;
+            dz[i][e] = fma2(dz[i][e], rstd, fma2(n[i][e], along, t[e]));
+          }
+        } else {
 #pragma unroll
-        for (int e = 0; e < P; ++e) {
-          if constexpr (kLayer) t[e] = t[e] + constant;
-          dz[i][e] = fma2(dz[i][e], rstd, fma2(n[i][e], along, t[e]));
+          for (int e = 0; e < P; ++e) dz[i][e] = fma2(dz[i][e], rstd, kLayer ? fma2(n[i][e], along, constant) : n[i][e] * along);
         }
       }
     } else {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (colOf(i) < cols) widenPairs<ELEM>(*slot(stage, slotDout, i), dz[i]);
+        if (has[i]) widenPairs<ELEM>(readSlot(slot + atDout + i * perVector), dz[i]);
     }
 
     if constexpr (!kPostPart) {
-      fetch(ahead, stage);
+      fetch(ahead, slot);
       ahead.advance(plan, rows);
+      char *to = rowTo(p.dx, row);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (colOf(i) < cols) storePairs<ELEM>(p.dx.base, static_cast<int64_t>(row) * p.dx.ld + colOf(i), dz[i]);
+        if (has[i]) store(to, i, dz[i]);
     } else {
       const F2 rstd = splat(at.rstdA), shift = splat(kLayer ? -at.meanA : 0.0f), alpha = splat(p.alpha);
       F2 s[kValues];
 #pragma unroll
       for (int k = 0; k < kValues; ++k) s[k] = zero;
+      char *toDx = rowTo(p.dx, row), *toDgate = kToken ? rowTo(p.dgate, row) : nullptr;
+      const char *gateRow = GATE == kGateGroup ? rowOf(p.gate, group) : nullptr;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int col = colOf(i);
-        if (col >= cols) continue;
-        F2 t[P], w[P];
-        if (packed) codePairs<ELEM>(*reinterpret_cast<const uint2 *>(slot(stage, slotY, i)), at.exps[i], n[i]);
-        else widenPairs<ELEM>(*slot(stage, slotY, i), n[i]);
+        if (!has[i]) continue;
+        const int col = col0 + i * apart;
+        F2 t[P], w[P], scaled[P];  // scaled: the stream's gradient times the residual scale
+        const uint4 raw = readSlot(slot + atY + i * perVector);
+        if (packed) codePairs<ELEM>(make_uint2(raw.x, raw.y), at.exps[i], n[i]);
+        else widenPairs<ELEM>(raw, n[i]);
 #pragma unroll
         for (int e = 0; e < P; ++e) {
           n[i][e] = kLayer ? (n[i][e] + shift) * rstd : n[i][e] * rstd;
           t[e] = dz[i][e] * alpha;
+          scaled[e] = dz[i][e];
         }
-        storePairs<ELEM>(p.dx.base, static_cast<int64_t>(row) * p.dx.ld + col, t);
-        loadParamPairs<ELEM>(p.a.weight, p.paramType, col, w);
-        F2 scale[P];
-        if (p.scale) loadParamPairs<ELEM>(p.scale, p.paramType, col, scale);
-        else {
+        store(toDx, i, t);
+        if (p.scale) {
+          loadParamPairs<ELEM>(p.scale, p.paramType, col, t);
 #pragma unroll
-          for (int e = 0; e < P; ++e) scale[e] = splat(1.0f);
+          for (int e = 0; e < P; ++e) scaled[e] = scaled[e] * t[e];
         }
-        if (p.gateForm == kGateNone) {
+        loadParamPairs<ELEM>(p.a.weight, p.paramType, col, w);
+        if constexpr (GATE == kGateNone) {
 #pragma unroll
           for (int e = 0; e < P; ++e) {
             sumA[0][i][e] = fma2(dz[i][e], n[i][e], sumA[0][i][e]);
             if constexpr (kLayer) sumA[1][i][e] = sumA[1][i][e] + dz[i][e];
-            dz[i][e] = dz[i][e] * (scale[e] * w[e]);
+            dz[i][e] = scaled[e] * w[e];
           }
         } else {
           F2 a[P];
-          if (token) widenPairs<ELEM>(*slot(stage, slotGate, i), a);
-          else loadPairs<ELEM>(p.gate.base, static_cast<int64_t>(group) * p.gate.ld + col, a);
+          if constexpr (kToken) widenPairs<ELEM>(readSlot(slot + atGate + i * perVector), a);
+          else widenPairs<ELEM>(*reinterpret_cast<const uint4 *>(gateRow + i * apart * EB), a);
           gatePairs(a, p.gateAct);
-          if (token) {
+          if constexpr (kToken) {
             F2 u[P];
             if constexpr (kLayer) loadParamPairs<ELEM>(p.a.bias, p.paramType, col, u);
 #pragma unroll
             for (int e = 0; e < P; ++e) {
               u[e] = kLayer ? fma2(n[i][e], w[e], u[e]) : n[i][e] * w[e];
-              t[e] = dz[i][e] * scale[e] * u[e] * gateSlopePair(a[e], p.gateAct);
+              t[e] = scaled[e] * u[e] * gateSlopePair(a[e], p.gateAct);
+              const F2 gated = dz[i][e] * a[e];
+              sumA[0][i][e] = fma2(gated, n[i][e], sumA[0][i][e]);
+              if constexpr (kLayer) sumA[1][i][e] = sumA[1][i][e] + gated;
             }
-            storePairs<ELEM>(p.dgate.base, static_cast<int64_t>(row) * p.dgate.ld + col, t);
+            store(toDgate, i, t);
+          } else {
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+              sumA[0][i][e] = fma2(dz[i][e], n[i][e], sumA[0][i][e]);
+              if constexpr (kLayer) sumA[1][i][e] = sumA[1][i][e] + dz[i][e];
+            }
           }
 #pragma unroll
-          for (int e = 0; e < P; ++e) {
-            const F2 gated = dz[i][e] * a[e], forSums = token ? gated : dz[i][e];
-            sumA[0][i][e] = fma2(forSums, n[i][e], sumA[0][i][e]);
-            if constexpr (kLayer) sumA[1][i][e] = sumA[1][i][e] + forSums;
-            dz[i][e] = gated * (scale[e] * w[e]);
-          }
+          for (int e = 0; e < P; ++e) dz[i][e] = scaled[e] * (a[e] * w[e]);
         }
 #pragma unroll
         for (int e = 0; e < P; ++e) {
@@ -286,7 +309,7 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
           if constexpr (kLayer) s[1] = s[1] + dz[i][e];
         }
       }
-      fetch(ahead, stage);  // this row's slots have been read
+      fetch(ahead, slot);  // this row's slots have been read
       ahead.advance(plan, rows);
       float total[kValues];
 #pragma unroll
@@ -294,38 +317,32 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
       teamSum(team, total);
       const F2 along = splat(-total[0] * share * at.rstdA);
       const F2 constant = splat(kLayer ? -total[kValues - 1] * share * at.rstdA : 0.0f);
+      char *toDy = rowTo(p.dy, row);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        if (colOf(i) >= cols) continue;
+        if (!has[i]) continue;
 #pragma unroll
-        for (int e = 0; e < P; ++e) {
-          F2 t = kLayer ? fma2(n[i][e], along, constant) : n[i][e] * along;
-          n[i][e] = fma2(dz[i][e], rstd, t);
-        }
-        storePairs<ELEM>(p.dy.base, static_cast<int64_t>(row) * p.dy.ld + colOf(i), n[i]);
+        for (int e = 0; e < P; ++e) n[i][e] = fma2(dz[i][e], rstd, kLayer ? fma2(n[i][e], along, constant) : n[i][e] * along);
+        store(toDy, i, n[i]);
       }
       if (now.run != run) {  // the run ends here: leave its sums and begin the next one's
+        storeRunSums(run);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          if (colOf(i) < cols) {
-#pragma unroll
-            for (int k = 0; k < kValues; ++k) storeSumPairs(plan.sumsA + (static_cast<int64_t>(run) * kValues + k) * plan.sumsLd + colOf(i), sumA[k][i]);
-          }
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
           for (int k = 0; k < kValues; ++k)
 #pragma unroll
             for (int e = 0; e < P; ++e) sumA[k][i][e] = zero;
-        }
       }
     }
-    stage = stage + 1 == stages ? 0 : stage + 1;
+    slot = slot + used == slotEnd ? slot0 : slot + used;
   }
   if constexpr (kPrePart) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (colOf(i) >= cols) continue;
+      if (!has[i]) continue;
 #pragma unroll
-      for (int k = 0; k < kValues; ++k) storeSumPairs(plan.sumsB + (static_cast<int64_t>(teamIndex) * kValues + k) * plan.sumsLd + colOf(i), sumB[k][i]);
+      for (int k = 0; k < kValues; ++k) storeSumPairs(plan.sumsB + (static_cast<int64_t>(teamIndex) * kValues + k) * plan.sumsLd + col0 + i * apart, sumB[k][i]);
     }
   }
 }

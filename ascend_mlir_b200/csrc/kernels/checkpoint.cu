@@ -7,8 +7,8 @@
 
 #include <algorithm>
 
-#include "kernels/block_norm_device.cuh"
 #include "kernels/launch_util.h"
+#include "kernels/pairs.cuh"
 
 namespace afir {
 namespace kernels {
@@ -46,22 +46,7 @@ __global__ void __launch_bounds__(kThreads) checkpointPackVectorKernel(const __g
                        : make_uint4(0u, 0u, 0u, 0u);
     }
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      float v[VEC];
-      unpack<ELEM, VEC>(raw[i], v);
-      float top = 0.0f;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) top = fmaxf(top, finiteMagnitude(v[e]));
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (!live[i]) continue;
-      const int e8 = checkpointExponent<ELEM>(top);
-      const CheckpointScale s = checkpointScale<ELEM>(e8);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = scaledForCode(v[e], s);
-      storeCodes<VEC>(p.out.codes + row[i] * p.out.codesLd + col[i], v);
-      if (col[i] % kCheckpointBlock == 0) p.out.exps[row[i] * p.out.expsLd + col[i] / kCheckpointBlock] = static_cast<uint8_t>(e8);
-    }
+    for (int i = 0; i < kAhead; ++i) packVector<ELEM>(raw[i], live[i], col[i], row[i], p.out);
   }
 }
 
@@ -93,7 +78,7 @@ __global__ void __launch_bounds__(kThreads) checkpointPackScalarKernel(const __g
       const int col = b * kCheckpointBlock + i * 32 + lane;
       if (col >= cols) continue;
       v[i][0] = scaledForCode(v[i][0], s);
-      storeCodes<1>(p.out.codes + row * p.out.codesLd + col, v[i]);
+      p.out.codes[row * p.out.codesLd + col] = static_cast<uint8_t>(codePair(v[i][0], 0.0f) & 0xffu);
     }
     if (lane == 0) p.out.exps[row * p.out.expsLd + b] = static_cast<uint8_t>(e8);
   }

@@ -2,6 +2,8 @@
 // the arithmetic of row kernels that would otherwise be bound by the number of instructions they issue.
 #pragma once
 
+#include <type_traits>
+
 #include "kernels/block_norm_device.cuh"
 
 namespace afir {
@@ -114,13 +116,19 @@ template <int ELEM> __device__ __forceinline__ void codePairs(const uint2 &raw, 
   }
 }
 // act(gate) of a vector in place; the derivative from the value.  The row kernels' sigmoid takes the hardware's exponential
-// and reciprocal (a few units in the last place of f32, far below a 16-bit step).
+// and reciprocal directly (2 and 1 units in the last place; beyond |g| = 87 it is 0 or 1, as f32's own would be to 1e-38).
+__device__ __forceinline__ float sigmoidOf(float g) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return r;
+}
 template <int N> __device__ __forceinline__ void gatePairs(F2 (&g)[N], int act) {
   if (act == kActNone) return;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const float2 f = valuesOf(g[i]);
-    if (act == kActSigmoid) g[i] = pairOf(__fdividef(1.0f, 1.0f + __expf(-f.x)), __fdividef(1.0f, 1.0f + __expf(-f.y)));
+    if (act == kActSigmoid) g[i] = pairOf(sigmoidOf(f.x), sigmoidOf(f.y));
     else g[i] = pairOf(tanhf(f.x), tanhf(f.y));
   }
 }
@@ -131,17 +139,93 @@ __device__ __forceinline__ F2 gateSlopePair(F2 a, int act) {
   return one;
 }
 
+// ---- packing a vector -----------------------------------------------------------------------------------------------
+// Largest magnitude among 16 bytes of elements, NaN left out; 16-bit types compare as they are, two at a time.
+template <int ELEM> __device__ __forceinline__ float largestMagnitude(const uint4 &raw) {
+  if constexpr (ELEM == kF32) {
+    return fmaxf(fmaxf(fabsf(__uint_as_float(raw.x)), fabsf(__uint_as_float(raw.y))), fmaxf(fabsf(__uint_as_float(raw.z)), fabsf(__uint_as_float(raw.w))));
+  } else {
+    using T2 = typename std::conditional<ELEM == kF16, __half2, __nv_bfloat162>::type;
+    const unsigned int w[4] = {raw.x & 0x7fff7fffu, raw.y & 0x7fff7fffu, raw.z & 0x7fff7fffu, raw.w & 0x7fff7fffu};
+    const T2 *v = reinterpret_cast<const T2 *>(w);
+    const T2 m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
+    return fmaxf(ElemOf<ELEM>::widen(m.x), ElemOf<ELEM>::widen(m.y));
+  }
+}
+// A vector's part of a checkpoint: the lanes of a block of 128 columns (128 / VEC neighbours, all lanes of the warp take
+// part) agree on the power, each stores its codes, the block's first the exponent.  In the ordinary case, no infinity in
+// the block and no magnitude that needs the highest power, a code is one product and one conversion: the power brings
+// every magnitude to 448 or less.  (f16 multiplies in f16: a product below its normal range is below the smallest code's
+// half step as well.)
+template <int ELEM>
+__device__ __forceinline__ void packVector(const uint4 &raw, bool live, int col, int64_t row, const CheckpointOut &c) {
+  constexpr int VEC = ElemOf<ELEM>::kVec, kGroup = kCheckpointBlock / VEC, W = VEC / 4;
+  float top = largestMagnitude<ELEM>(raw);
+#pragma unroll
+  for (int o = kGroup / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  int e8 = checkpointExponent<ELEM>(top);
+  unsigned int codes[W];
+  if (!__any_sync(0xffffffffu, e8 == CheckpointRange<ELEM>::kHigh)) {
+    const float inverse = powerOfExponent(254 - e8);
+    if constexpr (ELEM == kF16) {
+      const __half2 scale = __float2half2_rn(inverse);
+      const __half2 *v = reinterpret_cast<const __half2 *>(&raw);
+      unsigned int q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __half2 r = __hmul2(v[i], scale);
+        q[i] = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(r), __NV_SATFINITE, __NV_E4M3);
+      }
+      codes[0] = q[0] | (q[1] << 16);
+      if constexpr (W > 1) codes[W - 1] = q[2] | (q[3] << 16);
+    } else {
+      F2 v[VEC / 2];
+      widenPairs<ELEM>(raw, v);
+      const F2 scale = splat(inverse);
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const float2 lo = valuesOf(v[2 * i] * scale), hi = valuesOf(v[2 * i + 1] * scale);
+        codes[i] = codePair(lo.x, lo.y) | (codePair(hi.x, hi.y) << 16);
+      }
+    }
+  } else {
+    float v[VEC];
+    unpack<ELEM, VEC>(raw, v);
+    top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) top = fmaxf(top, finiteMagnitude(v[e]));
+#pragma unroll
+    for (int o = kGroup / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    e8 = checkpointExponent<ELEM>(top);
+    const CheckpointScale s = checkpointScale<ELEM>(e8);
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+      codes[i] = codePair(scaledForCode(v[4 * i], s), scaledForCode(v[4 * i + 1], s)) |
+                 (codePair(scaledForCode(v[4 * i + 2], s), scaledForCode(v[4 * i + 3], s)) << 16);
+  }
+  if (!live) return;
+  uint8_t *to = c.codes + row * c.codesLd + col;
+  if constexpr (W == 2) *reinterpret_cast<uint2 *>(to) = make_uint2(codes[0], codes[W - 1]);
+  else *reinterpret_cast<unsigned int *>(to) = codes[0];
+  if (col % kCheckpointBlock == 0) c.exps[row * c.expsLd + col / kCheckpointBlock] = static_cast<uint8_t>(e8);
+}
+
 // ---- rows fetched ahead -------------------------------------------------------------------------------------------
 // Every thread copies the very vectors that it will use into slots of its own in shared memory, asynchronously and
 // several rows ahead, so that nothing has to be signalled between threads: waiting for one's own copies is enough.
-__device__ __forceinline__ void copyAhead16(void *slot, const void *from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<unsigned int>(__cvta_generic_to_shared(slot))), "l"(from) : "memory");
+__device__ __forceinline__ void copyAhead16(unsigned int slot, const void *from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot), "l"(from) : "memory");
 }
-__device__ __forceinline__ void copyAhead8(void *slot, const void *from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(static_cast<unsigned int>(__cvta_generic_to_shared(slot))), "l"(from) : "memory");
+__device__ __forceinline__ void copyAhead8(unsigned int slot, const void *from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(slot), "l"(from) : "memory");
 }
-__device__ __forceinline__ void copyAhead4(void *slot, const void *from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<unsigned int>(__cvta_generic_to_shared(slot))), "l"(from) : "memory");
+__device__ __forceinline__ void copyAhead4(unsigned int slot, const void *from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(slot), "l"(from) : "memory");
+}
+__device__ __forceinline__ uint4 readSlot(unsigned int slot) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(slot) : "memory");
+  return v;
 }
 __device__ __forceinline__ void copiesCommit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Until all but the newest `left` groups have arrived (left = 1, 2 or 3).
