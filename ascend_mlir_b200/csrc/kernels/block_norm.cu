@@ -130,26 +130,31 @@ TeamShape forwardShape(int elemType, int64_t rows, int64_t cols, bool vector, in
   return shapeOf(vec, nv, cols);
 }
 
-// Columns per thread of the gradient: 16 for an rms norm, 8 for a layer norm (which keeps twice the column sums) while
-// that leaves a team of at most 512 threads; beyond, what the width needs.
+// The gradient with rows fetched ahead, 512 threads per SM: two vectors per thread (one of a 16-bit layer norm, which keeps
+// twice the column sums in registers), in a team of up to 512 threads, beyond that what the width needs; fewer where
+// that makes every thread's vectors lie inside the row, which spares the kernel its tests.
 TeamShape gradShape(int elemType, int kind, int64_t cols, bool vector) {
   const int vec = vector ? (elemType == kF32 ? 4 : 8) : 1;
   if (!vector) return shapeOf(1, scalarElements(cols), cols);
-  const int64_t perThread = kind == kLayerNorm ? 8 : 16;
-  int nv = 1;
-  while (nv * vec < perThread && static_cast<int64_t>(nv) * vec * 32 < cols) nv *= 2;
+  int nv = kind == kLayerNorm && elemType != kF32 ? 1 : 2;
+  if (nv == 2 && cols % (64 * vec) != 0 && (cols % (32 * vec) == 0 || cols < 32 * vec) && cols <= 512 * vec) nv = 1;
   while (static_cast<int64_t>(nv) * vec * 512 < cols) nv *= 2;
   return shapeOf(vec, nv, cols);
 }
+// Without rows ahead: 4 vectors per thread, 8 for the widest f32 rows.
+TeamShape wideShape(int elemType, int64_t cols) {
+  const int vec = elemType == kF32 ? 4 : 8;
+  return shapeOf(vec, 4 * vec * 512 < cols ? 8 : 4, cols);
+}
 
-GradAheadKernel aheadKernel(int elemType, int kind, int pass, int gate, int nv) {
+GradAheadKernel aheadKernel(int elemType, int kind, int pass, bool token, bool full, int nv) {
   if (kind == kLayerNorm)
-    return elemType == kF32   ? gradAheadKernel<kF32, kLayerNorm>(pass, gate, nv)
-           : elemType == kF16 ? gradAheadKernel<kF16, kLayerNorm>(pass, gate, nv)
-                              : gradAheadKernel<kBF16, kLayerNorm>(pass, gate, nv);
-  return elemType == kF32   ? gradAheadKernel<kF32, kRmsNorm>(pass, gate, nv)
-         : elemType == kF16 ? gradAheadKernel<kF16, kRmsNorm>(pass, gate, nv)
-                            : gradAheadKernel<kBF16, kRmsNorm>(pass, gate, nv);
+    return elemType == kF32   ? gradAheadKernel<kF32, kLayerNorm>(pass, token, full, nv)
+           : elemType == kF16 ? gradAheadKernel<kF16, kLayerNorm>(pass, token, full, nv)
+                              : gradAheadKernel<kBF16, kLayerNorm>(pass, token, full, nv);
+  return elemType == kF32   ? gradAheadKernel<kF32, kRmsNorm>(pass, token, full, nv)
+         : elemType == kF16 ? gradAheadKernel<kF16, kRmsNorm>(pass, token, full, nv)
+                            : gradAheadKernel<kBF16, kRmsNorm>(pass, token, full, nv);
 }
 
 bool rowsAligned(const void *base, int64_t ld, int64_t elemBytes, int64_t bytes) {
@@ -157,18 +162,21 @@ bool rowsAligned(const void *base, int64_t ld, int64_t elemBytes, int64_t bytes)
 }
 bool vectorAligned(const void *base) { return (reinterpret_cast<uintptr_t>(base) & 15u) == 0; }
 
-int64_t gradTeamsPerSm(int kind, int64_t cols) {
-  return std::min<int64_t>(16, std::max<int64_t>(1, (kind == kLayerNorm ? 4096 : 8192) / cols));
+// Columns of the rows that an SM works on at once: what its threads hold, and half of that for f32 rows, of which two
+// would not fit in shared memory otherwise.
+int64_t gradTeamsPerSm(int elemType, int kind, int64_t cols) {
+  const int64_t most = (kind == kLayerNorm ? 4096 : 8192) / (elemType == kF32 ? 2 : 1);
+  return std::min<int64_t>(16, std::max<int64_t>(1, most / cols));
 }
 
-GradPlan gradPlan(int kind, int gateForm, int64_t rows, int64_t cols, int64_t groupRows, int smCount) {
+GradPlan gradPlan(int elemType, int kind, int gateForm, int64_t rows, int64_t cols, int64_t groupRows, int smCount) {
   GradPlan plan = {};
   const int64_t all = std::max<int64_t>(rows, 1);
   const int64_t perGroup = gateForm == kGateGroup ? std::min(groupRows, all) : all;
   const int64_t groups = gateForm == kGateGroup ? (rows + perGroup - 1) / perGroup : 1;
-  // 512 threads' worth of teams per SM (they have 128 registers each): enough rows under way to cover a row's two
-  // sums, few enough that the teams' sums (f32, one or two rows each) stay small beside the row tensors.
-  const int64_t teams = std::max<int64_t>(1, std::min<int64_t>(rows, smCount * gradTeamsPerSm(kind, cols)));
+  // As many teams as an SM holds: enough rows under
+  // way to cover a row's two sums, few enough that the teams' sums (f32, one or two rows each) stay small beside the rows.
+  const int64_t teams = std::max<int64_t>(1, std::min<int64_t>(rows, smCount * gradTeamsPerSm(elemType, kind, cols)));
   const int64_t wanted = std::max<int64_t>(1, groups ? teams / groups : 1);
   const int64_t chunkRows = (perGroup + wanted - 1) / wanted;
   const int64_t chunks = (perGroup + chunkRows - 1) / chunkRows;
@@ -236,8 +244,8 @@ int launchBlockNorm(const BlockNormLaunch &l, cudaStream_t stream, int *launched
   return e;
 }
 
-size_t blockNormGradWorkspaceBytes(int pass, int kind, int gateForm, int64_t rows, int64_t cols, int64_t groupRows, int smCount) {
-  return static_cast<size_t>(sumsFloats(gradPlan(kind, gateForm, rows, cols, groupRows, smCount), pass, kind)) * sizeof(float);
+size_t blockNormGradWorkspaceBytes(int pass, int elemType, int kind, int gateForm, int64_t rows, int64_t cols, int64_t groupRows, int smCount) {
+  return static_cast<size_t>(sumsFloats(gradPlan(elemType, kind, gateForm, rows, cols, groupRows, smCount), pass, kind)) * sizeof(float);
 }
 
 int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *launched) {
@@ -245,7 +253,7 @@ int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *
   if (l.cols <= 0 || l.cols > kMaxNormCols || l.rows > kMaxNormRows) return cudaErrorInvalidValue;
   int device = 0;
   if (const cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return e;
-  GradPlan plan = gradPlan(l.kind, l.gateForm, l.rows, l.cols, l.groupRows, deviceSmCount(device));
+  GradPlan plan = gradPlan(l.elemType, l.kind, l.gateForm, l.rows, l.cols, l.groupRows, deviceSmCount(device));
   const size_t need = static_cast<size_t>(sumsFloats(plan, l.pass, l.kind)) * sizeof(float);
   if (!l.workspace || l.workspaceBytes < need || !vectorAligned(l.workspace)) return cudaErrorInvalidValue;
   const int64_t values = l.kind == kLayerNorm ? 2 : 1;
@@ -261,21 +269,25 @@ int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *
     if (l.gateForm == kGateToken) vector = vector && rowsAligned(l.dgate.base, l.dgate.ld, eb, 16);
     for (const void *v : {l.a.weight, l.a.bias, l.b.weight, l.scale}) vector = vector && vectorAligned(v);
     vector = vector && rowsAligned(l.checkpoint.codes, l.checkpoint.codesLd, 1, vec);
-    const TeamShape s = gradShape(l.elemType, l.kind, l.cols, vector);
+    TeamShape s = gradShape(l.elemType, l.kind, l.cols, vector);
+    // rows fetched ahead: as many (2 to 4) as the CTAs of an SM have shared memory for beside their parameters; rows too
+    // wide for two take the kernel without
+    const int tensors = (l.pass != kPost ? 2 : 0) + (l.dout.base ? 1 : 0) + (l.pass != kPre ? 1 : 0) + (l.gateForm == kGateToken ? 1 : 0);
+    const int vectors = (l.pass != kPost ? 1 : 0) + (l.pass != kPre ? 1 : 0) + (l.gateForm == kGateToken && l.kind == kLayerNorm ? 1 : 0);
+    const size_t paramBytes = static_cast<size_t>(vectors) * static_cast<size_t>(plan.sumsLd) * sizeof(float);
+    const size_t rowBytes = static_cast<size_t>(tensors) * static_cast<size_t>(s.nv) * 16 * static_cast<size_t>(s.lanes) * static_cast<size_t>(s.teamsPerCta);
+    const int64_t ctasPerSm = std::max<int64_t>(1, (gradTeamsPerSm(l.elemType, l.kind, l.cols) + s.teamsPerCta - 1) / s.teamsPerCta);
+    constexpr size_t kAheadBytes = 225 * 1024;  // of the 227 KB that the CTAs of an SM can have, each with 1 KB of its own
+    const size_t perCta = kAheadBytes / static_cast<size_t>(ctasPerSm) - 1536;
+    const int stages = static_cast<int>(std::min<size_t>(4, std::max<size_t>(2, (perCta - std::min(perCta, paramBytes)) / rowBytes)));
+    const size_t slotBytes = static_cast<size_t>(stages) * rowBytes + paramBytes;
+    const GradAheadKernel ahead = vector && slotBytes <= kAheadBytes ? aheadKernel(l.elemType, l.kind, l.pass, l.gateForm == kGateToken, static_cast<int64_t>(s.lanes) * s.nv * vec == l.cols, s.nv) : nullptr;
+    if (!ahead && vector) s = wideShape(l.elemType, l.cols);
     const unsigned int threads = static_cast<unsigned int>(s.lanes * s.teamsPerCta);
     const dim3 grid(static_cast<unsigned int>((plan.teams + s.teamsPerCta - 1) / s.teamsPerCta));
-    // rows fetched ahead: as many (2 to 4) as the teams of an SM have shared memory for; rows too wide for two take the
-    // kernel without
-    const int tensors = (l.pass != kPost ? 2 : 0) + (l.dout.base ? 1 : 0) + (l.pass != kPre ? 1 : 0) + (l.gateForm == kGateToken ? 1 : 0);
-    const size_t rowBytes = static_cast<size_t>(tensors) * static_cast<size_t>(s.nv) * 16;
-    const size_t threadsPerSm = std::max<size_t>(threads, static_cast<size_t>(gradTeamsPerSm(l.kind, l.cols)) * static_cast<size_t>(s.lanes));
-    constexpr size_t kAheadBytesPerSm = 200 * 1024, kAheadBytesPerCta = 220 * 1024;
-    const int stages = static_cast<int>(std::min<size_t>(4, std::max<size_t>(2, kAheadBytesPerSm / (rowBytes * threadsPerSm))));
-    const size_t slotBytes = static_cast<size_t>(stages) * rowBytes * threads;
-    const GradAheadKernel ahead = vector && slotBytes <= kAheadBytesPerCta ? aheadKernel(l.elemType, l.kind, l.pass, l.gateForm, s.nv) : nullptr;
     cudaError_t e;
     if (ahead) {
-      if (e = reserveSharedMemory(reinterpret_cast<const void *>(ahead), static_cast<int>(kAheadBytesPerCta)); e != cudaSuccess) return e;
+      if (e = reserveSharedMemory(reinterpret_cast<const void *>(ahead), static_cast<int>(kAheadBytes)); e != cudaSuccess) return e;
       e = launchDependent(ahead, grid, dim3(threads), slotBytes, stream, l, plan, s.lanes, stages);
     } else {
       const GradKernel kernel = l.elemType == kF32   ? gradKernel<kF32>(l.kind, l.pass, vector, s.nv)

@@ -78,7 +78,7 @@ struct BlockNormGradLaunch {
   void *workspace;
   size_t workspaceBytes;
 };
-size_t blockNormGradWorkspaceBytes(int pass, int kind, int gateForm, int64_t rows, int64_t cols, int64_t groupRows, int smCount);
+size_t blockNormGradWorkspaceBytes(int pass, int elemType, int kind, int gateForm, int64_t rows, int64_t cols, int64_t groupRows, int smCount);
 int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *launched);
 
 struct CheckpointPackLaunch {

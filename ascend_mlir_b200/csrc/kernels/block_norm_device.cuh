@@ -100,7 +100,7 @@ template <int ELEM, int VEC> __device__ __forceinline__ void loadParam(const voi
 }
 
 // ---- teams ------------------------------------------------------------------------------------------------------
-// `lanes` threads (a multiple of 32, at most 512) that hold one row; a CTA of up to 512 threads has one or more of them.
+// `lanes` threads (a multiple of 32, at most 1024) that hold one row; a CTA has one or more teams.
 // Sums over a team: a shuffle tree in each warp, then the warps' sums through shared memory, added by every warp in the
 // same order.  The two halves of the buffer alternate, so one barrier per sum is enough: whoever writes a half again has
 // passed the barrier of the sum between, which every reader of that half reached after reading.
@@ -109,7 +109,7 @@ struct Team {
   float *scratch;                 // this team's slice of the CTA's buffer
   int half;
 };
-constexpr int kTeamScratchFloats = 2 * 2 * 16;  // halves x values x warps of a 512-thread CTA
+constexpr int kTeamScratchFloats = 2 * 2 * 32;  // halves x values x warps of a CTA
 
 __device__ __forceinline__ Team makeTeam(int lanes, float *scratch) {
   Team t;
@@ -131,21 +131,20 @@ template <int N> __device__ __forceinline__ void teamSum(Team &t, float (&v)[N])
 #pragma unroll
   for (int n = 0; n < N; ++n) v[n] = warpSum(v[n]);
   if (t.lanes == 32) return;
-  float *buf = t.scratch + t.half * 32;
+  float *buf = t.scratch + t.half * 64;
   t.half ^= 1;
   const int lane = threadIdx.x & 31;
   if (lane == 0) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) buf[n * 16 + (t.lane >> 5)] = v[n];
+    for (int n = 0; n < N; ++n) buf[n * 32 + (t.lane >> 5)] = v[n];
   }
   asm volatile("bar.sync %0, %1;" ::"r"(t.index + 1), "r"(t.lanes) : "memory");
   const int warps = t.lanes >> 5;
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    v[n] = lane < warps ? buf[n * 16 + lane] : 0.0f;
+    v[n] = lane < warps ? buf[n * 32 + lane] : 0.0f;
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
-    v[n] = __shfl_sync(0xffffffffu, v[n], 0);
+    for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
   }
 }
 

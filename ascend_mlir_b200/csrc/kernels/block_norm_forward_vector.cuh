@@ -56,16 +56,16 @@ __device__ __forceinline__ void pairStatistics(Team &team, const F2 (&v)[NV][kPa
     if (team.lanes == 32) {
       mean = centre;
     } else {
-      float *buf = team.scratch + team.half * 32;
+      float *buf = team.scratch + team.half * 64;
       team.half ^= 1;
       const int lane = threadIdx.x & 31, warps = team.lanes >> 5;
       if (lane == 0) {
         buf[team.lane >> 5] = s;
-        buf[16 + (team.lane >> 5)] = squares;
+        buf[32 + (team.lane >> 5)] = squares;
       }
       asm volatile("bar.sync %0, %1;" ::"r"(team.index + 1), "r"(team.lanes) : "memory");
       const float n = lane < warps ? columnsOf(lane) : 0.0f;
-      const float sw = lane < warps ? buf[lane] : 0.0f, qw = lane < warps ? buf[16 + lane] : 0.0f;
+      const float sw = lane < warps ? buf[lane] : 0.0f, qw = lane < warps ? buf[32 + lane] : 0.0f;
       float total = sw;
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);

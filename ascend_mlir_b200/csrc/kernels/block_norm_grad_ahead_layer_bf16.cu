@@ -2,6 +2,6 @@
 
 namespace afir {
 namespace kernels {
-template GradAheadKernel gradAheadKernel<kBF16, kLayerNorm>(int pass, int gate, int nv);
+template GradAheadKernel gradAheadKernel<kBF16, kLayerNorm>(int pass, bool token, bool full, int nv);
 } // namespace kernels
 } // namespace afir

@@ -7,24 +7,20 @@
 namespace afir {
 namespace kernels {
 
-template <int ELEM, int KIND, int PASS, int GATE> GradAheadKernel gradAheadKernelOf(int nv) {
+template <int ELEM, int KIND, int PASS, bool TOKEN, bool FULL> GradAheadKernel gradAheadKernelOf(int nv) {
   switch (nv) {
-  case 1: return blockNormGradVectorKernel<ELEM, KIND, PASS, GATE, 1>;
-  case 2: return blockNormGradVectorKernel<ELEM, KIND, PASS, GATE, 2>;
-  case 4:
-    if constexpr (ELEM == kF32) return blockNormGradVectorKernel<ELEM, KIND, PASS, GATE, 4>;
-    else return nullptr;
+  case 1: return blockNormGradVectorKernel<ELEM, KIND, PASS, TOKEN, FULL, 1>;
+  case 2: return blockNormGradVectorKernel<ELEM, KIND, PASS, TOKEN, FULL, 2>;
   default: return nullptr;
   }
 }
-template <int ELEM, int KIND, int PASS> GradAheadKernel gradAheadKernelOf(int gate, int nv) {
-  if (gate == kGateToken) return gradAheadKernelOf<ELEM, KIND, PASS, kGateToken>(nv);
-  if (gate == kGateGroup) return gradAheadKernelOf<ELEM, KIND, PASS, kGateGroup>(nv);
-  return gradAheadKernelOf<ELEM, KIND, PASS, kGateNone>(nv);
+template <int ELEM, int KIND, int PASS, bool TOKEN> GradAheadKernel gradAheadKernelOf(bool full, int nv) {
+  return full ? gradAheadKernelOf<ELEM, KIND, PASS, TOKEN, true>(nv) : gradAheadKernelOf<ELEM, KIND, PASS, TOKEN, false>(nv);
 }
-template <int ELEM, int KIND> GradAheadKernel gradAheadKernel(int pass, int gate, int nv) {
-  if (pass == kPre) return gradAheadKernelOf<ELEM, KIND, kPre, kGateNone>(nv);
-  return pass == kPost ? gradAheadKernelOf<ELEM, KIND, kPost>(gate, nv) : gradAheadKernelOf<ELEM, KIND, kPostPre>(gate, nv);
+template <int ELEM, int KIND> GradAheadKernel gradAheadKernel(int pass, bool token, bool full, int nv) {
+  if (pass == kPre) return gradAheadKernelOf<ELEM, KIND, kPre, false>(full, nv);
+  if (pass == kPost) return token ? gradAheadKernelOf<ELEM, KIND, kPost, true>(full, nv) : gradAheadKernelOf<ELEM, KIND, kPost, false>(full, nv);
+  return token ? gradAheadKernelOf<ELEM, KIND, kPostPre, true>(full, nv) : gradAheadKernelOf<ELEM, KIND, kPostPre, false>(full, nv);
 }
 
 } // namespace kernels

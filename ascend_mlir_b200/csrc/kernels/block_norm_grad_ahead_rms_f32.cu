@@ -2,6 +2,6 @@
 
 namespace afir {
 namespace kernels {
-template GradAheadKernel gradAheadKernel<kF32, kRmsNorm>(int pass, int gate, int nv);
+template GradAheadKernel gradAheadKernel<kF32, kRmsNorm>(int pass, bool token, bool full, int nv);
 } // namespace kernels
 } // namespace afir

@@ -2,7 +2,8 @@
 //
 // A row of the longest form is five tensors in and three out, so a team that loads when it needs the data leaves HBM
 // idle while it sums.  Here every thread fetches its vectors two to four rows ahead into slots of its own in shared
-// memory (cp.async), so a row's sums run while the next rows arrive.  The arithmetic is done on pairs of f32
+// memory (cp.async), so a row's sums run while the next rows arrive.  The parameter vectors are kept there too: beside the
+// rows they would not stay in what is left of the L1 (15 % hits), and every pass would wait for L2.  The arithmetic is done on pairs of f32
 // (fma.rn.f32x2): at 8192 bf16 columns the plain form needs as many issue cycles as HBM needs time.
 #pragma once
 
@@ -37,14 +38,14 @@ struct RowCursor {
   }
 };
 
-// GATE: GateForm (kGateNone for kPre).
-template <int ELEM, int KIND, int PASS, int GATE, int NV>
+// TOKEN: a gate value per element (kGateToken); FULL: every thread's vectors lie inside the row.
+template <int ELEM, int KIND, int PASS, bool TOKEN, bool FULL, int NV>
 __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_constant__ BlockNormGradLaunch p, const __grid_constant__ GradPlan plan,
                                                                  int teamLanes, int stages) {
   gridDependencyPrologue();
   constexpr bool kLayer = KIND == kLayerNorm;
   constexpr int kValues = kLayer ? 2 : 1;
-  constexpr bool kPostPart = PASS != kPre, kPrePart = PASS != kPost, kToken = GATE == kGateToken;
+  constexpr bool kPostPart = PASS != kPre, kPrePart = PASS != kPost, kToken = TOKEN;
   constexpr int VEC = ElemOf<ELEM>::kVec, P = kPairs<ELEM>, EB = 16 / VEC;
   extern __shared__ uint4 slots[];  // [stages][tensors][NV][threads]
   __shared__ float scratch[kTeamScratchFloats];
@@ -58,9 +59,10 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
   const int col0 = team.lane * VEC, apart = team.lanes * VEC;
   bool has[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) has[i] = col0 + i * apart < cols;
+  for (int i = 0; i < NV; ++i) has[i] = FULL || col0 + i * apart < cols;
 
   // Slots by byte: tensors present get one each, in this order.
+  const bool grouped = !kToken && p.gateForm == kGateGroup;
   const bool packed = p.checkpoint.codes != nullptr, hasDout = p.dout.base != nullptr;
   const unsigned int perTensor = NV * blockDim.x * 16, perVector = blockDim.x * 16;
   unsigned int used = 0;
@@ -74,10 +76,45 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
   if (kPostPart) used += perTensor;
   const unsigned int atGate = used;
   if (kToken) used += perTensor;
-  const unsigned int slot0 = static_cast<unsigned int>(__cvta_generic_to_shared(slots)) + threadIdx.x * 16, slotEnd = slot0 + stages * used;
+  const unsigned int slot0 = threadIdx.x * 16, slotEnd = slot0 + stages * used;
+  const unsigned int slotsAt = static_cast<unsigned int>(__cvta_generic_to_shared(slots));
+  auto readSlot = [&](unsigned int at) { return *reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(slots) + at); };
 
-  auto rowOf = [&](const RowsIn &r, int row) { return static_cast<const char *>(r.base) + (static_cast<int64_t>(row) * r.ld + col0) * EB; };
-  auto rowTo = [&](const RowsOut &r, int row) { return static_cast<char *>(r.base) + (static_cast<int64_t>(row) * r.ld + col0) * EB; };
+  // Parameters as f32 behind the slots, for all teams of the CTA: normB's weight, normA's weight times the residual scale and,
+  // where a token's gate needs it, normA's bias times it.  Each thread reads only what it has written itself (teams
+  // write the same values), so nothing waits here.
+  float *weightB = reinterpret_cast<float *>(reinterpret_cast<char *>(slots) + stages * used);
+  float *weightA = weightB + (kPrePart ? plan.sumsLd : 0), *biasA = weightA + (kPostPart ? plan.sumsLd : 0);
+  auto writeParams = [&](float *to, const void *v, const void *times) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (!has[i]) continue;
+      F2 x[P], y[P];
+      loadParamPairs<ELEM>(v, p.paramType, col0 + i * apart, x);
+      if (times) {
+        loadParamPairs<ELEM>(times, p.paramType, col0 + i * apart, y);
+#pragma unroll
+        for (int e = 0; e < P; ++e) x[e] = x[e] * y[e];
+      }
+#pragma unroll
+      for (int e = 0; e < P / 2; ++e) {
+        const F2 quad[2] = {x[2 * e], x[2 * e + 1]};
+        *reinterpret_cast<uint4 *>(to + col0 + i * apart + 4 * e) = narrowPairs<kF32>(quad);
+      }
+    }
+  };
+  auto readParams = [&](const float *from, int i, F2 (&v)[P]) {
+#pragma unroll
+    for (int e = 0; e < P / 2; ++e) {
+      F2 quad[2];
+      widenPairs<kF32>(*reinterpret_cast<const uint4 *>(from + col0 + i * apart + 4 * e), quad);
+      v[2 * e] = quad[0];
+      v[2 * e + 1] = quad[1];
+    }
+  };
+
+  auto rowOf = [&](const RowsIn &r, int row) { return static_cast<const char *>(r.base) + (static_cast<int64_t>(row) * static_cast<int>(r.ld) + col0) * EB; };  // ld < 2^24
+  auto rowTo = [&](const RowsOut &r, int row) { return static_cast<char *>(r.base) + (static_cast<int64_t>(row) * static_cast<int>(r.ld) + col0) * EB; };
   auto store = [&](char *to, int i, const F2 (&v)[P]) { *reinterpret_cast<uint4 *>(to + i * apart * EB) = narrowPairs<ELEM>(v); };
 
   auto fetch = [&](const RowCursor &c, unsigned int slot) {
@@ -86,15 +123,15 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
         const char *from = rowOf(r, c.row);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-          if (has[i]) copyAhead16(slot + at + i * perVector, from + i * apart * EB);
+          if (has[i]) copyAhead16(slotsAt + slot + at + i * perVector, from + i * apart * EB);
       };
       auto codes = [&](unsigned int at) {
-        const uint8_t *from = p.checkpoint.codes + static_cast<int64_t>(c.row) * p.checkpoint.codesLd + col0;
+        const uint8_t *from = p.checkpoint.codes + static_cast<int64_t>(c.row) * static_cast<int>(p.checkpoint.codesLd) + col0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           if (!has[i]) continue;
-          if constexpr (VEC == 8) copyAhead8(slot + at + i * perVector, from + i * apart);
-          else copyAhead4(slot + at + i * perVector, from + i * apart);
+          if constexpr (VEC == 8) copyAhead8(slotsAt + slot + at + i * perVector, from + i * apart);
+          else copyAhead4(slotsAt + slot + at + i * perVector, from + i * apart);
         }
       };
       if constexpr (kPrePart) {
@@ -126,7 +163,7 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
     if (packed) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (has[i]) s.exps[i] = __ldg(p.checkpoint.exps + static_cast<int64_t>(c.row) * p.checkpoint.expsLd + (col0 + i * apart) / kCheckpointBlock);
+        if (has[i]) s.exps[i] = __ldg(p.checkpoint.exps + static_cast<int64_t>(c.row) * static_cast<int>(p.checkpoint.expsLd) + (col0 + i * apart) / kCheckpointBlock);
     }
   };
 
@@ -140,6 +177,10 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
     fetch(ahead, s);
     ahead.advance(plan, rows);
   }
+
+  if constexpr (kPrePart) writeParams(weightB, p.b.weight, nullptr);
+  if constexpr (kPostPart) writeParams(weightA, p.a.weight, p.scale);
+  if constexpr (kToken && kLayer) writeParams(biasA, p.a.bias, p.scale);
 
   const F2 zero = splat(0.0f);
   F2 sumB[kPrePart ? kValues : 1][NV][P], sumA[kPostPart ? kValues : 1][NV][P];
@@ -167,12 +208,13 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
         if (has[i]) storeSumPairs(plan.sumsA + (static_cast<int64_t>(run) * kValues + k) * plan.sumsLd + col0 + i * apart, sumA[k][i]);
   };
 
-  if constexpr (GATE == kGateGroup) {  // runs without rows, of a short last group: sums of nothing
+  if (kPostPart && grouped) {  // runs without rows, of a short last group: sums of nothing
     RowCursor c;
     for (c.enter(plan, rows, teamIndex); c.live(plan); c.enter(plan, rows, c.run + plan.teams))
       if (c.row >= c.end) storeRunSums(c.run);
   }
 
+  const GateSlope slope = gateSlopeOf(p.gateAct);
   unsigned int slot = slot0;
   while (now.live(plan)) {
     const RowScalars at = next;
@@ -195,7 +237,7 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
         if (PASS == kPre && packed) codePairs<ELEM>(make_uint2(raw.x, raw.y), at.exps[i], n[i]);
         else widenPairs<ELEM>(raw, n[i]);
         widenPairs<ELEM>(readSlot(slot + atDh + i * perVector), dz[i]);
-        loadParamPairs<ELEM>(p.b.weight, p.paramType, col0 + i * apart, w);
+        readParams(weightB, i, w);
 #pragma unroll
         for (int e = 0; e < P; ++e) {
           n[i][e] = kLayer ? (n[i][e] + shift) * rstd : n[i][e] * rstd;
@@ -247,12 +289,11 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
 #pragma unroll
       for (int k = 0; k < kValues; ++k) s[k] = zero;
       char *toDx = rowTo(p.dx, row), *toDgate = kToken ? rowTo(p.dgate, row) : nullptr;
-      const char *gateRow = GATE == kGateGroup ? rowOf(p.gate, group) : nullptr;
+      const char *gateRow = grouped ? rowOf(p.gate, group) : nullptr;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         if (!has[i]) continue;
-        const int col = col0 + i * apart;
-        F2 t[P], w[P], scaled[P];  // scaled: the stream's gradient times the residual scale
+        F2 t[P], w[P];  // w: normA's weight times the residual scale
         const uint4 raw = readSlot(slot + atY + i * perVector);
         if (packed) codePairs<ELEM>(make_uint2(raw.x, raw.y), at.exps[i], n[i]);
         else widenPairs<ELEM>(raw, n[i]);
@@ -260,48 +301,37 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
         for (int e = 0; e < P; ++e) {
           n[i][e] = kLayer ? (n[i][e] + shift) * rstd : n[i][e] * rstd;
           t[e] = dz[i][e] * alpha;
-          scaled[e] = dz[i][e];
         }
         store(toDx, i, t);
-        if (p.scale) {
-          loadParamPairs<ELEM>(p.scale, p.paramType, col, t);
+        readParams(weightA, i, w);
+        if constexpr (kToken) {
+          F2 a[P], bias[P];
+          widenPairs<ELEM>(readSlot(slot + atGate + i * perVector), a);
+          gatePairs(a, p.gateAct);
+          if constexpr (kLayer) readParams(biasA, i, bias);
 #pragma unroll
-          for (int e = 0; e < P; ++e) scaled[e] = scaled[e] * t[e];
-        }
-        loadParamPairs<ELEM>(p.a.weight, p.paramType, col, w);
-        if constexpr (GATE == kGateNone) {
+          for (int e = 0; e < P; ++e) {
+            const F2 gated = dz[i][e] * a[e];
+            sumA[0][i][e] = fma2(gated, n[i][e], sumA[0][i][e]);
+            if constexpr (kLayer) sumA[1][i][e] = sumA[1][i][e] + gated;
+            t[e] = dz[i][e] * (kLayer ? fma2(n[i][e], w[e], bias[e]) : n[i][e] * w[e]) * slopeAt(slope, a[e]);
+            dz[i][e] = gated * w[e];
+          }
+          store(toDgate, i, t);
+        } else {
 #pragma unroll
           for (int e = 0; e < P; ++e) {
             sumA[0][i][e] = fma2(dz[i][e], n[i][e], sumA[0][i][e]);
             if constexpr (kLayer) sumA[1][i][e] = sumA[1][i][e] + dz[i][e];
-            dz[i][e] = scaled[e] * w[e];
+            dz[i][e] = dz[i][e] * w[e];
           }
-        } else {
-          F2 a[P];
-          if constexpr (kToken) widenPairs<ELEM>(readSlot(slot + atGate + i * perVector), a);
-          else widenPairs<ELEM>(*reinterpret_cast<const uint4 *>(gateRow + i * apart * EB), a);
-          gatePairs(a, p.gateAct);
-          if constexpr (kToken) {
-            F2 u[P];
-            if constexpr (kLayer) loadParamPairs<ELEM>(p.a.bias, p.paramType, col, u);
+          if (grouped) {
+            F2 a[P];
+            widenPairs<ELEM>(*reinterpret_cast<const uint4 *>(gateRow + i * apart * EB), a);
+            gatePairs(a, p.gateAct);
 #pragma unroll
-            for (int e = 0; e < P; ++e) {
-              u[e] = kLayer ? fma2(n[i][e], w[e], u[e]) : n[i][e] * w[e];
-              t[e] = scaled[e] * u[e] * gateSlopePair(a[e], p.gateAct);
-              const F2 gated = dz[i][e] * a[e];
-              sumA[0][i][e] = fma2(gated, n[i][e], sumA[0][i][e]);
-              if constexpr (kLayer) sumA[1][i][e] = sumA[1][i][e] + gated;
-            }
-            store(toDgate, i, t);
-          } else {
-#pragma unroll
-            for (int e = 0; e < P; ++e) {
-              sumA[0][i][e] = fma2(dz[i][e], n[i][e], sumA[0][i][e]);
-              if constexpr (kLayer) sumA[1][i][e] = sumA[1][i][e] + dz[i][e];
-            }
+            for (int e = 0; e < P; ++e) dz[i][e] = dz[i][e] * a[e];
           }
-#pragma unroll
-          for (int e = 0; e < P; ++e) dz[i][e] = scaled[e] * (a[e] * w[e]);
         }
 #pragma unroll
         for (int e = 0; e < P; ++e) {

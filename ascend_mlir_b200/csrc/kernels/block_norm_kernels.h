@@ -16,7 +16,7 @@ template <int ELEM> ForwardKernel forwardKernel(int kind, int pass, bool vector,
 template <int ELEM> GradKernel gradKernel(int kind, int pass, bool vector, int nv);
 // With rows fetched ahead (block_norm_grad_vector.cuh); null where a thread would hold more than it has registers for.
 using GradAheadKernel = void (*)(const BlockNormGradLaunch, const GradPlan, int, int);
-template <int ELEM, int KIND> GradAheadKernel gradAheadKernel(int pass, int gate, int nv);
+template <int ELEM, int KIND> GradAheadKernel gradAheadKernel(int pass, bool token, bool full, int nv);
 
 } // namespace kernels
 } // namespace afir

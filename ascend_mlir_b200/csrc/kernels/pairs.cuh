@@ -90,7 +90,7 @@ template <int ELEM> __device__ __forceinline__ void loadPairs(const void *p, int
 template <int ELEM> __device__ __forceinline__ void storePairs(void *p, int64_t at, const F2 (&v)[kPairs<ELEM>]) {
   *reinterpret_cast<uint4 *>(static_cast<typename ElemOf<ELEM>::Type *>(p) + at) = narrowPairs<ELEM>(v);
 }
-// A parameter vector: of the rows' type or f32 (uniform over the launch); it stays in L1 from row to row.
+// A parameter vector: of the rows' type or f32 (uniform over the launch).
 template <int ELEM> __device__ __forceinline__ void loadParamPairs(const void *p, int type, int at, F2 (&v)[kPairs<ELEM>]) {
   if (ELEM == kF32 || type != kF32) {
     loadPairs<ELEM>(p, at, v);
@@ -132,12 +132,12 @@ template <int N> __device__ __forceinline__ void gatePairs(F2 (&g)[N], int act) 
     else g[i] = pairOf(tanhf(f.x), tanhf(f.y));
   }
 }
-__device__ __forceinline__ F2 gateSlopePair(F2 a, int act) {
-  const F2 one = splat(1.0f), minus = splat(-1.0f);
-  if (act == kActSigmoid) return a * fma2(a, minus, one);
-  if (act == kActTanh) return fma2(a * minus, a, one);
-  return one;
+// The derivative of the activation from its value, as a polynomial in it: a - a^2 (sigmoid), 1 - a^2 (tanh), 1.
+struct GateSlope { F2 c0, c1, c2; };
+__device__ __forceinline__ GateSlope gateSlopeOf(int act) {
+  return {splat(act == kActSigmoid ? 0.0f : 1.0f), splat(act == kActSigmoid ? 1.0f : 0.0f), splat(act == kActNone ? 0.0f : -1.0f)};
 }
+__device__ __forceinline__ F2 slopeAt(const GateSlope &g, F2 a) { return fma2(a, fma2(a, g.c2, g.c1), g.c0); }
 
 // ---- packing a vector -----------------------------------------------------------------------------------------------
 // Largest magnitude among 16 bytes of elements, NaN left out; 16-bit types compare as they are, two at a time.
@@ -221,11 +221,6 @@ __device__ __forceinline__ void copyAhead8(unsigned int slot, const void *from) 
 }
 __device__ __forceinline__ void copyAhead4(unsigned int slot, const void *from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(slot), "l"(from) : "memory");
-}
-__device__ __forceinline__ uint4 readSlot(unsigned int slot) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(slot) : "memory");
-  return v;
 }
 __device__ __forceinline__ void copiesCommit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Until all but the newest `left` groups have arrived (left = 1, 2 or 3).
