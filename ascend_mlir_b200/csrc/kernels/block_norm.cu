@@ -31,49 +31,62 @@ __device__ __forceinline__ float elemAt(const void *p, int type, int64_t at) {
   return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[at]);
 }
 
-constexpr int kFinishCols = 8, kFinishSlots = 64;
+constexpr int kFinishThreads = 512;
 
-// Adds one value per slot over `slots` neighbouring slots (a power of two); the first slot of each run gets the sum.
-__device__ __forceinline__ float slotSum(float v, float (*buf)[kFinishCols], int slots) {
-  const int c = threadIdx.x, s = threadIdx.y;
-  buf[s][c] = v;
+// Adds two values per slot over each run of `slots` neighbouring slots (a power of two), in slot order; the first slot of a
+// run gets the sums.  A CTA is blockDim.x columns by blockDim.y slots.
+__device__ __forceinline__ void slotSums(float (&v)[2], int values, float2 *buf, int slots) {
+  const int c = threadIdx.x, s = threadIdx.y, width = blockDim.x;
+  buf[s * width + c] = make_float2(v[0], v[1]);
   __syncthreads();
-  for (int o = slots / 2; o > 0; o >>= 1) {
-    if ((s & (slots - 1)) < o) buf[s][c] += buf[s + o][c];
-    __syncthreads();
+  if ((s & (slots - 1)) == 0) {
+    float2 sum = buf[s * width + c];
+#pragma unroll 4
+    for (int i = 1; i < slots; ++i) {
+      const float2 f = buf[(s + i) * width + c];
+      sum.x += f.x;
+      if (values > 1) sum.y += f.y;
+    }
+    v[0] = sum.x;
+    v[1] = sum.y;
   }
-  v = buf[s & ~(slots - 1)][c];
   __syncthreads();
-  return v;
 }
 
-// 8 columns (one 32-byte sector of every row of sums) x 64 slots per CTA: the slots share the rows of sums, and the
-// order in which they are added depends on the sizes alone.
-__global__ void __launch_bounds__(kFinishCols *kFinishSlots) blockNormFinishKernel(const __grid_constant__ FinishParams p) {
+// The rows of sums `first`, first + step, ... below `count` (each `values` rows of sumsLd floats), added.
+__device__ __forceinline__ void addRows(const float *sums, int64_t sumsLd, int values, int64_t first, int64_t step, int64_t count, float (&v)[2]) {
+  v[0] = v[1] = 0.0f;
+#pragma unroll 4
+  for (int64_t r = first; r < count; r += step) {
+    v[0] += sums[r * values * sumsLd];
+    if (values > 1) v[1] += sums[(r * values + 1) * sumsLd];
+  }
+}
+
+// Slots share the rows of sums; the order in which they are added depends on the sizes alone.
+__global__ void __launch_bounds__(kFinishThreads) blockNormFinishKernel(const __grid_constant__ FinishParams p) {
   gridDependencyPrologue();
-  __shared__ float buf[kFinishSlots][kFinishCols];
-  const int64_t col = static_cast<int64_t>(blockIdx.x) * kFinishCols + threadIdx.x;
+  __shared__ float2 buf[kFinishThreads];
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   const bool live = col < p.cols;
-  const int slot = threadIdx.y;
+  const int slot = threadIdx.y, allSlots = blockDim.y;
   const int values = p.layer ? 2 : 1;
   if (p.sumsA) {
     // slots as (groups at once) x (slots per group)
     int atOnce = 1;
-    while (atOnce < p.groups && atOnce < kFinishSlots) atOnce *= 2;
-    const int perGroup = kFinishSlots / atOnce;
+    while (atOnce < p.groups && atOnce < allSlots) atOnce *= 2;
+    const int perGroup = allSlots / atOnce;
     const float w = live ? elemAt(p.weight, p.paramType, col) : 0.0f;
     const float b = live && p.layer ? elemAt(p.bias, p.paramType, col) : 0.0f;
     const float scale = live && p.scale ? elemAt(p.scale, p.paramType, col) : 1.0f;
     float total[2] = {0.0f, 0.0f};
     for (int64_t g0 = 0; g0 < p.groups; g0 += atOnce) {
       const int64_t group = g0 + slot / perGroup;
+      const bool mine = live && group < p.groups;
       float s[2] = {0.0f, 0.0f};
-      if (live && group < p.groups)
-        for (int64_t c = slot & (perGroup - 1); c < p.chunks; c += perGroup)
-          for (int k = 0; k < values; ++k) s[k] += p.sumsA[((group * p.chunks + c) * values + k) * p.sumsLd + col];
-      if (perGroup > 1)
-        for (int k = 0; k < values; ++k) s[k] = slotSum(s[k], buf, perGroup);
-      if (live && group < p.groups && (slot & (perGroup - 1)) == 0) {
+      if (mine) addRows(p.sumsA + group * p.chunks * values * p.sumsLd + col, p.sumsLd, values, slot & (perGroup - 1), perGroup, p.chunks, s);
+      if (perGroup > 1) slotSums(s, values, buf, perGroup);
+      if (mine && (slot & (perGroup - 1)) == 0) {
         float a = 1.0f;
         if (p.gateForm == kGateGroup) {
           a = gateValue(elemAt(p.gate, p.elemType, group * p.gateLd + col), p.gateAct);
@@ -83,7 +96,7 @@ __global__ void __launch_bounds__(kFinishCols *kFinishSlots) blockNormFinishKern
         total[1] = fmaf(a, s[1], total[1]);
       }
     }
-    for (int k = 0; k < values; ++k) total[k] = slotSum(total[k], buf, kFinishSlots);
+    if (p.groups > 1) slotSums(total, values, buf, allSlots);
     if (live && slot == 0) {
       p.dweight[col] = scale * total[0];
       if (p.dbias) p.dbias[col] = scale * total[1];
@@ -92,10 +105,8 @@ __global__ void __launch_bounds__(kFinishCols *kFinishSlots) blockNormFinishKern
   }
   if (p.sumsB) {
     float s[2] = {0.0f, 0.0f};
-    if (live)
-      for (int64_t t = slot; t < p.teams; t += kFinishSlots)
-        for (int k = 0; k < values; ++k) s[k] += p.sumsB[(t * values + k) * p.sumsLd + col];
-    for (int k = 0; k < values; ++k) s[k] = slotSum(s[k], buf, kFinishSlots);
+    if (live) addRows(p.sumsB + col, p.sumsLd, values, slot, allSlots, p.teams, s);
+    slotSums(s, values, buf, allSlots);
     if (live && slot == 0) {
       p.nextWeight[col] = s[0];
       if (p.nextBias) p.nextBias[col] = s[1];
@@ -118,12 +129,12 @@ TeamShape shapeOf(int vec, int nv, int64_t cols) {
 int scalarElements(int64_t cols) { return cols <= kScalarSmall * 512 ? kScalarSmall : kScalarLarge; }
 
 // A team has at most 512 threads.  Few rows: one vector per thread while that is enough, for the shortest way through one
-// row.  Rows enough to fill the SMs: 16 columns per thread, which keeps more loads under way per thread and less
-// of the time in sums across warps.
+// row.  Rows enough to fill the SMs several times: 32 columns per thread, since what a row costs a thread besides its
+// vectors (statistics across warps, addresses) is as much as two or three vectors.
 TeamShape forwardShape(int elemType, int64_t rows, int64_t cols, bool vector, int smCount) {
   const int vec = vector ? (elemType == kF32 ? 4 : 8) : 1;
   if (!vector) return shapeOf(1, scalarElements(cols), cols);
-  const int64_t perThread = rows >= smCount ? 16 : vec;
+  const int64_t perThread = rows >= 4 * smCount ? 32 : rows >= smCount ? 16 : vec;
   int nv = 1;
   while (nv * vec < perThread && static_cast<int64_t>(nv) * vec * 32 < cols) nv *= 2;
   while (static_cast<int64_t>(nv) * vec * 512 < cols) nv *= 2;
@@ -274,7 +285,8 @@ int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *
     // wide for two take the kernel without
     const int tensors = (l.pass != kPost ? 2 : 0) + (l.dout.base ? 1 : 0) + (l.pass != kPre ? 1 : 0) + (l.gateForm == kGateToken ? 1 : 0);
     const int vectors = (l.pass != kPost ? 1 : 0) + (l.pass != kPre ? 1 : 0) + (l.gateForm == kGateToken && l.kind == kLayerNorm ? 1 : 0);
-    const size_t paramBytes = static_cast<size_t>(vectors) * static_cast<size_t>(plan.sumsLd) * sizeof(float);
+    const int perTeam = l.gateForm == kGateGroup && l.pass != kPre ? s.teamsPerCta - 1 : 0;  // a team's group has its own gate
+    const size_t paramBytes = static_cast<size_t>(vectors + perTeam) * static_cast<size_t>(plan.sumsLd) * sizeof(float);
     const size_t rowBytes = static_cast<size_t>(tensors) * static_cast<size_t>(s.nv) * 16 * static_cast<size_t>(s.lanes) * static_cast<size_t>(s.teamsPerCta);
     const int64_t ctasPerSm = std::max<int64_t>(1, (gradTeamsPerSm(l.elemType, l.kind, l.cols) + s.teamsPerCta - 1) / s.teamsPerCta);
     constexpr size_t kAheadBytes = 225 * 1024;  // of the 227 KB that the CTAs of an SM can have, each with 1 KB of its own
@@ -324,8 +336,10 @@ int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *
   f.nextBias = l.db.bias;
   f.dgate = static_cast<float *>(l.gateForm == kGateGroup ? l.dgate.base : nullptr);
   f.dgateLd = l.dgate.ld;
-  const unsigned int grid = static_cast<unsigned int>((l.cols + kFinishCols - 1) / kFinishCols);
-  const cudaError_t e = launchDependent(blockNormFinishKernel, dim3(grid), dim3(kFinishCols, kFinishSlots), 0, stream, f);
+  // whole 128-byte lines of the sums where that still gives 64 CTAs, else less of a line and more slots
+  const int width = l.cols >= 2048 ? 32 : l.cols >= 1024 ? 16 : 8;
+  const unsigned int grid = static_cast<unsigned int>((l.cols + width - 1) / width);
+  const cudaError_t e = launchDependent(blockNormFinishKernel, dim3(grid), dim3(static_cast<unsigned int>(width), static_cast<unsigned int>(kFinishThreads / width)), 0, stream, f);
   if (e == cudaSuccess && launched) *launched += 1;
   return e;
 }

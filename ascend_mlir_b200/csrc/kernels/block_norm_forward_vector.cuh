@@ -13,9 +13,8 @@ namespace kernels {
 
 // Mean and 1/sqrt(variance + eps) of the row in v; what lies beyond the row is zero in v and not counted.
 template <int ELEM, int KIND, int NV>
-__device__ __forceinline__ void pairStatistics(Team &team, const F2 (&v)[NV][kPairs<ELEM>], int cols, float eps, float &mean, float &rstd) {
+__device__ __forceinline__ void pairStatistics(Team &team, const F2 (&v)[NV][kPairs<ELEM>], int cols, float share, bool full, float eps, float &mean, float &rstd) {
   constexpr int VEC = ElemOf<ELEM>::kVec, P = kPairs<ELEM>;
-  const float share = 1.0f / static_cast<float>(cols);
   if constexpr (KIND == kRmsNorm) {
     F2 q = splat(0.0f);
 #pragma unroll
@@ -25,7 +24,7 @@ __device__ __forceinline__ void pairStatistics(Team &team, const F2 (&v)[NV][kPa
     float s[1] = {sumOf(q)};
     teamSum(team, s);
     mean = 0.0f;
-    rstd = 1.0f / sqrtf(s[0] * share + eps);
+    rstd = rsqrtf(s[0] * share + eps);
   } else {
     F2 sum = splat(0.0f);
 #pragma unroll
@@ -34,18 +33,19 @@ __device__ __forceinline__ void pairStatistics(Team &team, const F2 (&v)[NV][kPa
       for (int e = 0; e < P; ++e) sum = sum + v[i][e];
     const float s = warpSum(sumOf(sum));
     auto columnsOf = [&](int warp) {  // of the row, in this warp's lanes
+      if (full) return static_cast<float>(NV * 32 * VEC);
       int n = 0;
 #pragma unroll
       for (int i = 0; i < NV; ++i) n += max(0, min(32 * VEC, cols - (i * team.lanes + warp * 32) * VEC));
       return static_cast<float>(n);
     };
     const float mine = columnsOf(team.lane >> 5);
-    const float centre = s / fmaxf(mine, 1.0f);
+    const float centre = __fdividef(s, fmaxf(mine, 1.0f));  // any centre near the mean will do
     const F2 shift = splat(-centre);
     F2 q = splat(0.0f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if ((i * team.lanes + team.lane) * VEC >= cols) continue;
+      if (!full && (i * team.lanes + team.lane) * VEC >= cols) continue;
 #pragma unroll
       for (int e = 0; e < P; ++e) {
         const F2 d = v[i][e] + shift;
@@ -70,13 +70,13 @@ __device__ __forceinline__ void pairStatistics(Team &team, const F2 (&v)[NV][kPa
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
       mean = __shfl_sync(0xffffffffu, total, 0) * share;
-      const float off = sw / fmaxf(n, 1.0f) - mean;
+      const float off = __fdividef(sw, fmaxf(n, 1.0f)) - mean;  // the same quotient as the warp's centre
       squares = n > 0.0f ? fmaf(n * off, off, qw) : 0.0f;
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
       squares = __shfl_sync(0xffffffffu, squares, 0);
     }
-    rstd = 1.0f / sqrtf(squares * share + eps);
+    rstd = rsqrtf(squares * share + eps);
   }
 }
 
@@ -102,6 +102,8 @@ __global__ void __launch_bounds__(512) blockNormForwardVectorKernel(const __grid
   __shared__ float scratch[kTeamScratchFloats];
   Team team = makeTeam(teamLanes, scratch);
   const int cols = static_cast<int>(p.cols);
+  const float share = 1.0f / static_cast<float>(cols);
+  const bool full = team.lanes * NV * VEC == cols;
   const int64_t step = static_cast<int64_t>(gridDim.x) * team.count;
   auto colOf = [&](int i) { return (i * team.lanes + team.lane) * VEC; };
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * team.count + team.index; row < p.rows; row += step) {
@@ -111,7 +113,9 @@ __global__ void __launch_bounds__(512) blockNormForwardVectorKernel(const __grid
     };
     uint4 raw0[NV], rawX[kPostVectors], rawGate[kPostVectors];
     const bool gated = PASS != kPre && p.gateForm != kGateNone;
-    const int64_t gateRow = p.gateForm == kGateGroup ? row / p.groupRows : row;
+    int64_t gateRow = row;  // rows and groups are counted in 32 bits
+    if (PASS != kPre && p.gateForm == kGateGroup)
+      gateRow = static_cast<unsigned int>(row) / static_cast<unsigned int>(min(p.groupRows, static_cast<int64_t>(0x7fffffff)));
 #pragma unroll
     for (int i = 0; i < NV; ++i) raw0[i] = colOf(i) < cols ? raw(first, row, i) : make_uint4(0u, 0u, 0u, 0u);
     if constexpr (PASS != kPre) {
@@ -130,7 +134,7 @@ __global__ void __launch_bounds__(512) blockNormForwardVectorKernel(const __grid
       for (int i = 0; i < NV; ++i) packVector<ELEM>(raw0[i], colOf(i) < cols, colOf(i), row, p.checkpoint);
     }
     float mean, rstd;
-    pairStatistics<ELEM, KIND, NV>(team, v, cols, PASS == kPre ? p.epsB : p.epsA, mean, rstd);
+    pairStatistics<ELEM, KIND, NV>(team, v, cols, share, full, PASS == kPre ? p.epsB : p.epsA, mean, rstd);
     storeStatistics(team, PASS == kPre ? p.statsB : p.statsA, row, mean, rstd);
     if constexpr (PASS != kPre) {
       const F2 shift = splat(-mean), r = splat(rstd), alpha = splat(p.alpha);
@@ -159,7 +163,7 @@ __global__ void __launch_bounds__(512) blockNormForwardVectorKernel(const __grid
         if constexpr (PASS == kPostPre) widenPairs<ELEM>(stored, v[i]);  // as it is stored
       }
       if constexpr (PASS == kPostPre) {
-        pairStatistics<ELEM, KIND, NV>(team, v, cols, p.epsB, mean, rstd);
+        pairStatistics<ELEM, KIND, NV>(team, v, cols, share, full, p.epsB, mean, rstd);
         storeStatistics(team, p.statsB, row, mean, rstd);
       }
     }

@@ -85,7 +85,8 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
   // write the same values), so nothing waits here.
   float *weightB = reinterpret_cast<float *>(reinterpret_cast<char *>(slots) + stages * used);
   float *weightA = weightB + (kPrePart ? plan.sumsLd : 0), *biasA = weightA + (kPostPart ? plan.sumsLd : 0);
-  auto writeParams = [&](float *to, const void *v, const void *times) {
+  if (grouped) weightA += team.index * plan.sumsLd;  // each team its own: times the gate of the group it is in
+  auto writeParams = [&](float *to, const void *v, const void *times, int gateRow = -1) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (!has[i]) continue;
@@ -93,6 +94,12 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
       loadParamPairs<ELEM>(v, p.paramType, col0 + i * apart, x);
       if (times) {
         loadParamPairs<ELEM>(times, p.paramType, col0 + i * apart, y);
+#pragma unroll
+        for (int e = 0; e < P; ++e) x[e] = x[e] * y[e];
+      }
+      if (gateRow >= 0) {
+        loadPairs<ELEM>(p.gate.base, static_cast<int64_t>(gateRow) * p.gate.ld + col0 + i * apart, y);
+        gatePairs(y, p.gateAct);
 #pragma unroll
         for (int e = 0; e < P; ++e) x[e] = x[e] * y[e];
       }
@@ -179,7 +186,7 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
   }
 
   if constexpr (kPrePart) writeParams(weightB, p.b.weight, nullptr);
-  if constexpr (kPostPart) writeParams(weightA, p.a.weight, p.scale);
+  if constexpr (kPostPart) writeParams(weightA, p.a.weight, p.scale, grouped && now.live(plan) ? now.group : -1);
   if constexpr (kToken && kLayer) writeParams(biasA, p.a.bias, p.scale);
 
   const F2 zero = splat(0.0f);
@@ -218,7 +225,7 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
   unsigned int slot = slot0;
   while (now.live(plan)) {
     const RowScalars at = next;
-    const int row = now.row, run = now.run, group = now.group;
+    const int row = now.row, run = now.run;
     now.advance(plan, rows);
     fetchScalars(now, next);
     copiesWait(stages - 1);
@@ -289,7 +296,6 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
 #pragma unroll
       for (int k = 0; k < kValues; ++k) s[k] = zero;
       char *toDx = rowTo(p.dx, row), *toDgate = kToken ? rowTo(p.dgate, row) : nullptr;
-      const char *gateRow = grouped ? rowOf(p.gate, group) : nullptr;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         if (!has[i]) continue;
@@ -325,13 +331,6 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
             if constexpr (kLayer) sumA[1][i][e] = sumA[1][i][e] + dz[i][e];
             dz[i][e] = dz[i][e] * w[e];
           }
-          if (grouped) {
-            F2 a[P];
-            widenPairs<ELEM>(*reinterpret_cast<const uint4 *>(gateRow + i * apart * EB), a);
-            gatePairs(a, p.gateAct);
-#pragma unroll
-            for (int e = 0; e < P; ++e) dz[i][e] = dz[i][e] * a[e];
-          }
         }
 #pragma unroll
         for (int e = 0; e < P; ++e) {
@@ -363,6 +362,7 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
           for (int k = 0; k < kValues; ++k)
 #pragma unroll
             for (int e = 0; e < P; ++e) sumA[k][i][e] = zero;
+        if (grouped && now.live(plan)) writeParams(weightA, p.a.weight, p.scale, now.group);
       }
     }
     slot = slot + used == slotEnd ? slot0 : slot + used;
