@@ -50,6 +50,9 @@ CU_SOURCES = {
     "kernels/block_norm_grad_ahead_layer_f16.cu": [],
     "kernels/block_norm_grad_ahead_rms_bf16.cu": [],
     "kernels/block_norm_grad_ahead_layer_bf16.cu": [],
+    "kernels/block_norm_forward_ahead_f32.cu": [],
+    "kernels/block_norm_forward_ahead_f16.cu": [],
+    "kernels/block_norm_forward_ahead_bf16.cu": [],
     "kernels/checkpoint.cu": [],
     "kernels/checkpoint_grad_tcgen05.cu": [],
 }

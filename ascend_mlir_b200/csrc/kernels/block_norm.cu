@@ -33,88 +33,118 @@ __device__ __forceinline__ float elemAt(const void *p, int type, int64_t at) {
 
 constexpr int kFinishThreads = 512;
 
-// Adds two values per slot over each run of `slots` neighbouring slots (a power of two), in slot order; the first slot of a
-// run gets the sums.  A CTA is blockDim.x columns by blockDim.y slots.
-__device__ __forceinline__ void slotSums(float (&v)[2], int values, float2 *buf, int slots) {
-  const int c = threadIdx.x, s = threadIdx.y, width = blockDim.x;
-  buf[s * width + c] = make_float2(v[0], v[1]);
+__device__ __forceinline__ float4 plus(const float4 &a, const float4 &b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
+
+// Four columns per thread; a CTA is blockDim.x of them by blockDim.y slots.  Adds the slots' values over each run of
+// `slots` neighbouring slots (a power of two) in a tree; the first slot of a run gets the sums.
+template <int VALUES> __device__ __forceinline__ void slotSums(float4 (&v)[VALUES], float4 (*buf)[kFinishThreads], int slots) {
+  const int s = threadIdx.y, width = blockDim.x, at = s * width + threadIdx.x;
+#pragma unroll
+  for (int k = 0; k < VALUES; ++k) buf[k][at] = v[k];
   __syncthreads();
-  if ((s & (slots - 1)) == 0) {
-    float2 sum = buf[s * width + c];
-#pragma unroll 4
-    for (int i = 1; i < slots; ++i) {
-      const float2 f = buf[(s + i) * width + c];
-      sum.x += f.x;
-      if (values > 1) sum.y += f.y;
+  for (int o = slots / 2; o > 0; o >>= 1) {
+    if ((s & (slots - 1)) < o) {
+#pragma unroll
+      for (int k = 0; k < VALUES; ++k) buf[k][at] = plus(buf[k][at], buf[k][at + o * width]);
     }
-    v[0] = sum.x;
-    v[1] = sum.y;
+    __syncthreads();
   }
+#pragma unroll
+  for (int k = 0; k < VALUES; ++k) v[k] = buf[k][at];
   __syncthreads();
 }
 
-// The rows of sums `first`, first + step, ... below `count` (each `values` rows of sumsLd floats), added.
-__device__ __forceinline__ void addRows(const float *sums, int64_t sumsLd, int values, int64_t first, int64_t step, int64_t count, float (&v)[2]) {
-  v[0] = v[1] = 0.0f;
+// The rows of sums first, first + step, ... below `count` (VALUES rows of sumsLd floats each), added.
+template <int VALUES>
+__device__ __forceinline__ void addRows(const float *sums, int64_t sumsLd, int64_t first, int64_t step, int64_t count, float4 (&v)[VALUES]) {
+#pragma unroll
+  for (int k = 0; k < VALUES; ++k) v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
   for (int64_t r = first; r < count; r += step) {
-    v[0] += sums[r * values * sumsLd];
-    if (values > 1) v[1] += sums[(r * values + 1) * sumsLd];
+#pragma unroll
+    for (int k = 0; k < VALUES; ++k) v[k] = plus(v[k], *reinterpret_cast<const float4 *>(sums + (r * VALUES + k) * sumsLd));
   }
 }
 
-// Slots share the rows of sums; the order in which they are added depends on the sizes alone.
-__global__ void __launch_bounds__(kFinishThreads) blockNormFinishKernel(const __grid_constant__ FinishParams p) {
+// Slots share the rows of sums; the order in which they are added depends on the sizes alone.  Columns between `cols` and
+// sumsLd are read (they are in the workspace) and not stored.
+template <int VALUES> __global__ void __launch_bounds__(kFinishThreads) blockNormFinishKernel(const __grid_constant__ FinishParams p) {
   gridDependencyPrologue();
-  __shared__ float2 buf[kFinishThreads];
-  const int64_t col = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  __shared__ float4 buf[VALUES][kFinishThreads];
+  const int64_t col = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * 4;
   const bool live = col < p.cols;
   const int slot = threadIdx.y, allSlots = blockDim.y;
-  const int values = p.layer ? 2 : 1;
   if (p.sumsA) {
     // slots as (groups at once) x (slots per group)
     int atOnce = 1;
     while (atOnce < p.groups && atOnce < allSlots) atOnce *= 2;
     const int perGroup = allSlots / atOnce;
-    const float w = live ? elemAt(p.weight, p.paramType, col) : 0.0f;
-    const float b = live && p.layer ? elemAt(p.bias, p.paramType, col) : 0.0f;
-    const float scale = live && p.scale ? elemAt(p.scale, p.paramType, col) : 1.0f;
-    float total[2] = {0.0f, 0.0f};
+    float w[4], b[4], scale[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool some = col + j < p.cols;
+      w[j] = some ? elemAt(p.weight, p.paramType, col + j) : 0.0f;
+      b[j] = some && VALUES > 1 ? elemAt(p.bias, p.paramType, col + j) : 0.0f;
+      scale[j] = some && p.scale ? elemAt(p.scale, p.paramType, col + j) : 1.0f;
+    }
+    float4 total[VALUES];
+#pragma unroll
+    for (int k = 0; k < VALUES; ++k) total[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int64_t g0 = 0; g0 < p.groups; g0 += atOnce) {
       const int64_t group = g0 + slot / perGroup;
       const bool mine = live && group < p.groups;
-      float s[2] = {0.0f, 0.0f};
-      if (mine) addRows(p.sumsA + group * p.chunks * values * p.sumsLd + col, p.sumsLd, values, slot & (perGroup - 1), perGroup, p.chunks, s);
-      if (perGroup > 1) slotSums(s, values, buf, perGroup);
+      float4 s[VALUES];
+      addRows<VALUES>(p.sumsA + group * p.chunks * VALUES * p.sumsLd + col, p.sumsLd, slot & (perGroup - 1), perGroup, mine ? p.chunks : 0, s);
+      if (perGroup > 1) slotSums<VALUES>(s, buf, perGroup);
       if (mine && (slot & (perGroup - 1)) == 0) {
-        float a = 1.0f;
-        if (p.gateForm == kGateGroup) {
-          a = gateValue(elemAt(p.gate, p.elemType, group * p.gateLd + col), p.gateAct);
-          p.dgate[group * p.dgateLd + col] = scale * fmaf(w, s[0], b * s[1]) * gateSlope(a, p.gateAct);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (col + j >= p.cols) break;
+          float a = 1.0f;
+          const float s0 = reinterpret_cast<const float *>(&s[0])[j], s1 = VALUES > 1 ? reinterpret_cast<const float *>(&s[VALUES - 1])[j] : 0.0f;
+          if (p.gateForm == kGateGroup) {
+            a = gateValue(elemAt(p.gate, p.elemType, group * p.gateLd + col + j), p.gateAct);
+            p.dgate[group * p.dgateLd + col + j] = scale[j] * fmaf(w[j], s0, b[j] * s1) * gateSlope(a, p.gateAct);
+          }
+          float &t0 = reinterpret_cast<float *>(&total[0])[j];
+          t0 = fmaf(a, s0, t0);
+          if constexpr (VALUES > 1) {
+            float &t1 = reinterpret_cast<float *>(&total[1])[j];
+            t1 = fmaf(a, s1, t1);
+          }
         }
-        total[0] = fmaf(a, s[0], total[0]);
-        total[1] = fmaf(a, s[1], total[1]);
       }
     }
-    if (p.groups > 1) slotSums(total, values, buf, allSlots);
+    if (p.groups > 1) slotSums<VALUES>(total, buf, allSlots);
     if (live && slot == 0) {
-      p.dweight[col] = scale * total[0];
-      if (p.dbias) p.dbias[col] = scale * total[1];
-      if (p.dscale) p.dscale[col] = fmaf(w, total[0], b * total[1]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (col + j >= p.cols) break;
+        const float t0 = reinterpret_cast<const float *>(&total[0])[j], t1 = VALUES > 1 ? reinterpret_cast<const float *>(&total[VALUES - 1])[j] : 0.0f;
+        p.dweight[col + j] = scale[j] * t0;
+        if (p.dbias) p.dbias[col + j] = scale[j] * t1;
+        if (p.dscale) p.dscale[col + j] = fmaf(w[j], t0, b[j] * t1);
+      }
     }
   }
   if (p.sumsB) {
-    float s[2] = {0.0f, 0.0f};
-    if (live) addRows(p.sumsB + col, p.sumsLd, values, slot, allSlots, p.teams, s);
-    slotSums(s, values, buf, allSlots);
+    float4 s[VALUES];
+    addRows<VALUES>(p.sumsB + col, p.sumsLd, slot, allSlots, live ? p.teams : 0, s);
+    slotSums<VALUES>(s, buf, allSlots);
     if (live && slot == 0) {
-      p.nextWeight[col] = s[0];
-      if (p.nextBias) p.nextBias[col] = s[1];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (col + j >= p.cols) break;
+        p.nextWeight[col + j] = reinterpret_cast<const float *>(&s[0])[j];
+        if (p.nextBias) p.nextBias[col + j] = reinterpret_cast<const float *>(&s[VALUES - 1])[j];
+      }
     }
   }
 }
 
 // ---- launch shape -----------------------------------------------------------------------------------------------
+constexpr size_t kAheadBytes = 225 * 1024;  // of the 227 KB that the CTAs of an SM can have, each with 1 KB of its own
+
 struct TeamShape { bool vector; int nv, lanes, teamsPerCta; };
 
 TeamShape shapeOf(int vec, int nv, int64_t cols) {
@@ -129,12 +159,11 @@ TeamShape shapeOf(int vec, int nv, int64_t cols) {
 int scalarElements(int64_t cols) { return cols <= kScalarSmall * 512 ? kScalarSmall : kScalarLarge; }
 
 // A team has at most 512 threads.  Few rows: one vector per thread while that is enough, for the shortest way through one
-// row.  Rows enough to fill the SMs several times: 32 columns per thread, since what a row costs a thread besides its
-// vectors (statistics across warps, addresses) is as much as two or three vectors.
+// row; else 16 columns per thread.
 TeamShape forwardShape(int elemType, int64_t rows, int64_t cols, bool vector, int smCount) {
   const int vec = vector ? (elemType == kF32 ? 4 : 8) : 1;
   if (!vector) return shapeOf(1, scalarElements(cols), cols);
-  const int64_t perThread = rows >= 4 * smCount ? 32 : rows >= smCount ? 16 : vec;
+  const int64_t perThread = rows >= smCount ? 16 : vec;
   int nv = 1;
   while (nv * vec < perThread && static_cast<int64_t>(nv) * vec * 32 < cols) nv *= 2;
   while (static_cast<int64_t>(nv) * vec * 512 < cols) nv *= 2;
@@ -232,7 +261,38 @@ int launchBlockNorm(const BlockNormLaunch &l, cudaStream_t stream, int *launched
   vector = vector && rowsAligned(l.checkpoint.codes, l.checkpoint.codesLd, 1, vec);
   int device = 0;
   if (const cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return e;
-  const TeamShape s = forwardShape(l.elemType, l.rows, l.cols, vector, deviceSmCount(device));
+  const int sms = deviceSmCount(device);
+  // Rows fetched ahead by teams that stay, where every team gets several rows and two fit in shared memory beside the
+  // parameters: 1024 threads per SM (64 registers each) before a block, 512 behind it.
+  if (vector) {
+    TeamShape s = gradShape(l.elemType, kRmsNorm, l.cols, true);
+    const int threadsPerSm = l.pass == kPre ? 1024 : 512;
+    if (s.nv <= 2) {
+      s.teamsPerCta = std::max(1, std::min(15, 512 / s.lanes));
+      const int threads = s.lanes * s.teamsPerCta;
+      const int ctasPerSm = std::max(1, threadsPerSm / threads);
+      const int tensors = l.pass == kPre ? 1 : l.gateForm == kGateToken ? 3 : 2;
+      const int vectors = (l.kind == kLayerNorm ? 2 : 1) * (l.pass == kPostPre ? 2 : 1);
+      const int paramLd = static_cast<int>((l.cols + 3) / 4 * 4);
+      const size_t paramBytes = static_cast<size_t>(vectors) * static_cast<size_t>(paramLd) * sizeof(float);
+      const size_t rowBytes = static_cast<size_t>(tensors) * static_cast<size_t>(s.nv) * 16 * static_cast<size_t>(threads);
+      const size_t perCta = kAheadBytes / static_cast<size_t>(ctasPerSm) - 1536;
+      const int stages = static_cast<int>(std::min<size_t>(4, (perCta - std::min(perCta, paramBytes)) / rowBytes));
+      if (stages >= 2 && l.rows >= static_cast<int64_t>(4) * sms * ctasPerSm * s.teamsPerCta) {
+        const bool full = static_cast<int64_t>(s.lanes) * s.nv * vec == l.cols;
+        const ForwardAheadKernel kernel = l.elemType == kF32   ? forwardAheadKernel<kF32>(l.kind, l.pass, full, s.nv)
+                                          : l.elemType == kF16 ? forwardAheadKernel<kF16>(l.kind, l.pass, full, s.nv)
+                                                               : forwardAheadKernel<kBF16>(l.kind, l.pass, full, s.nv);
+        cudaError_t e = reserveSharedMemory(reinterpret_cast<const void *>(kernel), static_cast<int>(kAheadBytes));
+        if (e != cudaSuccess) return e;
+        e = launchDependent(kernel, dim3(static_cast<unsigned int>(sms * ctasPerSm)), dim3(static_cast<unsigned int>(threads)),
+                            static_cast<size_t>(stages) * rowBytes + paramBytes, stream, l, s.lanes, stages, paramLd);
+        if (e == cudaSuccess && launched) *launched += 1;
+        return e;
+      }
+    }
+  }
+  const TeamShape s = forwardShape(l.elemType, l.rows, l.cols, vector, sms);
   const ForwardKernel kernel = l.elemType == kF32   ? forwardKernel<kF32>(l.kind, l.pass, vector, s.nv)
                                : l.elemType == kF16 ? forwardKernel<kF16>(l.kind, l.pass, vector, s.nv)
                                                     : forwardKernel<kBF16>(l.kind, l.pass, vector, s.nv);
@@ -289,7 +349,6 @@ int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *
     const size_t paramBytes = static_cast<size_t>(vectors + perTeam) * static_cast<size_t>(plan.sumsLd) * sizeof(float);
     const size_t rowBytes = static_cast<size_t>(tensors) * static_cast<size_t>(s.nv) * 16 * static_cast<size_t>(s.lanes) * static_cast<size_t>(s.teamsPerCta);
     const int64_t ctasPerSm = std::max<int64_t>(1, (gradTeamsPerSm(l.elemType, l.kind, l.cols) + s.teamsPerCta - 1) / s.teamsPerCta);
-    constexpr size_t kAheadBytes = 225 * 1024;  // of the 227 KB that the CTAs of an SM can have, each with 1 KB of its own
     const size_t perCta = kAheadBytes / static_cast<size_t>(ctasPerSm) - 1536;
     const int stages = static_cast<int>(std::min<size_t>(4, std::max<size_t>(2, (perCta - std::min(perCta, paramBytes)) / rowBytes)));
     const size_t slotBytes = static_cast<size_t>(stages) * rowBytes + paramBytes;
@@ -336,10 +395,11 @@ int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *
   f.nextBias = l.db.bias;
   f.dgate = static_cast<float *>(l.gateForm == kGateGroup ? l.dgate.base : nullptr);
   f.dgateLd = l.dgate.ld;
-  // whole 128-byte lines of the sums where that still gives 64 CTAs, else less of a line and more slots
-  const int width = l.cols >= 2048 ? 32 : l.cols >= 1024 ? 16 : 8;
-  const unsigned int grid = static_cast<unsigned int>((l.cols + width - 1) / width);
-  const cudaError_t e = launchDependent(blockNormFinishKernel, dim3(grid), dim3(static_cast<unsigned int>(width), static_cast<unsigned int>(kFinishThreads / width)), 0, stream, f);
+  // whole 128-byte lines of the sums (8 threads of 4 columns) for wide rows, half lines and twice the slots else
+  const int width = l.cols >= 4096 ? 8 : 4;
+  const unsigned int grid = static_cast<unsigned int>((l.cols + 4 * width - 1) / (4 * width));
+  const auto finish = f.layer ? blockNormFinishKernel<2> : blockNormFinishKernel<1>;
+  const cudaError_t e = launchDependent(finish, dim3(grid), dim3(static_cast<unsigned int>(width), static_cast<unsigned int>(kFinishThreads / width)), 0, stream, f);
   if (e == cudaSuccess && launched) *launched += 1;
   return e;
 }

@@ -1,0 +1,7 @@
+#include "kernels/block_norm_forward_ahead_pick.cuh"
+
+namespace afir {
+namespace kernels {
+template ForwardAheadKernel forwardAheadKernel<kBF16>(int kind, int pass, bool full, int nv);
+} // namespace kernels
+} // namespace afir

@@ -16,37 +16,32 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// 128 columns are 16 lanes (8 columns each, 16-bit types) or 32 lanes (4 each, f32).  Threads are numbered through
-// [rows, blocks of 128, lanes] (a row may end inside a block), and each takes kAhead places a stride apart, all loaded
-// before the first is used.
+// 128 columns are 16 lanes (8 columns each, 16-bit types) or 32 lanes (4 each, f32).  A team of whole warps walks a row,
+// kAhead vectors per thread at a time, all loaded before the first is used; a row may end inside a block.
 constexpr int kAhead = 4;
 template <int ELEM>
-__global__ void __launch_bounds__(kThreads) checkpointPackVectorKernel(const __grid_constant__ CheckpointPackLaunch p) {
+__global__ void __launch_bounds__(kThreads) checkpointPackVectorKernel(const __grid_constant__ CheckpointPackLaunch p, int lanes) {
   gridDependencyPrologue();
   constexpr int VEC = ElemOf<ELEM>::kVec;
-  constexpr int kLanes = kCheckpointBlock / VEC;
   const int cols = static_cast<int>(p.cols);
-  const unsigned int blocks = static_cast<unsigned int>((cols + kCheckpointBlock - 1) / kCheckpointBlock);
-  const int64_t units = p.rows * blocks * kLanes;
-  // whole warps go round together: the bound is rounded up to a warp
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * (kThreads * kAhead) + threadIdx.x; base < (units + 31) / 32 * 32;
-       base += static_cast<int64_t>(gridDim.x) * (kThreads * kAhead)) {
-    uint4 raw[kAhead];
-    int64_t row[kAhead];
-    int col[kAhead];
-    bool live[kAhead];
+  const int teams = kThreads / lanes, team = static_cast<int>(threadIdx.x) / lanes, lane = static_cast<int>(threadIdx.x) - team * lanes;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * teams;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * teams + team; row < p.rows; row += step) {
+    const char *from = static_cast<const char *>(p.x.base) + row * p.x.ld * (16 / VEC);
+    for (int base = lane * VEC; base - lane * VEC < cols; base += lanes * VEC * kAhead) {
+      uint4 raw[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int64_t u = base + i * kThreads, block = u / kLanes;
-      // the division by the row's blocks in 32 bits where the count allows
-      row[i] = block <= 0xffffffffll ? static_cast<unsigned int>(block) / blocks : block / blocks;
-      col[i] = static_cast<int>(block - row[i] * blocks) * kCheckpointBlock + static_cast<int>(u & (kLanes - 1)) * VEC;
-      live[i] = u < units && col[i] < cols;
-      raw[i] = live[i] ? *reinterpret_cast<const uint4 *>(static_cast<const char *>(p.x.base) + (row[i] * p.x.ld + col[i]) * (16 / VEC))
-                       : make_uint4(0u, 0u, 0u, 0u);
+      for (int i = 0; i < kAhead; ++i) {
+        const int col = base + i * lanes * VEC;
+        raw[i] = col < cols ? *reinterpret_cast<const uint4 *>(from + static_cast<int64_t>(col) * (16 / VEC)) : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int col = base + i * lanes * VEC;
+        if (col - lane * VEC >= cols) break;  // the whole team's
+        packVector<ELEM>(raw[i], col < cols, col, row, p.out);
+      }
     }
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) packVector<ELEM>(raw[i], live[i], col[i], row[i], p.out);
   }
 }
 
@@ -119,7 +114,9 @@ int launchCheckpointPack(const CheckpointPackLaunch &l, cudaStream_t stream, int
   cudaError_t e;
   if (vector) {
     const auto kernel = l.elemType == kF32 ? checkpointPackVectorKernel<kF32> : l.elemType == kF16 ? checkpointPackVectorKernel<kF16> : checkpointPackVectorKernel<kBF16>;
-    e = launchDependent(kernel, dim3(gridFor(l.rows * blocks * (kCheckpointBlock / vec), kThreads * kAhead)), dim3(kThreads), 0, stream, l);
+    int lanes = 32;  // the fewest (32, 64, 128 or 256) that take a row at one go
+    while (lanes < kThreads && lanes * vec * kAhead < l.cols) lanes *= 2;
+    e = launchDependent(kernel, dim3(gridFor(l.rows, kThreads / lanes)), dim3(kThreads), 0, stream, l, lanes);
   } else {
     const auto kernel = l.elemType == kF32 ? checkpointPackScalarKernel<kF32> : l.elemType == kF16 ? checkpointPackScalarKernel<kF16> : checkpointPackScalarKernel<kBF16>;
     e = launchDependent(kernel, dim3(gridFor(l.rows * blocks, kThreads / 32)), dim3(kThreads), 0, stream, l);

@@ -508,3 +508,56 @@ def test_combinations(rt):
             want.update(ref.next_norm(outs["out"].double(), w, c))
         check(outs, {k: v for k, v in want.items() if k in outs}, (kind, gate, nxt, stats, scaled))
         assert ("rstd" in outs) == stats
+
+
+# Rows enough for teams that stay and fetch rows ahead, with vectors that end at the row's end and beyond it.
+MANY = [(40000, 64), (20001, 136), (9999, 520), (5000, 1024), (5001, 1000), (2600, 2048), (2400, 4096), (1300, 4104), (1250, 8192)]
+
+
+@pytest.mark.parametrize("dtype,kind", [("bf16", "rms"), ("f16", "layer"), ("f32", "rms"), ("f32", "layer"), ("bf16", "layer")])
+def test_many_rows_forward(rt, dtype, kind):
+    for i, (T, D) in enumerate(MANY):
+        gate, a, G = GATES[i % len(GATES)]
+        c = case("norm", T, D, dtype, kind)
+        t = block_inputs(dict(c, gate=gate, G=G), 400 + i)
+        outs = call(rt, descriptors.block_norm(dtype, kind=kind, eps=EPS, checkpoint=i % 2 == 1), sizes(c), t)
+        torch.cuda.synchronize()
+        check(outs, ref.forward(wide(t), c), (T, D))
+        if i % 2:
+            check_checkpoint(t["x"], outs, (T, D))
+        for nxt in (False, True):
+            c = case("gated", T, D, dtype, kind, gate=gate, act=a, G=G, next=nxt)
+            spec = descriptors.gated_residual(dtype, kind=kind, eps=EPS, alpha=ALPHA, gate=gate, gate_act=a, next_norm=nxt, scale=i % 3 != 0,
+                                              checkpoint=i % 2 == 0)
+            outs = call(rt, spec, sizes(c), t)
+            torch.cuda.synchronize()
+            w = wide(t)
+            if i % 3 == 0:
+                del w["scale"]
+            check(outs, ref.forward(w, c), (T, D, gate, nxt))
+            if nxt:
+                check(outs, ref.next_norm(outs["out"].double(), w, c), (T, D, gate, "next"))
+            if i % 2 == 0:
+                check_checkpoint(t["y"], outs, (T, D))
+
+
+@pytest.mark.parametrize("dtype,kind", [("bf16", "rms"), ("f16", "layer"), ("f32", "rms")])
+def test_many_rows_gradients(rt, dtype, kind):
+    for i, (T, D) in enumerate(MANY):
+        gate, a, G = GATES[(i + 1) % len(GATES)]
+        c = case("gated", T, D, dtype, kind, gate=gate, act=a, G=G, next=i % 2 == 0)
+        t = block_inputs(c, 500 + i)
+        statistics_into(t, c, t["y"].double())
+        statistics_into(t, c, t["out"].double(), "next_")
+        spec = descriptors.gated_residual_grad(dtype, kind=kind, alpha=ALPHA, gate=gate, gate_act=a, next_norm=c["next"], scale=i % 3 != 0)
+        outs = call(rt, spec, sizes(c), t)
+        torch.cuda.synchronize()
+        w = wide(t)
+        if i % 3 == 0:
+            del w["scale"]
+        # a group's or a column's sum may run over (rows / teams) rows in a row of f32 adds: at most 300 here
+        saved, ref.COLUMN = ref.COLUMN, 400
+        try:
+            check(outs, ref.gradient(w, c), (T, D, gate))
+        finally:
+            ref.COLUMN = saved
