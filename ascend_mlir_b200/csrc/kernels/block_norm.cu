@@ -263,19 +263,18 @@ int launchBlockNorm(const BlockNormLaunch &l, cudaStream_t stream, int *launched
   if (const cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return e;
   const int sms = deviceSmCount(device);
   // Rows fetched ahead by teams that stay, where every team gets several rows and two fit in shared memory beside the
-  // parameters: 1024 threads per SM (64 registers each) before a block, 512 behind it.
+  // parameters: 1024 threads per SM (64 registers each) before a block, up to 768 (80 registers) behind it, in one CTA that
+  // shares its parameters.
   if (vector) {
     TeamShape s = gradShape(l.elemType, kRmsNorm, l.cols, true);
-    const int threadsPerSm = l.pass == kPre ? 1024 : 512;
     if (s.nv <= 2) {
-      s.teamsPerCta = std::max(1, std::min(15, 512 / s.lanes));
+      const int ctaThreads = l.pass == kPre ? kForwardAheadThreads : kForwardAheadPostThreads, ctasPerSm = l.pass == kPre ? 2 : 1;
+      s.teamsPerCta = std::max(1, std::min(15, ctaThreads / s.lanes));
       const int threads = s.lanes * s.teamsPerCta;
-      const int ctasPerSm = std::max(1, threadsPerSm / threads);
       const int tensors = l.pass == kPre ? 1 : l.gateForm == kGateToken ? 3 : 2;
       const int vectors = (l.kind == kLayerNorm ? 2 : 1) * (l.pass == kPostPre ? 2 : 1);
-      const int paramLd = static_cast<int>((l.cols + 3) / 4 * 4);
-      const size_t paramBytes = static_cast<size_t>(vectors) * static_cast<size_t>(paramLd) * sizeof(float);
-      const size_t rowBytes = static_cast<size_t>(tensors) * static_cast<size_t>(s.nv) * 16 * static_cast<size_t>(threads);
+      const size_t paramBytes = static_cast<size_t>(vectors) * static_cast<size_t>(s.lanes * s.nv * vec) * sizeof(float);
+      const size_t rowBytes = static_cast<size_t>(tensors) * static_cast<size_t>(s.nv) * 16 * static_cast<size_t>(ctaThreads);
       const size_t perCta = kAheadBytes / static_cast<size_t>(ctasPerSm) - 1536;
       const int stages = static_cast<int>(std::min<size_t>(4, (perCta - std::min(perCta, paramBytes)) / rowBytes));
       if (stages >= 2 && l.rows >= static_cast<int64_t>(4) * sms * ctasPerSm * s.teamsPerCta) {
@@ -286,7 +285,7 @@ int launchBlockNorm(const BlockNormLaunch &l, cudaStream_t stream, int *launched
         cudaError_t e = reserveSharedMemory(reinterpret_cast<const void *>(kernel), static_cast<int>(kAheadBytes));
         if (e != cudaSuccess) return e;
         e = launchDependent(kernel, dim3(static_cast<unsigned int>(sms * ctasPerSm)), dim3(static_cast<unsigned int>(threads)),
-                            static_cast<size_t>(stages) * rowBytes + paramBytes, stream, l, s.lanes, stages, paramLd);
+                            static_cast<size_t>(stages) * rowBytes + paramBytes, stream, l, s.lanes, stages);
         if (e == cudaSuccess && launched) *launched += 1;
         return e;
       }
@@ -341,15 +340,15 @@ int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *
     for (const void *v : {l.a.weight, l.a.bias, l.b.weight, l.scale}) vector = vector && vectorAligned(v);
     vector = vector && rowsAligned(l.checkpoint.codes, l.checkpoint.codesLd, 1, vec);
     TeamShape s = gradShape(l.elemType, l.kind, l.cols, vector);
+    if (vector) s.teamsPerCta = std::max(1, std::min(15, kGradAheadThreads / s.lanes));
     // rows fetched ahead: as many (2 to 4) as the CTAs of an SM have shared memory for beside their parameters; rows too
     // wide for two take the kernel without
     const int tensors = (l.pass != kPost ? 2 : 0) + (l.dout.base ? 1 : 0) + (l.pass != kPre ? 1 : 0) + (l.gateForm == kGateToken ? 1 : 0);
     const int vectors = (l.pass != kPost ? 1 : 0) + (l.pass != kPre ? 1 : 0) + (l.gateForm == kGateToken && l.kind == kLayerNorm ? 1 : 0);
     const int perTeam = l.gateForm == kGateGroup && l.pass != kPre ? s.teamsPerCta - 1 : 0;  // a team's group has its own gate
-    const size_t paramBytes = static_cast<size_t>(vectors + perTeam) * static_cast<size_t>(plan.sumsLd) * sizeof(float);
-    const size_t rowBytes = static_cast<size_t>(tensors) * static_cast<size_t>(s.nv) * 16 * static_cast<size_t>(s.lanes) * static_cast<size_t>(s.teamsPerCta);
-    const int64_t ctasPerSm = std::max<int64_t>(1, (gradTeamsPerSm(l.elemType, l.kind, l.cols) + s.teamsPerCta - 1) / s.teamsPerCta);
-    const size_t perCta = kAheadBytes / static_cast<size_t>(ctasPerSm) - 1536;
+    const size_t paramBytes = static_cast<size_t>(vectors + perTeam) * static_cast<size_t>(s.lanes * s.nv * vec) * sizeof(float);
+    const size_t rowBytes = static_cast<size_t>(tensors) * static_cast<size_t>(s.nv) * 16 * kGradAheadThreads;
+    const size_t perCta = kAheadBytes - 1536;
     const int stages = static_cast<int>(std::min<size_t>(4, std::max<size_t>(2, (perCta - std::min(perCta, paramBytes)) / rowBytes)));
     const size_t slotBytes = static_cast<size_t>(stages) * rowBytes + paramBytes;
     const GradAheadKernel ahead = vector && slotBytes <= kAheadBytes ? aheadKernel(l.elemType, l.kind, l.pass, l.gateForm == kGateToken, static_cast<int64_t>(s.lanes) * s.nv * vec == l.cols, s.nv) : nullptr;

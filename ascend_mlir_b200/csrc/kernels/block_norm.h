@@ -21,6 +21,9 @@ constexpr int64_t kMaxNormCols = 16384;  // a row stays in the registers of one 
 constexpr int64_t kMaxNormRows = 1ll << 30;  // rows, and rows of column sums, are counted in 32 bits
 constexpr int kCheckpointBlock = 128;    // columns that share one power of two
 
+// Threads of a CTA (at most) in the kernels that fetch rows ahead; a row's slots are laid out for that many.
+constexpr int kForwardAheadThreads = 512, kForwardAheadPostThreads = 768, kGradAheadThreads = 512;
+
 enum NormPass : int { kPre = 0, kPost = 1, kPostPre = 2 };
 enum NormKind : int { kRmsNorm = 0, kLayerNorm = 1 };
 enum GateForm : int { kGateNone = 0, kGateToken = 1, kGateGroup = 2 };  // none; a value per element; a row per group of rows

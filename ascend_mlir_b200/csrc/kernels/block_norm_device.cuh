@@ -100,16 +100,21 @@ template <int ELEM, int VEC> __device__ __forceinline__ void loadParam(const voi
 }
 
 // ---- teams ------------------------------------------------------------------------------------------------------
-// `lanes` threads (a multiple of 32, at most 1024) that hold one row; a CTA has one or more teams.
-// Sums over a team: a shuffle tree in each warp, then the warps' sums through shared memory, added by every warp in the
-// same order.  The two halves of the buffer alternate, so one barrier per sum is enough: whoever writes a half again has
-// passed the barrier of the sum between, which every reader of that half reached after reading.
+// `lanes` threads (a multiple of 32, at most 512) that hold one row; a CTA of up to 1024 threads has one or more of them
+// (at most 15 of more than a warp: each has a named barrier).  Sums over a team: a shuffle tree in each warp, then the
+// warps' sums through shared memory, which every thread of up to 8 warps adds up itself in the same order (a second shuffle
+// tree would be five more dependent latencies); of more warps, each warp adds them in a shuffle tree.  The two halves of the buffer alternate, so one barrier per sum is enough: whoever writes
+// a half again has passed the barrier of the sum between, which every reader of that half reached after reading.
 struct Team {
   int lanes, lane, index, count;  // threads in it; this thread's place; which of the CTA's; how many the CTA has
-  float *scratch;                 // this team's slice of the CTA's buffer
+  float *scratch;                 // this team's slice of the CTA's buffer: [halves][kTeamValues][slice], zero beyond its warps
   int half;
 };
-constexpr int kTeamScratchFloats = 2 * 2 * 32;  // halves x values x warps of a CTA
+constexpr int kTeamValues = 3;
+constexpr int kTeamSlice = 64;  // floats per value: the CTA's warps, each team's rounded up to 16 bytes
+constexpr int kTeamScratchFloats = 2 * kTeamValues * kTeamSlice;
+
+__device__ __forceinline__ void teamBarrier(const Team &t) { asm volatile("bar.sync %0, %1;" ::"r"(t.index + 1), "r"(t.lanes) : "memory"); }
 
 __device__ __forceinline__ Team makeTeam(int lanes, float *scratch) {
   Team t;
@@ -117,8 +122,16 @@ __device__ __forceinline__ Team makeTeam(int lanes, float *scratch) {
   t.index = static_cast<int>(threadIdx.x) / lanes;
   t.lane = static_cast<int>(threadIdx.x) - t.index * lanes;
   t.count = static_cast<int>(blockDim.x) / lanes;
-  t.scratch = scratch + t.index * (lanes >> 5);
+  const int slice = ((lanes >> 5) + 3) & ~3;
+  t.scratch = scratch + t.index * slice;
   t.half = 0;
+  if (lanes > 32) {
+    if (t.lane < slice) {
+#pragma unroll
+      for (int v = 0; v < 2 * kTeamValues; ++v) t.scratch[v * kTeamSlice + t.lane] = 0.0f;
+    }
+    teamBarrier(t);
+  }
   return t;
 }
 __device__ __forceinline__ float warpSum(float v) {
@@ -126,25 +139,44 @@ __device__ __forceinline__ float warpSum(float v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+// The warps' values of one kind, four at a time.
+template <class F> __device__ __forceinline__ void eachFourWarps(const Team &t, F f) {
+  const int warps = t.lanes >> 5;
+#pragma unroll
+  for (int w = 0; w < 16; w += 4)
+    if (w < warps) f(w);
+}
 template <int N> __device__ __forceinline__ void teamSum(Team &t, float (&v)[N]) {
-  static_assert(N <= 2, "the buffer holds two values per warp");
+  static_assert(N <= kTeamValues, "the buffer holds that many values per warp");
 #pragma unroll
   for (int n = 0; n < N; ++n) v[n] = warpSum(v[n]);
   if (t.lanes == 32) return;
-  float *buf = t.scratch + t.half * 64;
+  float *buf = t.scratch + t.half * (kTeamValues * kTeamSlice);
   t.half ^= 1;
-  const int lane = threadIdx.x & 31;
-  if (lane == 0) {
+  if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) buf[n * 32 + (t.lane >> 5)] = v[n];
+    for (int n = 0; n < N; ++n) buf[n * kTeamSlice + (t.lane >> 5)] = v[n];
   }
-  asm volatile("bar.sync %0, %1;" ::"r"(t.index + 1), "r"(t.lanes) : "memory");
-  const int warps = t.lanes >> 5;
+  teamBarrier(t);
+  if (t.lanes <= 256) {
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-    v[n] = lane < warps ? buf[n * 32 + lane] : 0.0f;
+    for (int n = 0; n < N; ++n) {
+      const float4 a = *reinterpret_cast<const float4 *>(buf + n * kTeamSlice);
+      v[n] = (a.x + a.y) + (a.z + a.w);
+      if (t.lanes > 128) {
+        const float4 b = *reinterpret_cast<const float4 *>(buf + n * kTeamSlice + 4);
+        v[n] += (b.x + b.y) + (b.z + b.w);
+      }
+    }
+  } else {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+    for (int n = 0; n < N; ++n) {
+      v[n] = lane < (t.lanes >> 5) ? buf[n * kTeamSlice + lane] : 0.0f;
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+      v[n] = __shfl_sync(0xffffffffu, v[n], 0);
+    }
   }
 }
 

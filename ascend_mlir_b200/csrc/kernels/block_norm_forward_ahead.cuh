@@ -13,12 +13,12 @@ namespace kernels {
 
 // FULL: every thread's vectors lie inside the row.
 template <int ELEM, int KIND, int PASS, bool FULL, int NV>
-__global__ void __launch_bounds__(PASS == kPre ? 1024 : 512, 1) blockNormForwardAheadKernel(const __grid_constant__ BlockNormLaunch p, int teamLanes,
-                                                                                          int stages, int paramLd) {
+__global__ void __launch_bounds__(PASS == kPre ? kForwardAheadThreads : kForwardAheadPostThreads, PASS == kPre ? 2 : 1) blockNormForwardAheadKernel(const __grid_constant__ BlockNormLaunch p, int teamLanes,
+                                                                                          int stages) {
   gridDependencyPrologue();
   constexpr bool kLayer = KIND == kLayerNorm;
   constexpr int VEC = ElemOf<ELEM>::kVec, P = kPairs<ELEM>, EB = 16 / VEC;
-  extern __shared__ uint4 slots[];  // [stages][tensors][NV][threads], then parameters
+  extern __shared__ uint4 slots[];  // [stages][tensors][NV][perVector / 16], then parameters
   __shared__ float scratch[kTeamScratchFloats];
   Team team = makeTeam(teamLanes, scratch);
   const int cols = static_cast<int>(p.cols), rows = static_cast<int>(p.rows);
@@ -34,8 +34,8 @@ __global__ void __launch_bounds__(PASS == kPre ? 1024 : 512, 1) blockNormForward
   const bool token = PASS != kPre && p.gateForm == kGateToken, grouped = PASS != kPre && p.gateForm == kGateGroup;
   const unsigned int groupRows = static_cast<unsigned int>(min(p.groupRows, static_cast<int64_t>(0x7fffffff)));
 
-  const unsigned int perVector = blockDim.x * 16, perTensor = NV * perVector;
-  const unsigned int atX = PASS == kPre ? 0 : perTensor, atGate = 2 * perTensor;
+  constexpr unsigned int perVector = (PASS == kPre ? kForwardAheadThreads : kForwardAheadPostThreads) * 16, perTensor = NV * perVector;
+  constexpr unsigned int atX = PASS == kPre ? 0 : perTensor, atGate = 2 * perTensor;
   const unsigned int used = PASS == kPre ? perTensor : token ? 3 * perTensor : 2 * perTensor;
   const unsigned int slot0 = threadIdx.x * 16, slotEnd = slot0 + stages * used;
   const unsigned int slotsAt = static_cast<unsigned int>(__cvta_generic_to_shared(slots));
@@ -69,6 +69,8 @@ __global__ void __launch_bounds__(PASS == kPre ? 1024 : 512, 1) blockNormForward
   for (unsigned int s = slot0; s < slotEnd; s += used, ahead += step) fetch(ahead, s);
 
   // Parameters of all teams of the CTA; a thread reads only what it has written itself (teams write the same values).
+  // 16-byte pieces in the order of the threads, free of bank conflicts.
+  const int paramLd = team.lanes * NV * VEC;
   float *weightA = reinterpret_cast<float *>(reinterpret_cast<char *>(slots) + stages * used);
   float *biasA = weightA + (PASS != kPre ? paramLd : 0), *weightB = biasA + (PASS != kPre && kLayer ? paramLd : 0);
   float *biasB = weightB + (PASS != kPost ? paramLd : 0);
@@ -86,7 +88,7 @@ __global__ void __launch_bounds__(PASS == kPre ? 1024 : 512, 1) blockNormForward
 #pragma unroll
       for (int e = 0; e < P / 2; ++e) {
         const F2 quad[2] = {x[2 * e], x[2 * e + 1]};
-        *reinterpret_cast<uint4 *>(to + col0 + i * apart + 4 * e) = narrowPairs<kF32>(quad);
+        *reinterpret_cast<uint4 *>(to + ((i * (P / 2) + e) * team.lanes + team.lane) * 4) = narrowPairs<kF32>(quad);
       }
     }
   };
@@ -94,7 +96,7 @@ __global__ void __launch_bounds__(PASS == kPre ? 1024 : 512, 1) blockNormForward
 #pragma unroll
     for (int e = 0; e < P / 2; ++e) {
       F2 quad[2];
-      widenPairs<kF32>(*reinterpret_cast<const uint4 *>(from + col0 + i * apart + 4 * e), quad);
+      widenPairs<kF32>(*reinterpret_cast<const uint4 *>(from + ((i * (P / 2) + e) * team.lanes + team.lane) * 4), quad);
       v[2 * e] = quad[0];
       v[2 * e + 1] = quad[1];
     }

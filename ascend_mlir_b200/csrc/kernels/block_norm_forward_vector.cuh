@@ -32,15 +32,15 @@ __device__ __forceinline__ void pairStatistics(Team &team, const F2 (&v)[NV][kPa
 #pragma unroll
       for (int e = 0; e < P; ++e) sum = sum + v[i][e];
     const float s = warpSum(sumOf(sum));
-    auto columnsOf = [&](int warp) {  // of the row, in this warp's lanes
-      if (full) return static_cast<float>(NV * 32 * VEC);
+    float mine = static_cast<float>(NV * 32 * VEC);  // of the row, in this warp's lanes
+    if (!full) {
       int n = 0;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) n += max(0, min(32 * VEC, cols - (i * team.lanes + warp * 32) * VEC));
-      return static_cast<float>(n);
-    };
-    const float mine = columnsOf(team.lane >> 5);
-    const float centre = __fdividef(s, fmaxf(mine, 1.0f));  // any centre near the mean will do
+      for (int i = 0; i < NV; ++i) n += max(0, min(32 * VEC, cols - (i * team.lanes + (team.lane & ~31)) * VEC));
+      mine = static_cast<float>(n);
+    }
+    constexpr float kWhole = 1.0f / (NV * 32 * VEC);  // a power of two
+    const float centre = full ? s * kWhole : __fdividef(s, fmaxf(mine, 1.0f));  // any centre near the mean will do
     const F2 shift = splat(-centre);
     F2 q = splat(0.0f);
 #pragma unroll
@@ -54,27 +54,49 @@ __device__ __forceinline__ void pairStatistics(Team &team, const F2 (&v)[NV][kPa
     }
     float squares = warpSum(sumOf(q));
     if (team.lanes == 32) {
-      mean = centre;
+      mean = s * share;
+      squares = fmaf(mine * (centre - mean), centre - mean, squares);
     } else {
-      float *buf = team.scratch + team.half * 64;
+      float *buf = team.scratch + team.half * (kTeamValues * kTeamSlice);
       team.half ^= 1;
-      const int lane = threadIdx.x & 31, warps = team.lanes >> 5;
-      if (lane == 0) {
-        buf[team.lane >> 5] = s;
-        buf[32 + (team.lane >> 5)] = squares;
+      if ((threadIdx.x & 31) == 0) {
+        const int w = team.lane >> 5;
+        buf[w] = s;
+        buf[kTeamSlice + w] = squares;
+        if (!full) buf[2 * kTeamSlice + w] = mine;
       }
-      asm volatile("bar.sync %0, %1;" ::"r"(team.index + 1), "r"(team.lanes) : "memory");
-      const float n = lane < warps ? columnsOf(lane) : 0.0f;
-      const float sw = lane < warps ? buf[lane] : 0.0f, qw = lane < warps ? buf[32 + lane] : 0.0f;
-      float total = sw;
+      teamBarrier(team);
+      float total = 0.0f;
+      eachFourWarps(team, [&](int w) {
+        const float4 f = *reinterpret_cast<const float4 *>(buf + w);
+        total += (f.x + f.y) + (f.z + f.w);
+      });
+      mean = total * share;
+      squares = 0.0f;
+      if (full) {
+        float apart = 0.0f;  // what the warps' means differ by
+        eachFourWarps(team, [&](int w) {
+          const float4 f = *reinterpret_cast<const float4 *>(buf + w), g = *reinterpret_cast<const float4 *>(buf + kTeamSlice + w);
+          const float sums[4] = {f.x, f.y, f.z, f.w};
+          squares += (g.x + g.y) + (g.z + g.w);
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-      mean = __shfl_sync(0xffffffffu, total, 0) * share;
-      const float off = __fdividef(sw, fmaxf(n, 1.0f)) - mean;  // the same quotient as the warp's centre
-      squares = n > 0.0f ? fmaf(n * off, off, qw) : 0.0f;
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
-      squares = __shfl_sync(0xffffffffu, squares, 0);
+          for (int j = 0; j < 4; ++j) {
+            const float off = w + j < (team.lanes >> 5) ? fmaf(sums[j], kWhole, -mean) : 0.0f;
+            apart = fmaf(off, off, apart);
+          }
+        });
+        squares = fmaf(apart, static_cast<float>(NV * 32 * VEC), squares);
+      } else {
+        eachFourWarps(team, [&](int w) {
+          const float4 f = *reinterpret_cast<const float4 *>(buf + w), g = *reinterpret_cast<const float4 *>(buf + kTeamSlice + w),
+                       n = *reinterpret_cast<const float4 *>(buf + 2 * kTeamSlice + w);
+          auto join = [&](float sum, float square, float count) {  // the same quotient as the warp's centre
+            const float off = __fdividef(sum, fmaxf(count, 1.0f)) - mean;
+            return fmaf(count * off, off, square);
+          };
+          squares += (join(f.x, g.x, n.x) + join(f.y, g.y, n.y)) + (join(f.z, g.z, n.z) + join(f.w, g.w, n.w));
+        });
+      }
     }
     rstd = rsqrtf(squares * share + eps);
   }

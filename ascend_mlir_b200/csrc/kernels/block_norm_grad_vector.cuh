@@ -40,14 +40,14 @@ struct RowCursor {
 
 // TOKEN: a gate value per element (kGateToken); FULL: every thread's vectors lie inside the row.
 template <int ELEM, int KIND, int PASS, bool TOKEN, bool FULL, int NV>
-__global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_constant__ BlockNormGradLaunch p, const __grid_constant__ GradPlan plan,
+__global__ void __launch_bounds__(kGradAheadThreads) blockNormGradVectorKernel(const __grid_constant__ BlockNormGradLaunch p, const __grid_constant__ GradPlan plan,
                                                                  int teamLanes, int stages) {
   gridDependencyPrologue();
   constexpr bool kLayer = KIND == kLayerNorm;
   constexpr int kValues = kLayer ? 2 : 1;
   constexpr bool kPostPart = PASS != kPre, kPrePart = PASS != kPost, kToken = TOKEN;
   constexpr int VEC = ElemOf<ELEM>::kVec, P = kPairs<ELEM>, EB = 16 / VEC;
-  extern __shared__ uint4 slots[];  // [stages][tensors][NV][threads]
+  extern __shared__ uint4 slots[];  // [stages][tensors][NV][kGradAheadThreads], then parameters
   __shared__ float scratch[kTeamScratchFloats];
   Team team = makeTeam(teamLanes, scratch);
   const int cols = static_cast<int>(p.cols);
@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
   // Slots by byte: tensors present get one each, in this order.
   const bool grouped = !kToken && p.gateForm == kGateGroup;
   const bool packed = p.checkpoint.codes != nullptr, hasDout = p.dout.base != nullptr;
-  const unsigned int perTensor = NV * blockDim.x * 16, perVector = blockDim.x * 16;
+  constexpr unsigned int perVector = kGradAheadThreads * 16, perTensor = NV * perVector;
   unsigned int used = 0;
   const unsigned int atDh = used;
   if (kPrePart) used += perTensor;
@@ -84,8 +84,9 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
   // where a token's gate needs it, normA's bias times it.  Each thread reads only what it has written itself (teams
   // write the same values), so nothing waits here.
   float *weightB = reinterpret_cast<float *>(reinterpret_cast<char *>(slots) + stages * used);
-  float *weightA = weightB + (kPrePart ? plan.sumsLd : 0), *biasA = weightA + (kPostPart ? plan.sumsLd : 0);
-  if (grouped) weightA += team.index * plan.sumsLd;  // each team its own: times the gate of the group it is in
+  const int paramLd = team.lanes * NV * VEC;  // 16-byte pieces in the order of the threads, free of bank conflicts
+  float *weightA = weightB + (kPrePart ? paramLd : 0), *biasA = weightA + (kPostPart ? paramLd : 0);
+  if (grouped) weightA += team.index * paramLd;  // each team its own: times the gate of the group it is in
   auto writeParams = [&](float *to, const void *v, const void *times, int gateRow = -1) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -106,7 +107,7 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
 #pragma unroll
       for (int e = 0; e < P / 2; ++e) {
         const F2 quad[2] = {x[2 * e], x[2 * e + 1]};
-        *reinterpret_cast<uint4 *>(to + col0 + i * apart + 4 * e) = narrowPairs<kF32>(quad);
+        *reinterpret_cast<uint4 *>(to + ((i * (P / 2) + e) * team.lanes + team.lane) * 4) = narrowPairs<kF32>(quad);
       }
     }
   };
@@ -114,7 +115,7 @@ __global__ void __launch_bounds__(512) blockNormGradVectorKernel(const __grid_co
 #pragma unroll
     for (int e = 0; e < P / 2; ++e) {
       F2 quad[2];
-      widenPairs<kF32>(*reinterpret_cast<const uint4 *>(from + col0 + i * apart + 4 * e), quad);
+      widenPairs<kF32>(*reinterpret_cast<const uint4 *>(from + ((i * (P / 2) + e) * team.lanes + team.lane) * 4), quad);
       v[2 * e] = quad[0];
       v[2 * e + 1] = quad[1];
     }

@@ -14,7 +14,7 @@ using ForwardKernel = void (*)(const BlockNormLaunch, int);
 using GradKernel = void (*)(const BlockNormGradLaunch, const GradPlan, int);
 template <int ELEM> ForwardKernel forwardKernel(int kind, int pass, bool vector, int nv);
 // Teams that stay, with rows fetched ahead (block_norm_forward_ahead.cuh).
-using ForwardAheadKernel = void (*)(const BlockNormLaunch, int, int, int);
+using ForwardAheadKernel = void (*)(const BlockNormLaunch, int, int);
 template <int ELEM> ForwardAheadKernel forwardAheadKernel(int kind, int pass, bool full, int nv);
 template <int ELEM> GradKernel gradKernel(int kind, int pass, bool vector, int nv);
 // With rows fetched ahead (block_norm_grad_vector.cuh); null where a thread would hold more than it has registers for.
