@@ -4,11 +4,15 @@
 // 16-bit type of dy, which is exact (four significant bits times a power of two), and go to the tensor cores from shared
 // memory.
 //
-//   warp 0      TMA producer: codes [64 tokens x TM] and dy [64 tokens x 256] into a ring of stages;
+//   warp 0      TMA producer of dy: [64 tokens x 256] per stage;
 //   warp 1      MMA issuer: tcgen05.mma.cta_group::1.kind::f16, 128 x 256 x 16, both operands with their long side
 //               contiguous (tokens are the summed dimension and the rows of both tensors);
-//   warps 2..9  convert a stage's codes into the A operand (a ring of two tiles, 128-byte swizzle), and write the
-//               finished tile out: tcgen05.ld, convert, 16-byte stores that cover whole 128-byte lines.
+//   warps 2..17 load codes straight into registers two stages ahead (a token's 128 columns are one line), convert them into
+//               the A operand (128-byte swizzle), and write the finished tile out: tcgen05.ld, convert, 16-byte
+//               stores that cover whole 128-byte lines.
+// What bounds it is shared memory: a stage of 256 x 256 x 64 takes 1024 cycles of the tensor cores, which read 96 KB of
+// operands (768 cycles) while dy comes in (256) and A is written (256).  Codes staged in shared memory as well cost another
+// 256 cycles and were measured slower.
 // TM = 128 * MB rows of dweight per CTA; MB = 2 halves what dy costs per flop.  One persistent CTA per SM.  Where the
 // tiles of dweight are fewer than the SMs the tokens are cut into slices whose partial tiles (f32) a second kernel adds in order.
 //
@@ -20,6 +24,7 @@
 #include "kernels/block_norm.h"
 #include "kernels/block_norm_device.cuh"
 #include "kernels/launch_util.h"
+#include "kernels/pairs.cuh"
 #include "kernels/tcgen05_device.cuh"
 
 namespace afir {
@@ -28,38 +33,46 @@ namespace {
 
 constexpr int kTileN = 256;
 constexpr int kTokens = 64;                      // summed per stage
-constexpr int kCodeBoxBytes = kTokens * 128;     // 64 tokens x 128 columns of codes
 constexpr int kBlockBytes = kTokens * 64 * 2;    // 64 tokens x 64 columns of a 16-bit operand
 constexpr int kBStage = 4 * kBlockBytes;
-constexpr int kConvertWarps = 8;
+constexpr int kConvertWarps = 16;
 constexpr int kThreads = 64 + 32 * kConvertWarps;
-constexpr int kATiles = 2;
 
 template <int MB> struct GradShape {
   static constexpr int kTileM = 128 * MB;
-  static constexpr int kCodeStage = MB * kCodeBoxBytes;
-  static constexpr int kStageBytes = kCodeStage + kBStage;
-  static constexpr int kStages = MB == 1 ? 4 : 3;
   static constexpr int kATileBytes = MB * 2 * kBlockBytes;
+  static constexpr int kBStages = 4, kATiles = MB == 1 ? 4 : 3;
   static constexpr int kTmemCols = MB * kTileN;
-  static constexpr size_t kRing = static_cast<size_t>(kStages) * kStageBytes;
+  static constexpr size_t kAAt = static_cast<size_t>(kBStages) * kBStage, kControlAt = kAAt + static_cast<size_t>(kATiles) * kATileBytes;
   static_assert(kATiles * kATileBytes >= kConvertWarps * 4096, "the A tiles double as the staging area of the output");
 };
 template <int MB> struct GradControl {
-  unsigned long long full[GradShape<MB>::kStages], empty[GradShape<MB>::kStages];
-  unsigned long long aFull[kATiles], aEmpty[kATiles];
+  using S = GradShape<MB>;
+  unsigned long long bFull[S::kBStages], bEmpty[S::kBStages], aFull[S::kATiles], aEmpty[S::kATiles];
   unsigned long long tileFull, tileEmpty;
   unsigned int tmemBase;
   AbortState abort;
 };
-template <int MB> constexpr size_t gradSmemBytes() { return 1024 + GradShape<MB>::kRing + kATiles * GradShape<MB>::kATileBytes + sizeof(GradControl<MB>); }
+template <int MB> constexpr size_t gradSmemBytes() { return 1024 + GradShape<MB>::kControlAt + sizeof(GradControl<MB>); }
+static_assert(gradSmemBytes<1>() <= 227 * 1024 && gradSmemBytes<2>() <= 227 * 1024, "shared memory of a CTA");
+
+// Place in a ring of N and the parity of its round.
+template <int N> struct Ring {
+  int at = 0;
+  unsigned int phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++at == N) {
+      at = 0;
+      phase ^= 1u;
+    }
+  }
+};
 
 struct GradParams {
   int D, N, T;
   int tilesM, tilesN, kBlocks, splits, kPerSplit, band;
-  const uint8_t *exps;
-  int64_t expsLd;
-  int expCols;
+  const uint8_t *codes, *exps;
+  int64_t codesLd, expsLd;
   void *out;       // dweight, or the partial tiles [splits][D][N] f32
   int64_t outLd;
   int64_t splitStride;
@@ -68,29 +81,39 @@ struct GradParams {
   unsigned int *status;
 };
 
-// 16 codes -> 16 values of the operand type, times the power.
-template <int ELEM> __device__ __forceinline__ void widenCodes(const uint4 &raw, int exponent, uint4 (&out)[2]) {
+// 16 codes -> 16 values of the operand type, times the power (2^k as f32 bits).
+template <int ELEM> __device__ __forceinline__ void widenCodes(const uint4 &raw, float power, uint4 (&out)[2]) {
   const unsigned int w[4] = {raw.x, raw.y, raw.z, raw.w};
   unsigned int r[8];
+  if constexpr (ELEM == kF16) {
+    // the power as f16: 2^-15 (a subnormal) to 2^8, exact, and so is the product
+    const __half2 scale = __float2half2_rn(power);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const unsigned int pair = (w[i >> 1] >> ((i & 1) * 16)) & 0xffffu;
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(pair), __NV_E4M3);
-    const __half2 v = *reinterpret_cast<const __half2 *>(&h);
-    if constexpr (ELEM == kF16) {
-      // the power as f16: 2^-15 (a subnormal) to 2^8, exact, and so is the product
-      const __half p = __float2half_rn(powerOfExponent(exponent));
-      const __half2 m = __hmul2(v, __halves2half2(p, p));
+    for (int i = 0; i < 8; ++i) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>((w[i >> 1] >> ((i & 1) * 16)) & 0xffffu), __NV_E4M3);
+      const __half2 m = __hmul2(*reinterpret_cast<const __half2 *>(&h), scale);
       r[i] = *reinterpret_cast<const unsigned int *>(&m);
-    } else {
-      const float p = powerOfExponent(exponent);
-      const float2 f = __half22float2(v);
-      const __nv_bfloat162 m = __floats2bfloat162_rn(f.x * p, f.y * p);
-      r[i] = *reinterpret_cast<const unsigned int *>(&m);
+    }
+  } else {
+    const F2 scale = splat(power);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>((w[i >> 1] >> ((i & 1) * 16)) & 0xffffu), __NV_E4M3);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+      const float2 m = valuesOf(pairOf(f.x, f.y) * scale);
+      const __nv_bfloat162 b = __floats2bfloat162_rn(m.x, m.y);
+      r[i] = *reinterpret_cast<const unsigned int *>(&b);
     }
   }
   out[0] = make_uint4(r[0], r[1], r[2], r[3]);
   out[1] = make_uint4(r[4], r[5], r[6], r[7]);
+}
+
+// 16 bytes that nobody in this SM reads again soon.
+__device__ __forceinline__ uint4 loadOnce16(const uint8_t *p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
 }
 
 __device__ __forceinline__ uint4 addF32(const uint4 &a, const uint4 &b) {
@@ -100,21 +123,21 @@ __device__ __forceinline__ uint4 addF32(const uint4 &a, const uint4 &b) {
 
 template <int ELEM, int OUT, int MB>
 __global__ void __launch_bounds__(kThreads, 1)
-checkpointGradKernel(const __grid_constant__ CUtensorMap mapCodes, const __grid_constant__ CUtensorMap mapDy, const __grid_constant__ GradParams prm) {
+checkpointGradKernel(const __grid_constant__ CUtensorMap mapDy, const __grid_constant__ GradParams prm) {
   using S = GradShape<MB>;
-  constexpr int STAGES = S::kStages;
+  constexpr int kBStages = S::kBStages, kATiles = S::kATiles;
   extern __shared__ unsigned char smemRaw[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smemRaw) + 1023) & ~uintptr_t(1023));
-  unsigned char *aTiles = smem + S::kRing;
-  GradControl<MB> *ctl = reinterpret_cast<GradControl<MB> *>(aTiles + kATiles * S::kATileBytes);
+  unsigned char *aTiles = smem + S::kAAt;
+  GradControl<MB> *ctl = reinterpret_cast<GradControl<MB> *>(smem + S::kControlAt);
   volatile AbortState *abortFlag = &ctl->abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles = prm.tilesM * prm.tilesN, units = tiles * prm.splits;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbarInit(smemAddr(&ctl->full[s]), 1);
-      mbarInit(smemAddr(&ctl->empty[s]), 1);
+    for (int s = 0; s < kBStages; ++s) {
+      mbarInit(smemAddr(&ctl->bFull[s]), 1);
+      mbarInit(smemAddr(&ctl->bEmpty[s]), 1);
     }
     for (int a = 0; a < kATiles; ++a) {
       mbarInit(smemAddr(&ctl->aFull[a]), kConvertWarps);
@@ -126,7 +149,6 @@ checkpointGradKernel(const __grid_constant__ CUtensorMap mapCodes, const __grid_
     ctl->abort.status = prm.status;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    prefetchTensorMap(&mapCodes);
     prefetchTensorMap(&mapDy);
   }
   if (warp == 1) {
@@ -153,49 +175,47 @@ checkpointGradKernel(const __grid_constant__ CUtensorMap mapCodes, const __grid_
 
   if (warp == 0) {
     if (lane == 0) {
-      unsigned int it = 0;
+      Ring<kBStages> ring;
       bool ok = true;
       for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
         int tm, tn, k0, k1, split;
         unitCoords(u, tm, tn, k0, k1, split);
-        for (int kb = k0; kb < k1; ++kb, ++it) {
-          const int s = it % STAGES;
-          if (!mbarWait(smemAddr(&ctl->empty[s]), ((it / STAGES) & 1u) ^ 1u, abortFlag, 0)) { ok = false; break; }
-          const unsigned int full = smemAddr(&ctl->full[s]);
-          mbarExpectTx(full, S::kStageBytes);
-          unsigned char *stage = smem + static_cast<size_t>(s) * S::kStageBytes;
+        for (int kb = k0; kb < k1; ++kb, ring.next()) {
+          if (!mbarWait(smemAddr(&ctl->bEmpty[ring.at]), ring.phase ^ 1u, abortFlag, 0)) { ok = false; break; }
+          const unsigned int full = smemAddr(&ctl->bFull[ring.at]), to = smemAddr(smem + static_cast<size_t>(ring.at) * kBStage);
+          mbarExpectTx(full, kBStage);
 #pragma unroll
-          for (int h = 0; h < MB; ++h) tmaLoad2d(smemAddr(stage + h * kCodeBoxBytes), &mapCodes, tm * S::kTileM + h * 128, kb * kTokens, full);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) tmaLoad2d(smemAddr(stage + S::kCodeStage + j * kBlockBytes), &mapDy, tn * kTileN + j * 64, kb * kTokens, full);
+          for (int j = 0; j < 4; ++j) tmaLoad2d(to + j * kBlockBytes, &mapDy, tn * kTileN + j * 64, kb * kTokens, full);
         }
       }
       if (!ok) {
         // loads already issued still land in this CTA's shared memory: give them time before leaving
-        for (int s = 0; s < STAGES; ++s) {
+        for (int s = 0; s < kBStages; ++s) {
           const unsigned long long t0 = globalTimerNs();
-          while (!mbarTryWait(smemAddr(&ctl->full[s]), 0) && !mbarTryWait(smemAddr(&ctl->full[s]), 1) && globalTimerNs() - t0 < 1000000ull) {
+          while (!mbarTryWait(smemAddr(&ctl->bFull[s]), 0) && !mbarTryWait(smemAddr(&ctl->bFull[s]), 1) && globalTimerNs() - t0 < 1000000ull) {
           }
         }
       }
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      unsigned int it = 0, unit = 0;
+      unsigned int unit = 0;
+      Ring<kBStages> bRing;
+      Ring<kATiles> aRing;
       bool ok = true;
       for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++unit) {
         int tm, tn, k0, k1, split;
         unitCoords(u, tm, tn, k0, k1, split);
         if (!mbarWait(smemAddr(&ctl->tileEmpty), (unit & 1u) ^ 1u, abortFlag, 1)) break;
         tcgen05FenceAfter();
-        for (int kb = k0; kb < k1; ++kb, ++it) {
-          const int s = it % STAGES, a = it % kATiles;
+        for (int kb = k0; kb < k1; ++kb, bRing.next(), aRing.next()) {
+          const int s = bRing.at, a = aRing.at;
           // dy's copy and the converted codes: each is waited for where it becomes visible to the tensor cores
-          if (!mbarWait(smemAddr(&ctl->full[s]), (it / STAGES) & 1u, abortFlag, 1) ||
-              !mbarWait(smemAddr(&ctl->aFull[a]), (it / kATiles) & 1u, abortFlag, 1)) { ok = false; break; }
+          if (!mbarWait(smemAddr(&ctl->bFull[s]), bRing.phase, abortFlag, 1) ||
+              !mbarWait(smemAddr(&ctl->aFull[a]), aRing.phase, abortFlag, 1)) { ok = false; break; }
           tcgen05FenceAfter();
           const unsigned int aBase = smemAddr(aTiles + a * S::kATileBytes);
-          const unsigned int bBase = smemAddr(smem + static_cast<size_t>(s) * S::kStageBytes + S::kCodeStage);
+          const unsigned int bBase = smemAddr(smem + static_cast<size_t>(s) * kBStage);
 #pragma unroll
           for (int h = 0; h < MB; ++h) {
             const unsigned int dTmem = tmemBase + static_cast<unsigned int>(h * kTileN);
@@ -207,7 +227,7 @@ checkpointGradKernel(const __grid_constant__ CUtensorMap mapCodes, const __grid_
               ummaF16(dTmem, aDesc, bDesc, prm.idesc, (kb > k0 || k > 0) ? 1u : 0u);
             }
           }
-          ummaCommit(smemAddr(&ctl->empty[s]));
+          ummaCommit(smemAddr(&ctl->bEmpty[s]));
           ummaCommit(smemAddr(&ctl->aEmpty[a]));
         }
         if (!ok) break;
@@ -221,60 +241,77 @@ checkpointGradKernel(const __grid_constant__ CUtensorMap mapCodes, const __grid_
     const int tokenBase = (MB == 2 ? cw >> 1 : cw) * (kSteps * 4) + (lane >> 3);
     const int piece = lane & 7;                                 // 16 columns of the 128
     const int quarter = warp & 3;
-    unsigned int it = 0, unit = 0;
+    // Eight lanes write one token's 128 columns, two 64-column blocks: those of the second block write their upper half
+    // first, so that the eight 16-byte pieces of each store fall on different banks.
+    const bool upperFirst = (piece >> 2) != 0;
+    int to[kSteps];
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+      const int token = tokenBase + j * 4;
+      to[j] = (half * 2 + (piece >> 2)) * kBlockBytes + token * 128 + ((((piece & 3) * 2 + (upperFirst ? 1 : 0)) ^ (token & 7)) << 4);
+    }
+    unsigned int unit = 0;
+    Ring<kATiles> aRing;
     bool ok = true;
     for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++unit) {
       int tm, tn, k0, k1, split;
       unitCoords(u, tm, tn, k0, k1, split);
-      const int expCol = tm * MB + half;
-      const bool expLive = expCol < prm.expCols;
-      int exps[kSteps];
-      auto loadExps = [&](int kb) {
+      // This thread's codes and their exponents, two stages ahead.  Beyond the last token or column: zeros.
+      const int col = tm * S::kTileM + half * 128 + piece * 16;
+      const bool colLive = col < prm.D;  // D is a multiple of 16: a piece is wholly inside or outside
+      const int64_t firstToken = static_cast<int64_t>(k0) * kTokens + tokenBase;
+      const uint8_t *codeRow = prm.codes + firstToken * prm.codesLd + col, *expRow = prm.exps + firstToken * prm.expsLd + tm * MB + half;
+      int tokensLeft = prm.T - static_cast<int>(firstToken);
+      struct Ahead { uint4 raw[kSteps]; unsigned int exps[kSteps]; };
+      auto load = [&](Ahead &a) {
 #pragma unroll
         for (int j = 0; j < kSteps; ++j) {
-          const int token = kb * kTokens + tokenBase + j * 4;
-          exps[j] = expLive && token < prm.T ? __ldg(prm.exps + static_cast<int64_t>(token) * prm.expsLd + expCol) : 127;  // codes beyond are 0
+          const bool some = colLive && j * 4 < tokensLeft;
+          a.raw[j] = make_uint4(0u, 0u, 0u, 0u);
+          a.exps[j] = 127u;
+          if (some) {
+            a.raw[j] = loadOnce16(codeRow + j * 4 * prm.codesLd);
+            a.exps[j] = __ldg(expRow + j * 4 * prm.expsLd);
+          }
         }
+        codeRow += kTokens * prm.codesLd;
+        expRow += kTokens * prm.expsLd;
+        tokensLeft -= kTokens;
       };
-      loadExps(k0);
-      for (int kb = k0; kb < k1; ++kb, ++it) {
-        const int s = it % STAGES, a = it % kATiles;
-        const bool ready = mbarWait(smemAddr(&ctl->full[s]), (it / STAGES) & 1u, abortFlag, 3) &&
-                           mbarWait(smemAddr(&ctl->aEmpty[a]), ((it / kATiles) & 1u) ^ 1u, abortFlag, 3);
-        if (!__all_sync(0xffffffffu, ready)) { ok = false; break; }
-        const unsigned char *codes = smem + static_cast<size_t>(s) * S::kStageBytes + half * kCodeBoxBytes;
-        unsigned char *block = aTiles + a * S::kATileBytes + (half * 2 + (piece >> 2)) * kBlockBytes;
-        uint4 raw[kSteps];
-#pragma unroll
-        for (int j = 0; j < kSteps; ++j) raw[j] = *reinterpret_cast<const uint4 *>(codes + (tokenBase + j * 4) * 128 + piece * 16);
+      Ahead now, next, after;
+      load(now);
+      load(next);
+      for (int kb = k0; kb < k1; ++kb, aRing.next()) {
+        load(after);
+        const int a = aRing.at;
+        if (!__all_sync(0xffffffffu, mbarWait(smemAddr(&ctl->aEmpty[a]), aRing.phase ^ 1u, abortFlag, 3))) { ok = false; break; }
+        unsigned char *tile = aTiles + a * S::kATileBytes;
 #pragma unroll
         for (int j = 0; j < kSteps; ++j) {
-          const int token = tokenBase + j * 4;
           uint4 v[2];
-          widenCodes<ELEM>(raw[j], exps[j], v);
-          // eight lanes write one token's 128 columns, two 64-column blocks: those of the second block write their upper
-          // half first, so that the eight 16-byte pieces of each store fall on different banks
-          const int first = piece >> 2, at = (piece & 3) * 2;
-          unsigned char *row = block + token * 128;
-          *reinterpret_cast<uint4 *>(row + (((at + first) ^ (token & 7)) << 4)) = first ? v[1] : v[0];
-          *reinterpret_cast<uint4 *>(row + (((at + 1 - first) ^ (token & 7)) << 4)) = first ? v[0] : v[1];
+          widenCodes<ELEM>(now.raw[j], powerOfExponent(static_cast<int>(now.exps[j])), v);
+          *reinterpret_cast<uint4 *>(tile + to[j]) = upperFirst ? v[1] : v[0];
+          *reinterpret_cast<uint4 *>(tile + (to[j] ^ 16)) = upperFirst ? v[0] : v[1];
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbarArrive(smemAddr(&ctl->aFull[a]));
-        if (kb + 1 < k1) loadExps(kb + 1);
+        now = next;
+        next = after;
       }
       if (!ok) break;
 
-      // ---- the finished tile: warps 0..3 of the eight take the lower half (of its rows for MB = 2, of its columns for
-      // MB = 1), 4..7 the upper; the A tiles are free (every MMA has completed) and serve as staging
+      // ---- the finished tile: four warps share the tensor memory's lanes; for MB = 2 half of the fours take each accumulator
+      // and share its columns, for MB = 1 all share the columns.  The A tiles are free (every MMA has completed) and serve as
+      // staging.
       if (!__all_sync(0xffffffffu, mbarWait(smemAddr(&ctl->tileFull), unit & 1u, abortFlag, 2))) break;
       tcgen05FenceAfter();
       unsigned char *stg = aTiles + cw * 4096;
-      const int upper = cw >> 2;
-      const int rowBase = tm * S::kTileM + (MB == 2 ? upper * 128 : 0) + quarter * 32;
-      const int colBegin = MB == 2 ? 0 : upper * 128, colEnd = MB == 2 ? kTileN : colBegin + 128;
-      const unsigned int taddr = tmemBase + static_cast<unsigned int>(MB == 2 ? upper * kTileN : 0) + (static_cast<unsigned int>(quarter * 32) << 16);
+      const int share = cw >> 2;
+      constexpr int kPerTile = kConvertWarps / 4 / MB, kCols = kTileN / kPerTile;
+      const int rowBase = tm * S::kTileM + share / kPerTile * 128 + quarter * 32;
+      const int colBegin = share % kPerTile * kCols, colEnd = colBegin + kCols;
+      const unsigned int taddr = tmemBase + static_cast<unsigned int>(share / kPerTile * kTileN) + (static_cast<unsigned int>(quarter * 32) << 16);
       constexpr int kColsPerSlice = 128 / OutPack<OUT>::kBytes;
       unsigned char *out = static_cast<unsigned char *>(prm.out) + static_cast<size_t>(split) * prm.splitStride * OutPack<OUT>::kBytes;
 #pragma unroll 1
@@ -385,19 +422,19 @@ void gradFail(char *errorText, const char *msg) {
 }
 
 template <int ELEM, int OUT, int MB>
-int launchGradVariant(const CUtensorMap &codes, const CUtensorMap &dy, const GradParams &p, int grid, cudaStream_t stream) {
+int launchGradVariant(const CUtensorMap &dy, const GradParams &p, int grid, cudaStream_t stream) {
   auto kernel = checkpointGradKernel<ELEM, OUT, MB>;
   static PerDeviceOnce reserved;
   const cudaError_t e = reserved.run([&] {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(gradSmemBytes<MB>()));
   });
   if (e != cudaSuccess) return e;
-  return launchOrdinary(kernel, dim3(static_cast<unsigned int>(grid)), dim3(kThreads), gradSmemBytes<MB>(), stream, codes, dy, p);
+  return launchOrdinary(kernel, dim3(static_cast<unsigned int>(grid)), dim3(kThreads), gradSmemBytes<MB>(), stream, dy, p);
 }
-template <int ELEM> int launchGradTyped(int out, int mb, const CUtensorMap &codes, const CUtensorMap &dy, const GradParams &p, int grid, cudaStream_t stream) {
+template <int ELEM> int launchGradTyped(int out, int mb, const CUtensorMap &dy, const GradParams &p, int grid, cudaStream_t stream) {
   if (out == kF32)
-    return mb == 2 ? launchGradVariant<ELEM, kF32, 2>(codes, dy, p, grid, stream) : launchGradVariant<ELEM, kF32, 1>(codes, dy, p, grid, stream);
-  return mb == 2 ? launchGradVariant<ELEM, ELEM, 2>(codes, dy, p, grid, stream) : launchGradVariant<ELEM, ELEM, 1>(codes, dy, p, grid, stream);
+    return mb == 2 ? launchGradVariant<ELEM, kF32, 2>(dy, p, grid, stream) : launchGradVariant<ELEM, kF32, 1>(dy, p, grid, stream);
+  return mb == 2 ? launchGradVariant<ELEM, ELEM, 2>(dy, p, grid, stream) : launchGradVariant<ELEM, ELEM, 1>(dy, p, grid, stream);
 }
 
 } // namespace
@@ -434,11 +471,9 @@ int launchCheckpointGrad(const CheckpointGradLaunch &l, cudaStream_t stream, int
   const size_t need = checkpointGradWorkspaceBytes(l.cols, l.outCols, l.rows, sms);
   if (need && (!l.workspace || l.workspaceBytes < need)) { gradFail(errorText, "checkpoint gradient: workspace too small"); return 1; }
 
-  CUtensorMap mapCodes, mapDy;
+  CUtensorMap mapDy;
   const CUtensorMapDataType dt = l.elemType == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  if (!makeMap2d(&mapCodes, CU_TENSOR_MAP_DATA_TYPE_UINT8, l.in.codes, static_cast<uint64_t>(l.cols), static_cast<uint64_t>(l.rows),
-                 static_cast<uint64_t>(l.in.codesLd), 128, kTokens, CU_TENSOR_MAP_SWIZZLE_NONE) ||
-      !makeMap2d(&mapDy, dt, l.dy.base, static_cast<uint64_t>(l.outCols), static_cast<uint64_t>(l.rows), static_cast<uint64_t>(l.dy.ld) * 2, 64, kTokens)) {
+  if (!makeMap2d(&mapDy, dt, l.dy.base, static_cast<uint64_t>(l.outCols), static_cast<uint64_t>(l.rows), static_cast<uint64_t>(l.dy.ld) * 2, 64, kTokens)) {
     gradFail(errorText, "checkpoint gradient: cuTensorMapEncodeTiled failed (driver entry point missing or bad operand layout)");
     return 1;
   }
@@ -452,9 +487,10 @@ int launchCheckpointGrad(const CheckpointGradLaunch &l, cudaStream_t stream, int
   p.splits = plan.splits;
   p.kPerSplit = plan.kPerSplit;
   p.band = 16;
+  p.codes = l.in.codes;
+  p.codesLd = l.in.codesLd;
   p.exps = l.in.exps;
   p.expsLd = l.in.expsLd;
-  p.expCols = static_cast<int>((l.cols + kCheckpointBlock - 1) / kCheckpointBlock);
   p.status = l.status;
   const bool joined = plan.splits > 1;
   p.out = joined ? l.workspace : l.out.base;
@@ -466,8 +502,8 @@ int launchCheckpointGrad(const CheckpointGradLaunch &l, cudaStream_t stream, int
   p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (1u << 16) | ((kTileN >> 3) << 17) | ((128u >> 4) << 24);
   const int grid = std::min(sms, plan.tilesM * plan.tilesN * plan.splits);
   const int out = joined ? static_cast<int>(kF32) : l.outType;
-  int rc = l.elemType == kF16 ? launchGradTyped<kF16>(out, plan.mb, mapCodes, mapDy, p, grid, stream)
-                              : launchGradTyped<kBF16>(out, plan.mb, mapCodes, mapDy, p, grid, stream);
+  int rc = l.elemType == kF16 ? launchGradTyped<kF16>(out, plan.mb, mapDy, p, grid, stream)
+                              : launchGradTyped<kBF16>(out, plan.mb, mapDy, p, grid, stream);
   if (rc != 0) return rc;
   if (launched) *launched += 1;
   if (joined) {
