@@ -294,10 +294,9 @@ bool CudaExecutor::prepareGenerated(CachedKernel &kernel) {
 
 Status CudaExecutor::dispatch(CachedKernel &kernel, const std::map<std::string, int64_t> &tiling, const LaunchArgs &args, LaunchInfo &info) {
   const LaunchDescriptor &d = *kernel.desc;
-  const int mode = codegenMode();
   const bool classHasCode = d.kernelClass == KernelClass::Elementwise || d.kernelClass == KernelClass::RowReduce ||
                             d.kernelClass == KernelClass::Gather;
-  if (mode != 0 && classHasCode && !(kernel.generatedTried && !kernel.generatedUsable) &&
+  if (classHasCode && codegenMode() != 0 && !(kernel.generatedTried && !kernel.generatedUsable) &&
       generatedLaunchApplies(d, tiling, args) &&
       prepareGenerated(kernel)) {
     Status s = launchGenerated(d, tiling, args, kernel.binding, info);
@@ -580,7 +579,8 @@ Status CudaExecutor::launchDevice(const RunRequest &req, void *workspace, size_t
     args.workspace = workspace_.ptr;
     args.workspaceBytes = workspace_.capacity;
   }
-  if (launchTraceEnabled()) printLaunchTrace(req, *desc, args, device_, "device");
+  const bool trace = launchTraceEnabled();  // the environment is read once per launch
+  if (trace) printLaunchTrace(req, *desc, args, device_, "device");
   LaunchInfo info;
   // The status words (bad gather indices, a staged reduction's time-out) accumulate over the launches queued since
   // the last synchronize: they are cleared only when nothing unread is pending on this workspace.
@@ -597,8 +597,8 @@ Status CudaExecutor::launchDevice(const RunRequest &req, void *workspace, size_t
   lastLaunchGenerated_ = info.generated;
   totalLaunchCount_ += static_cast<uint64_t>(info.kernelsLaunched);
   if (!ls) return launchStage(ls);
-  if (launchTraceEnabled() && !info.plan.empty()) std::fprintf(stderr, "[cuda-launch] matmul plan: %s\n", info.plan.c_str());
-  if (launchTraceEnabled()) std::fprintf(stderr, "[cuda-launch] code=%s kernels=%d\n", info.generated ? "generated" : "library", info.kernelsLaunched);
+  if (trace && !info.plan.empty()) std::fprintf(stderr, "[cuda-launch] matmul plan: %s\n", info.plan.c_str());
+  if (trace) std::fprintf(stderr, "[cuda-launch] code=%s kernels=%d\n", info.generated ? "generated" : "library", info.kernelsLaunched);
   statusPending_ = statusPending_ || info.usesStatusBlock;
   if (info.usesStatusBlock) statusWorkspace_ = args.workspace;
   matmulPending_ = desc->kernelClass == KernelClass::Matmul;
