@@ -25,6 +25,8 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC,-fvisibility=hidden", "-I", str(CSRC), "-I", str(ROOT / "include"),
 ]
+# Many instantiations of one kernel: their device code is kept compressed in the library.
+COMPRESS = ["-Xfatbin", "-compress-all"]
 # Bandwidth-bound kernels must round after every op: no mul+add contraction.
 NO_FMA = ["-fmad=false"]
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-Wextra", "-I", str(CSRC),
@@ -37,24 +39,24 @@ CU_SOURCES = {
     "kernels/transpose.cu": [],
     "kernels/transpose_tma.cu": [],
     "kernels/matmul_tcgen05.cu": [],
-    "kernels/block_norm.cu": [],
-    "kernels/block_norm_forward_f32.cu": [],
-    "kernels/block_norm_forward_f16.cu": [],
-    "kernels/block_norm_forward_bf16.cu": [],
-    "kernels/block_norm_grad_f32.cu": [],
-    "kernels/block_norm_grad_f16.cu": [],
-    "kernels/block_norm_grad_bf16.cu": [],
-    "kernels/block_norm_grad_ahead_rms_f32.cu": [],
-    "kernels/block_norm_grad_ahead_layer_f32.cu": [],
-    "kernels/block_norm_grad_ahead_rms_f16.cu": [],
-    "kernels/block_norm_grad_ahead_layer_f16.cu": [],
-    "kernels/block_norm_grad_ahead_rms_bf16.cu": [],
-    "kernels/block_norm_grad_ahead_layer_bf16.cu": [],
-    "kernels/block_norm_forward_ahead_f32.cu": [],
-    "kernels/block_norm_forward_ahead_f16.cu": [],
-    "kernels/block_norm_forward_ahead_bf16.cu": [],
-    "kernels/checkpoint.cu": [],
-    "kernels/checkpoint_grad_tcgen05.cu": [],
+    "kernels/block_norm.cu": COMPRESS,
+    "kernels/block_norm_forward_f32.cu": COMPRESS,
+    "kernels/block_norm_forward_f16.cu": COMPRESS,
+    "kernels/block_norm_forward_bf16.cu": COMPRESS,
+    "kernels/block_norm_grad_f32.cu": COMPRESS,
+    "kernels/block_norm_grad_f16.cu": COMPRESS,
+    "kernels/block_norm_grad_bf16.cu": COMPRESS,
+    "kernels/block_norm_grad_ahead_rms_f32.cu": COMPRESS,
+    "kernels/block_norm_grad_ahead_layer_f32.cu": COMPRESS,
+    "kernels/block_norm_grad_ahead_rms_f16.cu": COMPRESS,
+    "kernels/block_norm_grad_ahead_layer_f16.cu": COMPRESS,
+    "kernels/block_norm_grad_ahead_rms_bf16.cu": COMPRESS,
+    "kernels/block_norm_grad_ahead_layer_bf16.cu": COMPRESS,
+    "kernels/block_norm_forward_ahead_f32.cu": COMPRESS,
+    "kernels/block_norm_forward_ahead_f16.cu": COMPRESS,
+    "kernels/block_norm_forward_ahead_bf16.cu": COMPRESS,
+    "kernels/checkpoint.cu": COMPRESS,
+    "kernels/checkpoint_grad_tcgen05.cu": COMPRESS,
 }
 CPP_SOURCES = ["common/json.cpp", "kernels/matmul_plan.cpp", "kernels/body_match.cpp", "codegen/kernel_source.cpp",
                "codegen/nvrtc_compile.cpp", "codegen/embedded_headers.cpp", "runtime/device_module.cpp", "runtime/caller_device.cpp", "runtime/host_staging.cpp", "runtime/descriptor.cpp", "runtime/launcher.cpp", "runtime/executor.cpp",

@@ -341,12 +341,11 @@ int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *
     vector = vector && rowsAligned(l.checkpoint.codes, l.checkpoint.codesLd, 1, vec);
     TeamShape s = gradShape(l.elemType, l.kind, l.cols, vector);
     if (vector) s.teamsPerCta = std::max(1, std::min(15, kGradAheadThreads / s.lanes));
-    // rows fetched ahead: as many (2 to 4) as the CTAs of an SM have shared memory for beside their parameters; rows too
-    // wide for two take the kernel without
+    // rows fetched ahead: as many (2 to 4) as a CTA has shared memory for beside its parameters; rows too wide for two take
+    // the kernel without
     const int tensors = (l.pass != kPost ? 2 : 0) + (l.dout.base ? 1 : 0) + (l.pass != kPre ? 1 : 0) + (l.gateForm == kGateToken ? 1 : 0);
     const int vectors = (l.pass != kPost ? 1 : 0) + (l.pass != kPre ? 1 : 0) + (l.gateForm == kGateToken && l.kind == kLayerNorm ? 1 : 0);
-    const int perTeam = l.gateForm == kGateGroup && l.pass != kPre ? s.teamsPerCta - 1 : 0;  // a team's group has its own gate
-    const size_t paramBytes = static_cast<size_t>(vectors + perTeam) * static_cast<size_t>(s.lanes * s.nv * vec) * sizeof(float);
+    const size_t paramBytes = static_cast<size_t>(vectors) * static_cast<size_t>(s.nv * vec) * kGradAheadThreads * sizeof(float);
     const size_t rowBytes = static_cast<size_t>(tensors) * static_cast<size_t>(s.nv) * 16 * kGradAheadThreads;
     const size_t perCta = kAheadBytes - 1536;
     const int stages = static_cast<int>(std::min<size_t>(4, std::max<size_t>(2, (perCta - std::min(perCta, paramBytes)) / rowBytes)));

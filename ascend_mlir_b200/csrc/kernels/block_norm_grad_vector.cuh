@@ -80,13 +80,11 @@ __global__ void __launch_bounds__(kGradAheadThreads) blockNormGradVectorKernel(c
   const unsigned int slotsAt = static_cast<unsigned int>(__cvta_generic_to_shared(slots));
   auto readSlot = [&](unsigned int at) { return *reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(slots) + at); };
 
-  // Parameters as f32 behind the slots, for all teams of the CTA: normB's weight, normA's weight times the residual scale and,
-  // where a token's gate needs it, normA's bias times it.  Each thread reads only what it has written itself (teams
-  // write the same values), so nothing waits here.
-  float *weightB = reinterpret_cast<float *>(reinterpret_cast<char *>(slots) + stages * used);
-  const int paramLd = team.lanes * NV * VEC;  // 16-byte pieces in the order of the threads, free of bank conflicts
-  float *weightA = weightB + (kPrePart ? paramLd : 0), *biasA = weightA + (kPostPart ? paramLd : 0);
-  if (grouped) weightA += team.index * paramLd;  // each team its own: times the gate of the group it is in
+  // Parameters as f32 behind the slots, each thread's own: normB's weight, normA's weight times the residual scale (and the
+  // gate of the group that the team is in), and, where a token's gate needs it, normA's bias times the scale.
+  constexpr unsigned int kParamFloats = NV * VEC * kGradAheadThreads;
+  float *weightB = reinterpret_cast<float *>(reinterpret_cast<char *>(slots) + stages * used) + threadIdx.x * 4;
+  float *weightA = weightB + (kPrePart ? kParamFloats : 0), *biasA = weightA + (kPostPart ? kParamFloats : 0);
   auto writeParams = [&](float *to, const void *v, const void *times, int gateRow = -1) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -107,7 +105,7 @@ __global__ void __launch_bounds__(kGradAheadThreads) blockNormGradVectorKernel(c
 #pragma unroll
       for (int e = 0; e < P / 2; ++e) {
         const F2 quad[2] = {x[2 * e], x[2 * e + 1]};
-        *reinterpret_cast<uint4 *>(to + ((i * (P / 2) + e) * team.lanes + team.lane) * 4) = narrowPairs<kF32>(quad);
+        *reinterpret_cast<uint4 *>(to + (i * (P / 2) + e) * (kGradAheadThreads * 4)) = narrowPairs<kF32>(quad);
       }
     }
   };
@@ -115,7 +113,7 @@ __global__ void __launch_bounds__(kGradAheadThreads) blockNormGradVectorKernel(c
 #pragma unroll
     for (int e = 0; e < P / 2; ++e) {
       F2 quad[2];
-      widenPairs<kF32>(*reinterpret_cast<const uint4 *>(from + ((i * (P / 2) + e) * team.lanes + team.lane) * 4), quad);
+      widenPairs<kF32>(*reinterpret_cast<const uint4 *>(from + (i * (P / 2) + e) * (kGradAheadThreads * 4)), quad);
       v[2 * e] = quad[0];
       v[2 * e + 1] = quad[1];
     }
