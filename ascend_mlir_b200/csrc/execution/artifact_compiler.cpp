@@ -93,7 +93,7 @@ Status compileArtifact(const CompileRequest &request, KernelArtifact &artifact) 
     if (!os) return Status::error("cannot write " + binPath);
   }
   const std::string manifestPath = request.outputDir + "/manifest.txt";
-  const bool matmul = desc.kernelClass == KernelClass::Matmul;
+  const bool matmul = desc.kernelClass == KernelClass::Matmul || desc.kernelClass == KernelClass::CheckpointGrad;
   {
     std::ofstream os(manifestPath, std::ios::trunc);
     os << "kernel_name=" << desc.kernel << "\n"

@@ -323,7 +323,8 @@ int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *
   if (l.cols <= 0 || l.cols > kMaxNormCols || l.rows > kMaxNormRows) return cudaErrorInvalidValue;
   int device = 0;
   if (const cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return e;
-  GradPlan plan = gradPlan(l.elemType, l.kind, l.gateForm, l.rows, l.cols, l.groupRows, deviceSmCount(device));
+  const int sms = deviceSmCount(device);
+  GradPlan plan = gradPlan(l.elemType, l.kind, l.gateForm, l.rows, l.cols, l.groupRows, sms);
   const size_t need = static_cast<size_t>(sumsFloats(plan, l.pass, l.kind)) * sizeof(float);
   if (!l.workspace || l.workspaceBytes < need || !vectorAligned(l.workspace)) return cudaErrorInvalidValue;
   const int64_t values = l.kind == kLayerNorm ? 2 : 1;
@@ -340,7 +341,8 @@ int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *
     for (const void *v : {l.a.weight, l.a.bias, l.b.weight, l.scale}) vector = vector && vectorAligned(v);
     vector = vector && rowsAligned(l.checkpoint.codes, l.checkpoint.codesLd, 1, vec);
     TeamShape s = gradShape(l.elemType, l.kind, l.cols, vector);
-    if (vector) s.teamsPerCta = std::max(1, std::min(15, kGradAheadThreads / s.lanes));
+    // (few teams: spread over the SMs)
+    if (vector) s.teamsPerCta = std::max(1, std::min({15, kGradAheadThreads / s.lanes, (plan.teams + sms - 1) / sms}));
     // rows fetched ahead: as many (2 to 4) as a CTA has shared memory for beside its parameters; rows too wide for two take
     // the kernel without
     const int tensors = (l.pass != kPost ? 2 : 0) + (l.dout.base ? 1 : 0) + (l.pass != kPre ? 1 : 0) + (l.gateForm == kGateToken ? 1 : 0);

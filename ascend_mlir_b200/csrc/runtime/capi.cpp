@@ -8,6 +8,7 @@
 #include <cerrno>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <fstream>
 #include <iterator>
 #include <string>
@@ -75,6 +76,19 @@ RunRequest makeRequest(const uint8_t *binary, size_t binaryLen, const char *fn, 
   return r;
 }
 
+// An exception (a descriptor that asks for more memory than there is, say) becomes the call's error: none crosses the C
+// boundary.
+template <class F> int guarded(char *buf, size_t len, F call) {
+  try {
+    return call();
+  } catch (const std::exception &e) {
+    writeErr(buf, len, std::string("unexpected failure: ") + e.what());
+  } catch (...) {
+    writeErr(buf, len, "unexpected failure");
+  }
+  return 1;
+}
+
 } // namespace
 
 AFIR_EXPORT AfirtCompiler afirt_compiler_create(const char *soc_version, const char *arch, int opt_level) {
@@ -90,22 +104,24 @@ AFIR_EXPORT void afirt_compiler_destroy(AfirtCompiler compiler) { delete reinter
 
 AFIR_EXPORT int afirt_compiler_compile(AfirtCompiler compiler, const char *src_file, const char *output_dir,
                                        const char *kernel_name, char *out_bin_path, size_t buf_len) {
-  auto *h = reinterpret_cast<CompilerHandle *>(compiler);
-  if (!h) { writeErr(out_bin_path, buf_len, "compiler handle is null"); return 1; }
-  if (!src_file || !*src_file) { writeErr(out_bin_path, buf_len, "kernel source path is required"); return 1; }
-  if (!output_dir || !*output_dir) { writeErr(out_bin_path, buf_len, "output directory is required"); return 1; }
-  if (!kernel_name || !*kernel_name) { writeErr(out_bin_path, buf_len, "kernel name is required"); return 1; }
-  CompileRequest request;
-  request.kernelSource = src_file;
-  request.outputDir = output_dir;
-  request.kernelName = kernel_name;
-  request.socVersion = h->socVersion;
-  request.arch = h->arch;
-  KernelArtifact artifact;
-  if (Status s = compileArtifact(request, artifact); !s) { writeErr(out_bin_path, buf_len, s.message()); return 1; }
-  const std::string binPath = artifact.deviceBinaryPath;
-  writeErr(out_bin_path, buf_len, binPath);
-  return 0;
+  return guarded(out_bin_path, buf_len, [&]() -> int {
+    auto *h = reinterpret_cast<CompilerHandle *>(compiler);
+    if (!h) { writeErr(out_bin_path, buf_len, "compiler handle is null"); return 1; }
+    if (!src_file || !*src_file) { writeErr(out_bin_path, buf_len, "kernel source path is required"); return 1; }
+    if (!output_dir || !*output_dir) { writeErr(out_bin_path, buf_len, "output directory is required"); return 1; }
+    if (!kernel_name || !*kernel_name) { writeErr(out_bin_path, buf_len, "kernel name is required"); return 1; }
+    CompileRequest request;
+    request.kernelSource = src_file;
+    request.outputDir = output_dir;
+    request.kernelName = kernel_name;
+    request.socVersion = h->socVersion;
+    request.arch = h->arch;
+    KernelArtifact artifact;
+    if (Status s = compileArtifact(request, artifact); !s) { writeErr(out_bin_path, buf_len, s.message()); return 1; }
+    const std::string binPath = artifact.deviceBinaryPath;
+    writeErr(out_bin_path, buf_len, binPath);
+    return 0;
+  });
 }
 
 AFIR_EXPORT AfirtExecutor afirt_executor_create(void) {
@@ -129,14 +145,16 @@ AFIR_EXPORT int afirt_executor_run(AfirtExecutor executor, const uint8_t *binary
                                    const size_t *input_bytes, int num_outputs, void **output_ptrs,
                                    const size_t *output_bytes, const uint8_t *tiling_data, size_t tiling_len,
                                    int block_dim, uint32_t magic, char *err_buf, size_t err_len) {
-  auto *ex = reinterpret_cast<CudaExecutor *>(executor);
-  if (!ex || !ex->initialized()) { writeErr(err_buf, err_len, "executor has not been initialized"); return 1; }
-  if (!binary_data || binary_len == 0) { writeErr(err_buf, err_len, "binary data is required"); return 1; }
-  RunRequest r = makeRequest(binary_data, binary_len, function_name, num_inputs, input_ptrs, input_bytes, num_outputs,
-                             output_ptrs, output_bytes, tiling_data, tiling_len, block_dim, magic);
-  CallerDeviceScope keepCallerDevice;
-  if (Status s = ex->runHost(r); !s) { writeErr(err_buf, err_len, s.message()); return 1; }
-  return 0;
+  return guarded(err_buf, err_len, [&]() -> int {
+    auto *ex = reinterpret_cast<CudaExecutor *>(executor);
+    if (!ex || !ex->initialized()) { writeErr(err_buf, err_len, "executor has not been initialized"); return 1; }
+    if (!binary_data || binary_len == 0) { writeErr(err_buf, err_len, "binary data is required"); return 1; }
+    RunRequest r = makeRequest(binary_data, binary_len, function_name, num_inputs, input_ptrs, input_bytes, num_outputs,
+                               output_ptrs, output_bytes, tiling_data, tiling_len, block_dim, magic);
+    CallerDeviceScope keepCallerDevice;
+    if (Status s = ex->runHost(r); !s) { writeErr(err_buf, err_len, s.message()); return 1; }
+    return 0;
+  });
 }
 
 AFIR_EXPORT int afirt_executor_run_file(AfirtExecutor executor, const char *binary_path, const char *function_name,
@@ -144,14 +162,16 @@ AFIR_EXPORT int afirt_executor_run_file(AfirtExecutor executor, const char *bina
                                         int num_outputs, void **output_ptrs, const size_t *output_bytes,
                                         const uint8_t *tiling_data, size_t tiling_len, int block_dim, uint32_t magic,
                                         char *err_buf, size_t err_len) {
-  auto *ex = reinterpret_cast<CudaExecutor *>(executor);
-  if (!ex || !ex->initialized()) { writeErr(err_buf, err_len, "executor has not been initialized"); return 1; }
-  if (!binary_path || !*binary_path) { writeErr(err_buf, err_len, "binary path is required"); return 1; }
-  std::vector<uint8_t> bytes;
-  std::string err;
-  if (!readFile(binary_path, bytes, err)) { writeErr(err_buf, err_len, err); return 1; }
-  return afirt_executor_run(executor, bytes.data(), bytes.size(), function_name, num_inputs, input_ptrs, input_bytes,
-                            num_outputs, output_ptrs, output_bytes, tiling_data, tiling_len, block_dim, magic, err_buf, err_len);
+  return guarded(err_buf, err_len, [&]() -> int {
+    auto *ex = reinterpret_cast<CudaExecutor *>(executor);
+    if (!ex || !ex->initialized()) { writeErr(err_buf, err_len, "executor has not been initialized"); return 1; }
+    if (!binary_path || !*binary_path) { writeErr(err_buf, err_len, "binary path is required"); return 1; }
+    std::vector<uint8_t> bytes;
+    std::string err;
+    if (!readFile(binary_path, bytes, err)) { writeErr(err_buf, err_len, err); return 1; }
+    return afirt_executor_run(executor, bytes.data(), bytes.size(), function_name, num_inputs, input_ptrs, input_bytes,
+                              num_outputs, output_ptrs, output_bytes, tiling_data, tiling_len, block_dim, magic, err_buf, err_len);
+  });
 }
 
 AFIR_EXPORT int afirt_executor_launch_device(AfirtExecutor executor, const uint8_t *binary_data, size_t binary_len,
@@ -160,16 +180,18 @@ AFIR_EXPORT int afirt_executor_launch_device(AfirtExecutor executor, const uint8
                                              const size_t *output_bytes, const uint8_t *tiling_data, size_t tiling_len,
                                              int block_dim, uint32_t magic, void *workspace, size_t workspace_bytes,
                                              void *cuda_stream, char *err_buf, size_t err_len) {
-  auto *ex = reinterpret_cast<CudaExecutor *>(executor);
-  if (!ex || !ex->initialized()) { writeErr(err_buf, err_len, "executor has not been initialized"); return 1; }
-  RunRequest r = makeRequest(binary_data, binary_len, function_name, num_inputs, input_ptrs, input_bytes, num_outputs,
-                             output_ptrs, output_bytes, tiling_data, tiling_len, block_dim, magic);
-  CallerDeviceScope keepCallerDevice;
-  if (Status s = ex->launchDevice(r, workspace, workspace_bytes, cuda_stream); !s) {
-    writeErr(err_buf, err_len, s.message());
-    return 1;
-  }
-  return 0;
+  return guarded(err_buf, err_len, [&]() -> int {
+    auto *ex = reinterpret_cast<CudaExecutor *>(executor);
+    if (!ex || !ex->initialized()) { writeErr(err_buf, err_len, "executor has not been initialized"); return 1; }
+    RunRequest r = makeRequest(binary_data, binary_len, function_name, num_inputs, input_ptrs, input_bytes, num_outputs,
+                               output_ptrs, output_bytes, tiling_data, tiling_len, block_dim, magic);
+    CallerDeviceScope keepCallerDevice;
+    if (Status s = ex->launchDevice(r, workspace, workspace_bytes, cuda_stream); !s) {
+      writeErr(err_buf, err_len, s.message());
+      return 1;
+    }
+    return 0;
+  });
 }
 
 AFIR_EXPORT int afirt_executor_launch_device_exchange(AfirtExecutor executor, const uint8_t *binary_data, size_t binary_len,
@@ -178,21 +200,23 @@ AFIR_EXPORT int afirt_executor_launch_device_exchange(AfirtExecutor executor, co
                                                       const size_t *output_bytes, const uint8_t *tiling_data, size_t tiling_len,
                                                       int block_dim, uint32_t magic, void *workspace, size_t workspace_bytes,
                                                       void *cuda_stream, AfirtRowsumExchange exchange, char *err_buf, size_t err_len) {
-  auto *ex = reinterpret_cast<CudaExecutor *>(executor);
-  if (!ex || !ex->initialized()) { writeErr(err_buf, err_len, "executor has not been initialized"); return 1; }
-  kernels::RowReduceExchange record;
-  int mailboxDevice = 0;
-  if (Status s = nextExchangeCall(exchange, record, mailboxDevice); !s) { writeErr(err_buf, err_len, s.message()); return 1; }
-  if (mailboxDevice != ex->device()) { writeErr(err_buf, err_len, "the exchange's mailbox is on another device than the executor"); return 1; }
-  RunRequest r = makeRequest(binary_data, binary_len, function_name, num_inputs, input_ptrs, input_bytes, num_outputs,
-                             output_ptrs, output_bytes, tiling_data, tiling_len, block_dim, magic);
-  CallerDeviceScope keepCallerDevice;
-  if (Status s = ex->launchDevice(r, workspace, workspace_bytes, cuda_stream, &record); !s) {
-    writeErr(err_buf, err_len, s.message());
-    return 1;
-  }
-  commitExchangeCall(exchange, record);
-  return 0;
+  return guarded(err_buf, err_len, [&]() -> int {
+    auto *ex = reinterpret_cast<CudaExecutor *>(executor);
+    if (!ex || !ex->initialized()) { writeErr(err_buf, err_len, "executor has not been initialized"); return 1; }
+    kernels::RowReduceExchange record;
+    int mailboxDevice = 0;
+    if (Status s = nextExchangeCall(exchange, record, mailboxDevice); !s) { writeErr(err_buf, err_len, s.message()); return 1; }
+    if (mailboxDevice != ex->device()) { writeErr(err_buf, err_len, "the exchange's mailbox is on another device than the executor"); return 1; }
+    RunRequest r = makeRequest(binary_data, binary_len, function_name, num_inputs, input_ptrs, input_bytes, num_outputs,
+                               output_ptrs, output_bytes, tiling_data, tiling_len, block_dim, magic);
+    CallerDeviceScope keepCallerDevice;
+    if (Status s = ex->launchDevice(r, workspace, workspace_bytes, cuda_stream, &record); !s) {
+      writeErr(err_buf, err_len, s.message());
+      return 1;
+    }
+    commitExchangeCall(exchange, record);
+    return 0;
+  });
 }
 
 AFIR_EXPORT int afirt_executor_launch_device_sharded_table(AfirtExecutor executor, const uint8_t *binary_data, size_t binary_len,
@@ -202,44 +226,50 @@ AFIR_EXPORT int afirt_executor_launch_device_sharded_table(AfirtExecutor executo
                                                            int block_dim, uint32_t magic, void *workspace, size_t workspace_bytes,
                                                            void *cuda_stream, int num_shards, const void **shard_ptrs,
                                                            int64_t rows_per_shard, char *err_buf, size_t err_len) {
-  auto *ex = reinterpret_cast<CudaExecutor *>(executor);
-  if (!ex || !ex->initialized()) { writeErr(err_buf, err_len, "executor has not been initialized"); return 1; }
-  if (num_shards < 1 || !shard_ptrs) { writeErr(err_buf, err_len, "at least one table shard is required"); return 1; }
-  if (rows_per_shard < 1) { writeErr(err_buf, err_len, "rows_per_shard must be positive"); return 1; }
-  std::vector<const void *> shards(shard_ptrs, shard_ptrs + num_shards);
-  RunRequest r = makeRequest(binary_data, binary_len, function_name, num_inputs, input_ptrs, input_bytes, num_outputs,
-                             output_ptrs, output_bytes, tiling_data, tiling_len, block_dim, magic);
-  CallerDeviceScope keepCallerDevice;
-  if (Status s = ex->launchDevice(r, workspace, workspace_bytes, cuda_stream, nullptr, shards, rows_per_shard); !s) {
-    writeErr(err_buf, err_len, s.message());
-    return 1;
-  }
-  return 0;
+  return guarded(err_buf, err_len, [&]() -> int {
+    auto *ex = reinterpret_cast<CudaExecutor *>(executor);
+    if (!ex || !ex->initialized()) { writeErr(err_buf, err_len, "executor has not been initialized"); return 1; }
+    if (num_shards < 1 || !shard_ptrs) { writeErr(err_buf, err_len, "at least one table shard is required"); return 1; }
+    if (rows_per_shard < 1) { writeErr(err_buf, err_len, "rows_per_shard must be positive"); return 1; }
+    std::vector<const void *> shards(shard_ptrs, shard_ptrs + num_shards);
+    RunRequest r = makeRequest(binary_data, binary_len, function_name, num_inputs, input_ptrs, input_bytes, num_outputs,
+                               output_ptrs, output_bytes, tiling_data, tiling_len, block_dim, magic);
+    CallerDeviceScope keepCallerDevice;
+    if (Status s = ex->launchDevice(r, workspace, workspace_bytes, cuda_stream, nullptr, shards, rows_per_shard); !s) {
+      writeErr(err_buf, err_len, s.message());
+      return 1;
+    }
+    return 0;
+  });
 }
 
 AFIR_EXPORT int afirt_executor_synchronize(AfirtExecutor executor, void *cuda_stream, char *err_buf, size_t err_len) {
-  auto *ex = reinterpret_cast<CudaExecutor *>(executor);
-  if (!ex || !ex->initialized()) { writeErr(err_buf, err_len, "executor has not been initialized"); return 1; }
-  CallerDeviceScope keepCallerDevice;
-  if (Status s = ex->synchronize(cuda_stream); !s) { writeErr(err_buf, err_len, s.message()); return 1; }
-  return 0;
+  return guarded(err_buf, err_len, [&]() -> int {
+    auto *ex = reinterpret_cast<CudaExecutor *>(executor);
+    if (!ex || !ex->initialized()) { writeErr(err_buf, err_len, "executor has not been initialized"); return 1; }
+    CallerDeviceScope keepCallerDevice;
+    if (Status s = ex->synchronize(cuda_stream); !s) { writeErr(err_buf, err_len, s.message()); return 1; }
+    return 0;
+  });
 }
 
 AFIR_EXPORT int afirt_executor_workspace_bytes(AfirtExecutor executor, const uint8_t *binary_data, size_t binary_len,
                                                const uint8_t *tiling_data, size_t tiling_len, size_t *out_bytes,
                                                char *err_buf, size_t err_len) {
-  auto *ex = reinterpret_cast<CudaExecutor *>(executor);
-  if (!ex || !ex->initialized()) { writeErr(err_buf, err_len, "executor has not been initialized"); return 1; }
-  if (!out_bytes) { writeErr(err_buf, err_len, "out_bytes is required"); return 1; }
-  LaunchDescriptor desc;
-  if (Status s = parseDescriptorBinary(binary_data, binary_len, desc); !s) { writeErr(err_buf, err_len, s.message()); return 1; }
-  std::map<std::string, int64_t> tiling;
-  if (Status s = unpackTiling(desc, tiling_data, tiling_len, tiling); !s) { writeErr(err_buf, err_len, s.message()); return 1; }
-  size_t bytes = 0;
-  CallerDeviceScope keepCallerDevice;
-  if (Status s = requiredWorkspaceBytes(desc, tiling, ex->device(), bytes); !s) { writeErr(err_buf, err_len, s.message()); return 1; }
-  *out_bytes = bytes;
-  return 0;
+  return guarded(err_buf, err_len, [&]() -> int {
+    auto *ex = reinterpret_cast<CudaExecutor *>(executor);
+    if (!ex || !ex->initialized()) { writeErr(err_buf, err_len, "executor has not been initialized"); return 1; }
+    if (!out_bytes) { writeErr(err_buf, err_len, "out_bytes is required"); return 1; }
+    LaunchDescriptor desc;
+    if (Status s = parseDescriptorBinary(binary_data, binary_len, desc); !s) { writeErr(err_buf, err_len, s.message()); return 1; }
+    std::map<std::string, int64_t> tiling;
+    if (Status s = unpackTiling(desc, tiling_data, tiling_len, tiling); !s) { writeErr(err_buf, err_len, s.message()); return 1; }
+    size_t bytes = 0;
+    CallerDeviceScope keepCallerDevice;
+    if (Status s = requiredWorkspaceBytes(desc, tiling, ex->device(), bytes); !s) { writeErr(err_buf, err_len, s.message()); return 1; }
+    *out_bytes = bytes;
+    return 0;
+  });
 }
 
 AFIR_EXPORT int afirt_executor_last_launch_count(AfirtExecutor executor) {

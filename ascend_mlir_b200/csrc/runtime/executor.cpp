@@ -311,6 +311,8 @@ Status CudaExecutor::runHost(const RunRequest &req) {
   std::map<std::string, int64_t> tiling;
   if (Status s = validate(req, kernel, tiling); !s) return s;
   const std::shared_ptr<const LaunchDescriptor> desc = kernel->desc;
+  if (desc->op.accumulate)
+    return Status::error("[cuda:bindings] kernel '" + desc->kernel + "' adds to its output: outputs are not copied in from the host, launch it on device tensors");
   if (Status s = ensureStream(); !s) return s.withStage("cuda:device");
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
 

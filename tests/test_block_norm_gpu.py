@@ -561,3 +561,80 @@ def test_many_rows_gradients(rt, dtype, kind):
             check(outs, ref.gradient(w, c), (T, D, gate))
         finally:
             ref.COLUMN = saved
+
+
+@pytest.mark.parametrize("act", ["none", "sigmoid", "tanh"])
+def test_gate_extremes(rt, act):
+    """Saturated and non-finite gate values: the activation's limits, and NaN only where the formula has it."""
+    for D in (256, 129):  # vectors; elements
+        c = case("gated", 3, D, "f32", "rms", gate="token", act=act)
+        t = block_inputs(c, 12)
+        values = torch.tensor([100.0, -100.0, 88.0, -88.0, 0.0, -0.0, 1e-30, 30.0], device="cuda")
+        t["gate"][:, :8] = values
+        outs = call(rt, descriptors.gated_residual("f32", eps=EPS, alpha=ALPHA, gate="token", gate_act=act), sizes(c), t)
+        want = ref.forward(wide(t), c)
+        check(outs, want, (act, D))
+        t["gate"][1, 9], t["gate"][1, 10], t["gate"][1, 11] = float("nan"), float("inf"), float("-inf")
+        outs = call(rt, descriptors.gated_residual("f32", eps=EPS, alpha=ALPHA, gate="token", gate_act=act), sizes(c), t)
+        got = outs["out"]
+        assert got[1, 9].isnan() and got[0].isfinite().all() and got[2].isfinite().all()
+        assert got[1, 10:12].isfinite().all() == (act != "none")
+
+
+def test_wide_rows_and_f32_parameters_gradients(rt):
+    """Widths whose rows do not fit twice in shared memory, and f32 parameters beside 16-bit rows."""
+    for T, D, dtype, kind, gate in ((20, 16384, "bf16", "rms", "token"), (9, 8192, "f32", "layer", "token"), (11, 8192, "f16", "layer", "token"),
+                                    (400, 4096, "bf16", "rms", "token"), (300, 2048, "f16", "layer", "group")):
+        c = case("gated", T, D, dtype, kind, gate=gate, act="sigmoid", G=37, next=True)
+        t = block_inputs(c, D, torch.float32)
+        statistics_into(t, c, t["y"].double())
+        statistics_into(t, c, t["out"].double(), "next_")
+        spec = descriptors.gated_residual_grad(dtype, kind=kind, alpha=ALPHA, gate=gate, gate_act="sigmoid", next_norm=True, param_dtype="f32")
+        check(call(rt, spec, sizes(c), t), ref.gradient(wide(t), c), (T, D, dtype, kind))
+
+
+def test_without_a_later_gradient(rt):
+    """dout may be left out before a block; the gradient then is the norm's alone, from values or from a checkpoint."""
+    c = case("norm", 600, 1024, "bf16", "rms")
+    t = block_inputs(c, 13)
+    statistics_into(t, c, t["x"].double())
+    t.update({k: v for k, v in call(rt, descriptors.checkpoint_pack("bf16"), sizes(c), {"x": t["x"]}).items() if k in ("codes", "exps")})
+    for packed in (False, True):
+        outs = call(rt, descriptors.block_norm_grad("bf16", checkpoint=packed), sizes(c), t)
+        w = wide(t)
+        del w["dout"]
+        if packed:
+            w["x"] = ref.restore(t["codes"], t["exps"])
+        check(outs, ref.gradient(w, c), packed)
+
+
+def test_rows_behind_the_last_stay(rt):
+    """A buffer with room for more rows than the call has: they are not touched."""
+    c = case("gated", 10, 128, "bf16", "rms", gate="group", act="sigmoid", G=4)
+    t = block_inputs(c, 14)
+    statistics_into(t, c, t["y"].double())
+    spec = descriptors.gated_residual_grad("bf16", alpha=ALPHA, gate="group", gate_act="sigmoid")
+    s = {"T": 10, "D": 128, "G": 4, "B": 6}
+    t["gate"] = torch.cat([t["gate"], torch.full((3, 128), 5.0, device="cuda").bfloat16()])
+    outs = outputs_for(spec, s, torch.device("cuda"), fill=9)
+    call(rt, spec, s, t, outs)
+    torch.cuda.synchronize()
+    assert (outs["dgate"][3:] == 9).all()
+    want = ref.gradient(dict(wide(t), gate=t["gate"][:3].double()), c)
+    check(dict(outs, dgate=outs["dgate"][:3]), want)
+
+
+def test_current_device_and_stream_order(rt):
+    """A launch on a side stream after its inputs were made there; the caller's device stays the current one."""
+    c = case("norm", 2000, 512, "bf16", "rms")
+    t = block_inputs(c, 15)
+    want = call(rt, descriptors.block_norm("bf16", eps=EPS), sizes(c), t)["h"].clone()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        x = torch.zeros_like(t["x"])
+        torch.cuda._sleep(2_000_000)
+        x.copy_(t["x"])
+        got = call(rt, descriptors.block_norm("bf16", eps=EPS), sizes(c), dict(t, x=x))["h"]
+    side.synchronize()
+    assert torch.equal(got, want) and torch.cuda.current_device() == 0

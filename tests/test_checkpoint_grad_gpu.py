@@ -172,3 +172,20 @@ def test_refusals(rt):
     ws = torch.empty(256, dtype=torch.uint8, device="cuda")
     with pytest.raises(ExecutorError, match="overlaps"):
         rt.launch_device(spec.binary, spec.name, a, [a[2][:1] + (32 * 8 * 2,)], spec.pack(s), 0, spec.magic, (ws.data_ptr(), 256), 0)
+
+
+def test_host_path(rt):
+    """Host arrays: the product is copied out; one that adds to its output is refused, since outputs are not copied in."""
+    import numpy as np
+    x, dy = inputs(40, 64, 32, "f16", 5)
+    codes, exps = packed(rt, x, "f16")
+    s = {"T": 40, "D": 64, "N": 32}
+    spec = descriptors.checkpoint_weight_grad("f16")
+    want = call(rt, spec, s, {"codes": codes, "exps": exps, "dy": dy})["dweight"]
+    host = [np.zeros((64, 32), np.float16)]
+    args = [codes.cpu().numpy(), exps.cpu().numpy(), dy.cpu().numpy()]
+    rt.run(spec.binary, spec.name, args, host, spec.pack(s))
+    assert np.array_equal(host[0], want.cpu().numpy())
+    spec = descriptors.checkpoint_weight_grad("f16", out_dtype="f32", accumulate=True)
+    with pytest.raises(ExecutorError, match="adds to its output"):
+        rt.run(spec.binary, spec.name, args, [np.zeros((64, 32), np.float32)], spec.pack(s))
