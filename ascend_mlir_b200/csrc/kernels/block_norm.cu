@@ -145,24 +145,21 @@ template <int VALUES> __global__ void __launch_bounds__(kFinishThreads) blockNor
 // ---- launch shape -----------------------------------------------------------------------------------------------
 constexpr size_t kAheadBytes = 225 * 1024;  // of the 227 KB that the CTAs of an SM can have, each with 1 KB of its own
 
-struct TeamShape { bool vector; int nv, lanes, teamsPerCta; };
+struct TeamShape { int nv, lanes, teamsPerCta; };
 
 TeamShape shapeOf(int vec, int nv, int64_t cols) {
   TeamShape s;
-  s.vector = vec > 1;
   s.nv = nv;
   const int64_t perThread = static_cast<int64_t>(nv) * vec;
   s.lanes = static_cast<int>(((cols + perThread - 1) / perThread + 31) / 32 * 32);
   s.teamsPerCta = std::max(1, 256 / s.lanes);
   return s;
 }
-int scalarElements(int64_t cols) { return cols <= kScalarSmall * 512 ? kScalarSmall : kScalarLarge; }
 
 // A team has at most 512 threads.  Few rows: one vector per thread while that is enough, for the shortest way through one
 // row; else 16 columns per thread.
-TeamShape forwardShape(int elemType, int64_t rows, int64_t cols, bool vector, int smCount) {
-  const int vec = vector ? (elemType == kF32 ? 4 : 8) : 1;
-  if (!vector) return shapeOf(1, scalarElements(cols), cols);
+TeamShape forwardShape(int elemType, int64_t rows, int64_t cols, int smCount) {
+  const int vec = elemType == kF32 ? 4 : 8;
   const int64_t perThread = rows >= smCount ? 16 : vec;
   int nv = 1;
   while (nv * vec < perThread && static_cast<int64_t>(nv) * vec * 32 < cols) nv *= 2;
@@ -173,18 +170,12 @@ TeamShape forwardShape(int elemType, int64_t rows, int64_t cols, bool vector, in
 // The gradient with rows fetched ahead, 512 threads per SM: two vectors per thread (one of a 16-bit layer norm, which keeps
 // twice the column sums in registers), in a team of up to 512 threads, beyond that what the width needs; fewer where
 // that makes every thread's vectors lie inside the row, which spares the kernel its tests.
-TeamShape gradShape(int elemType, int kind, int64_t cols, bool vector) {
-  const int vec = vector ? (elemType == kF32 ? 4 : 8) : 1;
-  if (!vector) return shapeOf(1, scalarElements(cols), cols);
+TeamShape gradShape(int elemType, int kind, int64_t cols) {
+  const int vec = elemType == kF32 ? 4 : 8;
   int nv = kind == kLayerNorm && elemType != kF32 ? 1 : 2;
   if (nv == 2 && cols % (64 * vec) != 0 && (cols % (32 * vec) == 0 || cols < 32 * vec) && cols <= 512 * vec) nv = 1;
   while (static_cast<int64_t>(nv) * vec * 512 < cols) nv *= 2;
   return shapeOf(vec, nv, cols);
-}
-// Without rows ahead: 4 vectors per thread, 8 for the widest f32 rows.
-TeamShape wideShape(int elemType, int64_t cols) {
-  const int vec = elemType == kF32 ? 4 : 8;
-  return shapeOf(vec, 4 * vec * 512 < cols ? 8 : 4, cols);
 }
 
 GradAheadKernel aheadKernel(int elemType, int kind, int pass, bool token, bool full, int nv) {
@@ -266,7 +257,7 @@ int launchBlockNorm(const BlockNormLaunch &l, cudaStream_t stream, int *launched
   // parameters: 1024 threads per SM (64 registers each) before a block, up to 768 (80 registers) behind it, in one CTA that
   // shares its parameters.
   if (vector) {
-    TeamShape s = gradShape(l.elemType, kRmsNorm, l.cols, true);
+    TeamShape s = gradShape(l.elemType, kRmsNorm, l.cols);
     if (s.nv <= 2) {
       const int ctaThreads = l.pass == kPre ? kForwardAheadThreads : kForwardAheadPostThreads, ctasPerSm = l.pass == kPre ? 2 : 1;
       s.teamsPerCta = std::max(1, std::min(15, ctaThreads / s.lanes));
@@ -291,24 +282,13 @@ int launchBlockNorm(const BlockNormLaunch &l, cudaStream_t stream, int *launched
       }
     }
   }
-  const TeamShape s = forwardShape(l.elemType, l.rows, l.cols, vector, sms);
+  const TeamShape s = forwardShape(l.elemType, l.rows, l.cols, sms);
   const ForwardKernel kernel = l.elemType == kF32   ? forwardKernel<kF32>(l.kind, l.pass, vector, s.nv)
                                : l.elemType == kF16 ? forwardKernel<kF16>(l.kind, l.pass, vector, s.nv)
                                                     : forwardKernel<kBF16>(l.kind, l.pass, vector, s.nv);
   if (!kernel) return cudaErrorInvalidValue;
   const int64_t ctas = (l.rows + s.teamsPerCta - 1) / s.teamsPerCta;
   const unsigned int grid = static_cast<unsigned int>(std::min<int64_t>(ctas, 0x7fffffff));
-  // without vectors a block of 128 columns spans warps: the checkpoint is a launch of its own, and the first one, in
-  // case an output takes the place of the tensor it reads
-  if (l.checkpoint.codes && !vector) {
-    CheckpointPackLaunch c = {};
-    c.elemType = l.elemType;
-    c.rows = l.rows;
-    c.cols = l.cols;
-    c.x = l.pass == kPre ? l.x : l.y;
-    c.out = l.checkpoint;
-    if (const int rc = launchCheckpointPack(c, stream, launched); rc != 0) return rc;
-  }
   const cudaError_t e = launchDependent(kernel, dim3(grid), dim3(static_cast<unsigned int>(s.lanes * s.teamsPerCta)), 0, stream, l, s.lanes);
   if (e == cudaSuccess && launched) *launched += 1;
   return e;
@@ -340,9 +320,9 @@ int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *
     if (l.gateForm == kGateToken) vector = vector && rowsAligned(l.dgate.base, l.dgate.ld, eb, 16);
     for (const void *v : {l.a.weight, l.a.bias, l.b.weight, l.scale}) vector = vector && vectorAligned(v);
     vector = vector && rowsAligned(l.checkpoint.codes, l.checkpoint.codesLd, 1, vec);
-    TeamShape s = gradShape(l.elemType, l.kind, l.cols, vector);
+    TeamShape s = gradShape(l.elemType, l.kind, l.cols);
     // (few teams: spread over the SMs)
-    if (vector) s.teamsPerCta = std::max(1, std::min({15, kGradAheadThreads / s.lanes, (plan.teams + sms - 1) / sms}));
+    s.teamsPerCta = std::max(1, std::min({15, kGradAheadThreads / s.lanes, (plan.teams + sms - 1) / sms}));
     // rows fetched ahead: as many (2 to 4) as a CTA has shared memory for beside its parameters; rows too wide for two take
     // the kernel without
     const int tensors = (l.pass != kPost ? 2 : 0) + (l.dout.base ? 1 : 0) + (l.pass != kPre ? 1 : 0) + (l.gateForm == kGateToken ? 1 : 0);
@@ -353,7 +333,6 @@ int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *
     const int stages = static_cast<int>(std::min<size_t>(4, std::max<size_t>(2, (perCta - std::min(perCta, paramBytes)) / rowBytes)));
     const size_t slotBytes = static_cast<size_t>(stages) * rowBytes + paramBytes;
     const GradAheadKernel ahead = vector && slotBytes <= kAheadBytes ? aheadKernel(l.elemType, l.kind, l.pass, l.gateForm == kGateToken, static_cast<int64_t>(s.lanes) * s.nv * vec == l.cols, s.nv) : nullptr;
-    if (!ahead && vector) s = wideShape(l.elemType, l.cols);
     const unsigned int threads = static_cast<unsigned int>(s.lanes * s.teamsPerCta);
     const dim3 grid(static_cast<unsigned int>((plan.teams + s.teamsPerCta - 1) / s.teamsPerCta));
     cudaError_t e;
@@ -361,9 +340,9 @@ int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *
       if (e = reserveSharedMemory(reinterpret_cast<const void *>(ahead), static_cast<int>(kAheadBytes)); e != cudaSuccess) return e;
       e = launchDependent(ahead, grid, dim3(threads), slotBytes, stream, l, plan, s.lanes, stages);
     } else {
-      const GradKernel kernel = l.elemType == kF32   ? gradKernel<kF32>(l.kind, l.pass, vector, s.nv)
-                                : l.elemType == kF16 ? gradKernel<kF16>(l.kind, l.pass, vector, s.nv)
-                                                     : gradKernel<kBF16>(l.kind, l.pass, vector, s.nv);
+      const GradKernel kernel = l.elemType == kF32   ? gradKernel<kF32>(l.kind, l.pass, s.nv)
+                                : l.elemType == kF16 ? gradKernel<kF16>(l.kind, l.pass, s.nv)
+                                                     : gradKernel<kBF16>(l.kind, l.pass, s.nv);
       if (!kernel) return cudaErrorInvalidValue;
       e = launchDependent(kernel, grid, dim3(threads), 0, stream, l, plan, s.lanes);
     }

@@ -233,19 +233,6 @@ template <int VEC> __device__ __forceinline__ void valuesOfCodes(const unsigned 
     }
   }
 }
-template <int VEC> __device__ __forceinline__ void loadCheckpoint(const CheckpointIn &c, int64_t row, int col, float (&v)[VEC]) {
-  const float power = powerOfExponent(c.exps[row * c.expsLd + col / kCheckpointBlock]);
-  const uint8_t *p = c.codes + row * c.codesLd + col;
-  unsigned int w[VEC / 4 > 0 ? VEC / 4 : 1];
-  if constexpr (VEC == 1) w[0] = *p;
-  else if constexpr (VEC == 8) {
-    const uint2 r = *reinterpret_cast<const uint2 *>(p);
-    w[0] = r.x;
-    w[1] = r.y;
-  } else w[0] = *reinterpret_cast<const unsigned int *>(p);
-  valuesOfCodes<VEC>(w, power, v);
-}
-
 // ---- the gate ---------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float gateValue(float g, int act) {
   if (act == kActSigmoid) return 1.0f / (1.0f + expf(-g));

@@ -6,7 +6,7 @@
 // rounded once each, and normB reads `out` as it was rounded, which is what the gradient pass will read.
 #pragma once
 
-#include "kernels/block_norm_device.cuh"
+#include "kernels/loose.cuh"
 
 namespace afir {
 namespace kernels {
@@ -31,7 +31,7 @@ __device__ __forceinline__ void rowStatistics(Team &team, const float (&v)[NV][V
     if ((i * team.lanes + team.lane) * VEC >= cols) continue;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const float d = v[i][e] - mean;
+      const float d = (i * team.lanes + team.lane) * VEC + e < cols ? v[i][e] - mean : 0.0f;
       q[0] += d * d;
     }
   }
@@ -47,15 +47,15 @@ __device__ __forceinline__ void storeNormed(const Team &team, const float (&v)[N
     const int col = (i * team.lanes + team.lane) * VEC;
     if (col >= cols) continue;
     float w[VEC], r[VEC];
-    loadParam<ELEM, VEC>(p.weight, paramType, col, w);
+    looseParam<ELEM, VEC>(p.weight, paramType, col, cols, w);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) r[e] = (v[i][e] - mean) * rstd * w[e];
     if constexpr (KIND == kLayerNorm) {
-      loadParam<ELEM, VEC>(p.bias, paramType, col, w);
+      looseParam<ELEM, VEC>(p.bias, paramType, col, cols, w);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) r[e] += w[e];
     }
-    storeElems<ELEM, VEC>(base, rowAt + col, r);
+    looseStore<ELEM, VEC>(base, rowAt, col, cols, r);
   }
 }
 
@@ -65,10 +65,11 @@ __device__ __forceinline__ void storeStatistics(const Team &team, const NormStat
   if (s.mean) s.mean[row] = mean;
 }
 
-// Any width and alignment, an element at a time.
-template <int ELEM, int KIND, int PASS, int VEC, int NV>
+// Any width and alignment (loose.cuh).
+template <int ELEM, int KIND, int PASS, int NV>
 __global__ void __launch_bounds__(512) blockNormForwardKernel(const __grid_constant__ BlockNormLaunch p, int teamLanes) {
   gridDependencyPrologue();
+  constexpr int VEC = ElemOf<ELEM>::kVec, EB = 16 / VEC;
   __shared__ float scratch[kTeamScratchFloats];
   Team team = makeTeam(teamLanes, scratch);
   const int cols = static_cast<int>(p.cols);
@@ -81,7 +82,18 @@ __global__ void __launch_bounds__(512) blockNormForwardKernel(const __grid_const
       const int col = (i * team.lanes + team.lane) * VEC;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) v[i][e] = 0.0f;
-      if (col < cols) loadElems<ELEM, VEC>(first.base, row * first.ld + col, v[i]);
+      if (col < cols) looseLoad<ELEM, VEC>(first.base, row * first.ld, col, cols, innerRow(row, p.rows, first.ld * EB), v[i]);
+    }
+    if (p.checkpoint.codes) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int col = (i * team.lanes + team.lane) * VEC;
+        unsigned int codes[VEC / 4];
+        const int e8 = codesOf<ELEM>(pack<ELEM, VEC>(v[i]), codes);  // the values as they were
+        if (col >= cols) continue;
+        looseCodes(p.checkpoint.codes + row * p.checkpoint.codesLd + col, col, cols, codes);
+        if (col % kCheckpointBlock == 0) p.checkpoint.exps[row * p.checkpoint.expsLd + col / kCheckpointBlock] = static_cast<uint8_t>(e8);
+      }
     }
     float mean, rstd;
     rowStatistics<KIND, NV, VEC>(team, v, cols, PASS == kPre ? p.epsB : p.epsA, mean, rstd);
@@ -90,35 +102,36 @@ __global__ void __launch_bounds__(512) blockNormForwardKernel(const __grid_const
       storeNormed<ELEM, KIND, NV, VEC>(team, v, cols, mean, rstd, p.b, p.paramType, p.h.base, row * p.h.ld);
     } else {
       storeStatistics(team, p.statsA, row, mean, rstd);
-      const int64_t gateRow = p.gateForm == kGateGroup ? row / p.groupRows : row;
+      const bool grouped = p.gateForm == kGateGroup;
+      const int64_t gateRow = grouped ? row / p.groupRows : row, gateRows = grouped ? (p.rows + p.groupRows - 1) / p.groupRows : p.rows;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int col = (i * team.lanes + team.lane) * VEC;
         if (col >= cols) continue;
         float t[VEC];
-        loadParam<ELEM, VEC>(p.a.weight, p.paramType, col, t);
+        looseParam<ELEM, VEC>(p.a.weight, p.paramType, col, cols, t);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[i][e] = (v[i][e] - mean) * rstd * t[e];
         if constexpr (KIND == kLayerNorm) {
-          loadParam<ELEM, VEC>(p.a.bias, p.paramType, col, t);
+          looseParam<ELEM, VEC>(p.a.bias, p.paramType, col, cols, t);
 #pragma unroll
           for (int e = 0; e < VEC; ++e) v[i][e] += t[e];
         }
         if (p.gateForm != kGateNone) {
-          loadElems<ELEM, VEC>(p.gate.base, gateRow * p.gate.ld + col, t);
+          looseLoad<ELEM, VEC>(p.gate.base, gateRow * p.gate.ld, col, cols, innerRow(gateRow, gateRows, p.gate.ld * EB), t);
 #pragma unroll
           for (int e = 0; e < VEC; ++e) v[i][e] *= gateValue(t[e], p.gateAct);
         }
         if (p.scale) {
-          loadParam<ELEM, VEC>(p.scale, p.paramType, col, t);
+          looseParam<ELEM, VEC>(p.scale, p.paramType, col, cols, t);
 #pragma unroll
           for (int e = 0; e < VEC; ++e) v[i][e] *= t[e];
         }
-        loadElems<ELEM, VEC>(p.x.base, row * p.x.ld + col, t);
+        looseLoad<ELEM, VEC>(p.x.base, row * p.x.ld, col, cols, innerRow(row, p.rows, p.x.ld * EB), t);
 #pragma unroll
         for (int e = 0; e < VEC; ++e)  // as it is stored
           v[i][e] = ElemOf<ELEM>::widen(ElemOf<ELEM>::narrow(fmaf(p.alpha, t[e], v[i][e])));
-        storeElems<ELEM, VEC>(p.out.base, row * p.out.ld + col, v[i]);
+        looseStore<ELEM, VEC>(p.out.base, row * p.out.ld, col, cols, v[i]);
       }
       if constexpr (PASS == kPostPre) {
         rowStatistics<KIND, NV, VEC>(team, v, cols, p.epsB, mean, rstd);

@@ -9,13 +9,12 @@ namespace afir {
 namespace kernels {
 
 template <int ELEM, int KIND, int PASS> ForwardKernel forwardKernelOf(bool vector, int nv) {
-  if (!vector) return nv <= kScalarSmall ? blockNormForwardKernel<ELEM, KIND, PASS, 1, kScalarSmall> : blockNormForwardKernel<ELEM, KIND, PASS, 1, kScalarLarge>;
   switch (nv) {
-  case 1: return blockNormForwardVectorKernel<ELEM, KIND, PASS, 1>;
-  case 2: return blockNormForwardVectorKernel<ELEM, KIND, PASS, 2>;
-  case 4: return blockNormForwardVectorKernel<ELEM, KIND, PASS, 4>;
+  case 1: return vector ? blockNormForwardVectorKernel<ELEM, KIND, PASS, 1> : blockNormForwardKernel<ELEM, KIND, PASS, 1>;
+  case 2: return vector ? blockNormForwardVectorKernel<ELEM, KIND, PASS, 2> : blockNormForwardKernel<ELEM, KIND, PASS, 2>;
+  case 4: return vector ? blockNormForwardVectorKernel<ELEM, KIND, PASS, 4> : blockNormForwardKernel<ELEM, KIND, PASS, 4>;
   default:
-    if constexpr (ELEM == kF32) return blockNormForwardVectorKernel<ELEM, KIND, PASS, 8>;
+    if constexpr (ELEM == kF32) return vector ? blockNormForwardVectorKernel<ELEM, KIND, PASS, 8> : blockNormForwardKernel<ELEM, KIND, PASS, 8>;
     else return nullptr;
   }
 }

@@ -15,7 +15,7 @@
 // (no atomics: the same inputs give the same bits).
 #pragma once
 
-#include "kernels/block_norm_device.cuh"
+#include "kernels/loose.cuh"
 
 namespace afir {
 namespace kernels {
@@ -32,19 +32,14 @@ struct GradPlan {
   float *sumsA, *sumsB;   // [groups*chunks][values][sumsLd], [teams][values][sumsLd]
 };
 
-template <int VEC> __device__ __forceinline__ void storeSums(float *to, const float (&v)[VEC]) {
-  if constexpr (VEC == 1) *to = v[0];
-  else {
-#pragma unroll
-    for (int i = 0; i < VEC / 4; ++i) reinterpret_cast<float4 *>(to)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-  }
-}
-
-template <int ELEM, int KIND, int PASS, int VEC, int NV>
+// Any width and alignment (loose.cuh); aligned rows too that are too wide for block_norm_grad_vector.cuh.  Elements beyond
+// the row are zeros, as are the parameters read for them, so they add nothing to a row's sums; they are not stored.
+template <int ELEM, int KIND, int PASS, int NV>
 __global__ void __launch_bounds__(512) blockNormGradKernel(const __grid_constant__ BlockNormGradLaunch p, const __grid_constant__ GradPlan plan,
                                                            int teamLanes) {
   gridDependencyPrologue();
   constexpr bool kLayer = KIND == kLayerNorm;
+  constexpr int VEC = ElemOf<ELEM>::kVec, EB = 16 / VEC;
   constexpr int kValues = kLayer ? 2 : 1;
   constexpr bool kPostPart = PASS != kPre, kPrePart = PASS != kPost;
   __shared__ float scratch[kTeamScratchFloats];
@@ -91,10 +86,10 @@ __global__ void __launch_bounds__(512) blockNormGradKernel(const __grid_constant
           const int col = (i * team.lanes + team.lane) * VEC;
           if (col >= cols) continue;
           float w[VEC];
-          if (fromCodes) loadCheckpoint<VEC>(p.checkpoint, row, col, n[i]);
-          else loadElems<ELEM, VEC>(p.source.base, row * p.source.ld + col, n[i]);
-          loadElems<ELEM, VEC>(p.dh.base, row * p.dh.ld + col, dz[i]);
-          loadParam<ELEM, VEC>(p.b.weight, p.paramType, col, w);
+          if (fromCodes) looseCheckpoint<VEC>(p.checkpoint, row, col, cols, innerRow(row, p.rows, p.checkpoint.codesLd), n[i]);
+          else looseLoad<ELEM, VEC>(p.source.base, row * p.source.ld, col, cols, innerRow(row, p.rows, p.source.ld * EB), n[i]);
+          looseLoad<ELEM, VEC>(p.dh.base, row * p.dh.ld, col, cols, innerRow(row, p.rows, p.dh.ld * EB), dz[i]);
+          looseParam<ELEM, VEC>(p.b.weight, p.paramType, col, cols, w);
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
             n[i][e] = (n[i][e] - mean) * rstd;
@@ -117,7 +112,7 @@ __global__ void __launch_bounds__(512) blockNormGradKernel(const __grid_constant
           for (int e = 0; e < VEC; ++e) dz[i][e] = rstd * (dz[i][e] - n[i][e] * along - constant);
           if (p.dout.base) {
             float t[VEC];
-            loadElems<ELEM, VEC>(p.dout.base, row * p.dout.ld + col, t);
+            looseLoad<ELEM, VEC>(p.dout.base, row * p.dout.ld, col, cols, innerRow(row, p.rows, p.dout.ld * EB), t);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) dz[i][e] += t[e];
           }
@@ -126,14 +121,14 @@ __global__ void __launch_bounds__(512) blockNormGradKernel(const __grid_constant
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           const int col = (i * team.lanes + team.lane) * VEC;
-          if (col < cols) loadElems<ELEM, VEC>(p.dout.base, row * p.dout.ld + col, dz[i]);
+          if (col < cols) looseLoad<ELEM, VEC>(p.dout.base, row * p.dout.ld, col, cols, innerRow(row, p.rows, p.dout.ld * EB), dz[i]);
         }
       }
       if constexpr (!kPostPart) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           const int col = (i * team.lanes + team.lane) * VEC;
-          if (col < cols) storeElems<ELEM, VEC>(p.dx.base, row * p.dx.ld + col, dz[i]);
+          if (col < cols) looseStore<ELEM, VEC>(p.dx.base, row * p.dx.ld, col, cols, dz[i]);
         }
       } else {
         // ---- through the gated sum and normA
@@ -149,8 +144,8 @@ __global__ void __launch_bounds__(512) blockNormGradKernel(const __grid_constant
           const int col = (i * team.lanes + team.lane) * VEC;
           if (col >= cols) continue;
           float t[VEC], a[VEC], scale[VEC], w[VEC];
-          if (fromCodes) loadCheckpoint<VEC>(p.checkpoint, row, col, n[i]);
-          else loadElems<ELEM, VEC>(p.y.base, row * p.y.ld + col, n[i]);
+          if (fromCodes) looseCheckpoint<VEC>(p.checkpoint, row, col, cols, innerRow(row, p.rows, p.checkpoint.codesLd), n[i]);
+          else looseLoad<ELEM, VEC>(p.y.base, row * p.y.ld, col, cols, innerRow(row, p.rows, p.y.ld * EB), n[i]);
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
             n[i][e] = (n[i][e] - mean) * rstd;
@@ -158,23 +153,26 @@ __global__ void __launch_bounds__(512) blockNormGradKernel(const __grid_constant
             scale[e] = 1.0f;
           }
           if (p.gateForm != kGateNone) {
-            loadElems<ELEM, VEC>(p.gate.base, (token ? row : group) * p.gate.ld + col, a);
+            {
+              const int64_t gateRow = token ? row : group;
+              looseLoad<ELEM, VEC>(p.gate.base, gateRow * p.gate.ld, col, cols, innerRow(gateRow, token ? p.rows : plan.groups, p.gate.ld * EB), a);
+            }
 #pragma unroll
             for (int e = 0; e < VEC; ++e) a[e] = gateValue(a[e], p.gateAct);
           }
-          if (p.scale) loadParam<ELEM, VEC>(p.scale, p.paramType, col, scale);
-          loadParam<ELEM, VEC>(p.a.weight, p.paramType, col, w);
+          if (p.scale) looseParam<ELEM, VEC>(p.scale, p.paramType, col, cols, scale);
+          looseParam<ELEM, VEC>(p.a.weight, p.paramType, col, cols, w);
 #pragma unroll
           for (int e = 0; e < VEC; ++e) t[e] = p.alpha * dz[i][e];
-          storeElems<ELEM, VEC>(p.dx.base, row * p.dx.ld + col, t);
+          looseStore<ELEM, VEC>(p.dx.base, row * p.dx.ld, col, cols, t);
           if (token) {
             float bias[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) bias[e] = 0.0f;
-            if constexpr (kLayer) loadParam<ELEM, VEC>(p.a.bias, p.paramType, col, bias);
+            if constexpr (kLayer) looseParam<ELEM, VEC>(p.a.bias, p.paramType, col, cols, bias);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) t[e] = dz[i][e] * scale[e] * fmaf(n[i][e], w[e], bias[e]) * gateSlope(a[e], p.gateAct);
-            storeElems<ELEM, VEC>(p.dgate.base, row * p.dgate.ld + col, t);
+            looseStore<ELEM, VEC>(p.dgate.base, row * p.dgate.ld, col, cols, t);
           }
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
@@ -197,7 +195,7 @@ __global__ void __launch_bounds__(512) blockNormGradKernel(const __grid_constant
           float t[VEC];
 #pragma unroll
           for (int e = 0; e < VEC; ++e) t[e] = rstd * (dz[i][e] - n[i][e] * along - constant);
-          storeElems<ELEM, VEC>(p.dy.base, row * p.dy.ld + col, t);
+          looseStore<ELEM, VEC>(p.dy.base, row * p.dy.ld, col, cols, t);
         }
       }
     }
@@ -207,7 +205,7 @@ __global__ void __launch_bounds__(512) blockNormGradKernel(const __grid_constant
         const int col = (i * team.lanes + team.lane) * VEC;
         if (col >= cols) continue;
 #pragma unroll
-        for (int k = 0; k < kValues; ++k) storeSums<VEC>(plan.sumsA + (static_cast<int64_t>(run) * kValues + k) * plan.sumsLd + col, sumA[k][i]);
+        for (int k = 0; k < kValues; ++k) looseSums<VEC>(plan.sumsA + (static_cast<int64_t>(run) * kValues + k) * plan.sumsLd + col, col, cols, sumA[k][i]);
       }
     }
   }
@@ -217,7 +215,7 @@ __global__ void __launch_bounds__(512) blockNormGradKernel(const __grid_constant
       const int col = (i * team.lanes + team.lane) * VEC;
       if (col >= cols) continue;
 #pragma unroll
-      for (int k = 0; k < kValues; ++k) storeSums<VEC>(plan.sumsB + (static_cast<int64_t>(teamIndex) * kValues + k) * plan.sumsLd + col, sumB[k][i]);
+      for (int k = 0; k < kValues; ++k) looseSums<VEC>(plan.sumsB + (static_cast<int64_t>(teamIndex) * kValues + k) * plan.sumsLd + col, col, cols, sumB[k][i]);
     }
   }
 }

@@ -2,6 +2,6 @@
 
 namespace afir {
 namespace kernels {
-template GradKernel gradKernel<kF32>(int kind, int pass, bool vector, int nv);
+template GradKernel gradKernel<kF32>(int kind, int pass, int nv);
 } // namespace kernels
 } // namespace afir

@@ -7,18 +7,20 @@
 namespace afir {
 namespace kernels {
 
-// Vectors without rows fetched ahead: rows too wide for two of them in shared memory.
-template <int ELEM, int KIND, int PASS> GradKernel gradKernelOf(bool vector, int nv) {
-  constexpr int V = ElemOf<ELEM>::kVec;
-  if (!vector) return nv <= kScalarSmall ? blockNormGradKernel<ELEM, KIND, PASS, 1, kScalarSmall> : blockNormGradKernel<ELEM, KIND, PASS, 1, kScalarLarge>;
-  if (nv <= 4) return blockNormGradKernel<ELEM, KIND, PASS, V, 4>;
-  if constexpr (ELEM == kF32) return blockNormGradKernel<ELEM, KIND, PASS, V, 8>;
-  else return nullptr;
+template <int ELEM, int KIND, int PASS> GradKernel gradKernelOf(int nv) {
+  switch (nv) {
+  case 1: return blockNormGradKernel<ELEM, KIND, PASS, 1>;
+  case 2: return blockNormGradKernel<ELEM, KIND, PASS, 2>;
+  case 4: return blockNormGradKernel<ELEM, KIND, PASS, 4>;
+  default:
+    if constexpr (ELEM == kF32) return blockNormGradKernel<ELEM, KIND, PASS, 8>;
+    else return nullptr;
+  }
 }
-template <int ELEM> GradKernel gradKernel(int kind, int pass, bool vector, int nv) {
+template <int ELEM> GradKernel gradKernel(int kind, int pass, int nv) {
   if (kind == kLayerNorm)
-    return pass == kPre ? gradKernelOf<ELEM, kLayerNorm, kPre>(vector, nv) : pass == kPost ? gradKernelOf<ELEM, kLayerNorm, kPost>(vector, nv) : gradKernelOf<ELEM, kLayerNorm, kPostPre>(vector, nv);
-  return pass == kPre ? gradKernelOf<ELEM, kRmsNorm, kPre>(vector, nv) : pass == kPost ? gradKernelOf<ELEM, kRmsNorm, kPost>(vector, nv) : gradKernelOf<ELEM, kRmsNorm, kPostPre>(vector, nv);
+    return pass == kPre ? gradKernelOf<ELEM, kLayerNorm, kPre>(nv) : pass == kPost ? gradKernelOf<ELEM, kLayerNorm, kPost>(nv) : gradKernelOf<ELEM, kLayerNorm, kPostPre>(nv);
+  return pass == kPre ? gradKernelOf<ELEM, kRmsNorm, kPre>(nv) : pass == kPost ? gradKernelOf<ELEM, kRmsNorm, kPost>(nv) : gradKernelOf<ELEM, kRmsNorm, kPostPre>(nv);
 }
 } // namespace kernels
 } // namespace afir

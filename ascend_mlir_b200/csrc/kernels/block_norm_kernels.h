@@ -7,16 +7,14 @@
 namespace afir {
 namespace kernels {
 
-// `vector`: 16-byte accesses; nv = vectors (or, without them, elements) per thread.
-constexpr int kScalarSmall = 8, kScalarLarge = 32;
-
+// `vector`: everything is aligned for 16-byte accesses; nv = vectors per thread.
 using ForwardKernel = void (*)(const BlockNormLaunch, int);
 using GradKernel = void (*)(const BlockNormGradLaunch, const GradPlan, int);
 template <int ELEM> ForwardKernel forwardKernel(int kind, int pass, bool vector, int nv);
 // Teams that stay, with rows fetched ahead (block_norm_forward_ahead.cuh).
 using ForwardAheadKernel = void (*)(const BlockNormLaunch, int, int);
 template <int ELEM> ForwardAheadKernel forwardAheadKernel(int kind, int pass, bool full, int nv);
-template <int ELEM> GradKernel gradKernel(int kind, int pass, bool vector, int nv);
+template <int ELEM> GradKernel gradKernel(int kind, int pass, int nv);
 // With rows fetched ahead (block_norm_grad_vector.cuh); null where a thread would hold more than it has registers for.
 using GradAheadKernel = void (*)(const BlockNormGradLaunch, const GradPlan, int, int);
 template <int ELEM, int KIND> GradAheadKernel gradAheadKernel(int pass, bool token, bool full, int nv);

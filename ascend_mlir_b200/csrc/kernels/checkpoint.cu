@@ -8,7 +8,7 @@
 #include <algorithm>
 
 #include "kernels/launch_util.h"
-#include "kernels/pairs.cuh"
+#include "kernels/loose.cuh"
 
 namespace afir {
 namespace kernels {
@@ -17,10 +17,11 @@ namespace {
 constexpr int kThreads = 256;
 
 // 128 columns are 16 lanes (8 columns each, 16-bit types) or 32 lanes (4 each, f32).  A team of whole warps walks a row,
-// kAhead vectors per thread at a time, all loaded before the first is used; a row may end inside a block.
+// kAhead vectors per thread at a time, all loaded before the first is used; a row may end inside a block.  LOOSE: rows of any
+// width and alignment (loose.cuh).
 constexpr int kAhead = 4;
-template <int ELEM>
-__global__ void __launch_bounds__(kThreads) checkpointPackVectorKernel(const __grid_constant__ CheckpointPackLaunch p, int lanes) {
+template <int ELEM, bool LOOSE>
+__global__ void __launch_bounds__(kThreads) checkpointPackKernel(const __grid_constant__ CheckpointPackLaunch p, int lanes) {
   gridDependencyPrologue();
   constexpr int VEC = ElemOf<ELEM>::kVec;
   const int cols = static_cast<int>(p.cols);
@@ -33,63 +34,51 @@ __global__ void __launch_bounds__(kThreads) checkpointPackVectorKernel(const __g
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         const int col = base + i * lanes * VEC;
-        raw[i] = col < cols ? *reinterpret_cast<const uint4 *>(from + static_cast<int64_t>(col) * (16 / VEC)) : make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (LOOSE) {
+          float v[VEC];
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) v[e] = 0.0f;
+          if (col < cols) looseLoad<ELEM, VEC>(p.x.base, row * p.x.ld, col, cols, innerRow(row, p.rows, p.x.ld * (16 / VEC)), v);
+          raw[i] = pack<ELEM, VEC>(v);  // the values as they were
+        } else raw[i] = col < cols ? *reinterpret_cast<const uint4 *>(from + static_cast<int64_t>(col) * (16 / VEC)) : make_uint4(0u, 0u, 0u, 0u);
       }
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         const int col = base + i * lanes * VEC;
         if (col - lane * VEC >= cols) break;  // the whole team's
-        packVector<ELEM>(raw[i], col < cols, col, row, p.out);
+        if constexpr (LOOSE) {
+          unsigned int codes[VEC / 4];
+          const int e8 = codesOf<ELEM>(raw[i], codes);
+          if (col >= cols) continue;
+          looseCodes(p.out.codes + row * p.out.codesLd + col, col, cols, codes);
+          if (col % kCheckpointBlock == 0) p.out.exps[row * p.out.expsLd + col / kCheckpointBlock] = static_cast<uint8_t>(e8);
+        } else packVector<ELEM>(raw[i], col < cols, col, row, p.out);
       }
     }
   }
 }
 
-// Any width and alignment: a warp per block, four columns per lane.
-template <int ELEM>
-__global__ void __launch_bounds__(kThreads) checkpointPackScalarKernel(const __grid_constant__ CheckpointPackLaunch p) {
-  gridDependencyPrologue();
-  const int cols = static_cast<int>(p.cols), lane = threadIdx.x & 31;
-  const int64_t blocks = (cols + kCheckpointBlock - 1) / kCheckpointBlock;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / 32);
-  for (int64_t block = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); block < p.rows * blocks; block += step) {
-    const int64_t row = block / blocks;
-    const int b = static_cast<int>(block - row * blocks);
-    float v[4][1];
-    float top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int col = b * kCheckpointBlock + i * 32 + lane;
-      v[i][0] = 0.0f;
-      if (col < cols) loadElems<ELEM, 1>(p.x.base, row * p.x.ld + col, v[i]);
-      top = fmaxf(top, finiteMagnitude(v[i][0]));
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const int e8 = checkpointExponent<ELEM>(top);
-    const CheckpointScale s = checkpointScale<ELEM>(e8);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int col = b * kCheckpointBlock + i * 32 + lane;
-      if (col >= cols) continue;
-      v[i][0] = scaledForCode(v[i][0], s);
-      p.out.codes[row * p.out.codesLd + col] = static_cast<uint8_t>(codePair(v[i][0], 0.0f) & 0xffu);
-    }
-    if (lane == 0) p.out.exps[row * p.out.expsLd + b] = static_cast<uint8_t>(e8);
-  }
-}
-
-template <int ELEM, int VEC>
+template <int ELEM, bool LOOSE>
 __global__ void __launch_bounds__(kThreads) checkpointRestoreKernel(const __grid_constant__ CheckpointRestoreLaunch p) {
   gridDependencyPrologue();
-  const int64_t perRow = p.cols / VEC;
+  constexpr int VEC = ElemOf<ELEM>::kVec;
+  const int cols = static_cast<int>(p.cols);
+  const int64_t perRow = (p.cols + VEC - 1) / VEC;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
   for (int64_t u = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; u < p.rows * perRow; u += step) {
     const int64_t row = u / perRow;
     const int col = static_cast<int>(u - row * perRow) * VEC;
-    float v[VEC];
-    loadCheckpoint<VEC>(p.in, row, col, v);
-    storeElems<ELEM, VEC>(p.out.base, row * p.out.ld + col, v);
+    if constexpr (LOOSE) {
+      float v[VEC];
+      looseCheckpoint<VEC>(p.in, row, col, cols, innerRow(row, p.rows, p.in.codesLd), v);
+      looseStore<ELEM, VEC>(p.out.base, row * p.out.ld, col, cols, v);
+    } else {
+      const uint8_t *from = p.in.codes + row * p.in.codesLd + col;
+      F2 v[VEC / 2];
+      const uint2 codes = VEC == 8 ? *reinterpret_cast<const uint2 *>(from) : make_uint2(*reinterpret_cast<const unsigned int *>(from), 0u);
+      codePairs<ELEM>(codes, p.in.exps[row * p.in.expsLd + col / kCheckpointBlock], v);
+      storePairs<ELEM>(p.out.base, row * p.out.ld + col, v);
+    }
   }
 }
 
@@ -109,18 +98,13 @@ int launchCheckpointPack(const CheckpointPackLaunch &l, cudaStream_t stream, int
   if (l.rows == 0) return 0;
   if (l.cols <= 0 || l.cols > (1ll << 30)) return cudaErrorInvalidValue;
   const int64_t eb = elemBytes(l.elemType), vec = 16 / eb;
-  const int64_t blocks = (l.cols + kCheckpointBlock - 1) / kCheckpointBlock;
   const bool vector = l.cols % vec == 0 && aligned(l.x.base, l.x.ld * eb, 16) && aligned(l.out.codes, l.out.codesLd, vec);
-  cudaError_t e;
-  if (vector) {
-    const auto kernel = l.elemType == kF32 ? checkpointPackVectorKernel<kF32> : l.elemType == kF16 ? checkpointPackVectorKernel<kF16> : checkpointPackVectorKernel<kBF16>;
-    int lanes = 32;  // the fewest (32, 64, 128 or 256) that take a row at one go
-    while (lanes < kThreads && lanes * vec * kAhead < l.cols) lanes *= 2;
-    e = launchDependent(kernel, dim3(gridFor(l.rows, kThreads / lanes)), dim3(kThreads), 0, stream, l, lanes);
-  } else {
-    const auto kernel = l.elemType == kF32 ? checkpointPackScalarKernel<kF32> : l.elemType == kF16 ? checkpointPackScalarKernel<kF16> : checkpointPackScalarKernel<kBF16>;
-    e = launchDependent(kernel, dim3(gridFor(l.rows * blocks, kThreads / 32)), dim3(kThreads), 0, stream, l);
-  }
+  const auto kernel = l.elemType == kF32   ? (vector ? checkpointPackKernel<kF32, false> : checkpointPackKernel<kF32, true>)
+                      : l.elemType == kF16 ? (vector ? checkpointPackKernel<kF16, false> : checkpointPackKernel<kF16, true>)
+                                           : (vector ? checkpointPackKernel<kBF16, false> : checkpointPackKernel<kBF16, true>);
+  int lanes = 32;  // the fewest (32, 64, 128 or 256) that take a row at one go
+  while (lanes < kThreads && lanes * vec * kAhead < l.cols) lanes *= 2;
+  const cudaError_t e = launchDependent(kernel, dim3(gridFor(l.rows, kThreads / lanes)), dim3(kThreads), 0, stream, l, lanes);
   if (e == cudaSuccess && launched) *launched += 1;
   return e;
 }
@@ -130,10 +114,10 @@ int launchCheckpointRestore(const CheckpointRestoreLaunch &l, cudaStream_t strea
   if (l.cols <= 0 || l.cols > (1ll << 30)) return cudaErrorInvalidValue;
   const int64_t eb = elemBytes(l.elemType), vec = 16 / eb;
   const bool vector = l.cols % vec == 0 && aligned(l.out.base, l.out.ld * eb, 16) && aligned(l.in.codes, l.in.codesLd, vec);
-  const auto kernel = l.elemType == kF32   ? (vector ? checkpointRestoreKernel<kF32, 4> : checkpointRestoreKernel<kF32, 1>)
-                      : l.elemType == kF16 ? (vector ? checkpointRestoreKernel<kF16, 8> : checkpointRestoreKernel<kF16, 1>)
-                                           : (vector ? checkpointRestoreKernel<kBF16, 8> : checkpointRestoreKernel<kBF16, 1>);
-  const cudaError_t e = launchDependent(kernel, dim3(gridFor(l.rows * (l.cols / (vector ? vec : 1)), kThreads)), dim3(kThreads), 0, stream, l);
+  const auto kernel = l.elemType == kF32   ? (vector ? checkpointRestoreKernel<kF32, false> : checkpointRestoreKernel<kF32, true>)
+                      : l.elemType == kF16 ? (vector ? checkpointRestoreKernel<kF16, false> : checkpointRestoreKernel<kF16, true>)
+                                           : (vector ? checkpointRestoreKernel<kBF16, false> : checkpointRestoreKernel<kBF16, true>);
+  const cudaError_t e = launchDependent(kernel, dim3(gridFor(l.rows * ((l.cols + vec - 1) / vec), kThreads)), dim3(kThreads), 0, stream, l);
   if (e == cudaSuccess && launched) *launched += 1;
   return e;
 }

@@ -152,19 +152,17 @@ template <int ELEM> __device__ __forceinline__ float largestMagnitude(const uint
     return fmaxf(ElemOf<ELEM>::widen(m.x), ElemOf<ELEM>::widen(m.y));
   }
 }
-// A vector's part of a checkpoint: the lanes of a block of 128 columns (128 / VEC neighbours, all lanes of the warp take
-// part) agree on the power, each stores its codes, the block's first the exponent.  In the ordinary case, no infinity in
+// A vector's codes: the lanes of a block of 128 columns (128 / VEC neighbours, all lanes of the warp take part) agree on the
+// power, whose exponent is returned.  In the ordinary case, no infinity in
 // the block and no magnitude that needs the highest power, a code is one product and one conversion: the power brings
 // every magnitude to 448 or less.  (f16 multiplies in f16: a product below its normal range is below the smallest code's
 // half step as well.)
-template <int ELEM>
-__device__ __forceinline__ void packVector(const uint4 &raw, bool live, int col, int64_t row, const CheckpointOut &c) {
+template <int ELEM> __device__ __forceinline__ int codesOf(const uint4 &raw, unsigned int (&codes)[ElemOf<ELEM>::kVec / 4]) {
   constexpr int VEC = ElemOf<ELEM>::kVec, kGroup = kCheckpointBlock / VEC, W = VEC / 4;
   float top = largestMagnitude<ELEM>(raw);
 #pragma unroll
   for (int o = kGroup / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   int e8 = checkpointExponent<ELEM>(top);
-  unsigned int codes[W];
   if (!__any_sync(0xffffffffu, e8 == CheckpointRange<ELEM>::kHigh)) {
     const float inverse = powerOfExponent(254 - e8);
     if constexpr (ELEM == kF16) {
@@ -203,6 +201,13 @@ __device__ __forceinline__ void packVector(const uint4 &raw, bool live, int col,
       codes[i] = codePair(scaledForCode(v[4 * i], s), scaledForCode(v[4 * i + 1], s)) |
                  (codePair(scaledForCode(v[4 * i + 2], s), scaledForCode(v[4 * i + 3], s)) << 16);
   }
+  return e8;
+}
+template <int ELEM>
+__device__ __forceinline__ void packVector(const uint4 &raw, bool live, int col, int64_t row, const CheckpointOut &c) {
+  constexpr int W = ElemOf<ELEM>::kVec / 4;
+  unsigned int codes[W];
+  const int e8 = codesOf<ELEM>(raw, codes);
   if (!live) return;
   uint8_t *to = c.codes + row * c.codesLd + col;
   if constexpr (W == 2) *reinterpret_cast<uint2 *>(to) = make_uint2(codes[0], codes[W - 1]);
