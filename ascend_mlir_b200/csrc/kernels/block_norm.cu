@@ -262,7 +262,7 @@ int launchBlockNorm(const BlockNormLaunch &l, cudaStream_t stream, int *launched
       const int ctaThreads = l.pass == kPre ? kForwardAheadThreads : kForwardAheadPostThreads, ctasPerSm = l.pass == kPre ? 2 : 1;
       s.teamsPerCta = std::max(1, std::min(15, ctaThreads / s.lanes));
       const int threads = s.lanes * s.teamsPerCta;
-      const int tensors = l.pass == kPre ? 1 : l.gateForm == kGateToken ? 3 : 2;
+      const int tensors = l.pass == kPre ? 1 : l.gateForm != kGateNone ? 3 : 2;
       const int vectors = (l.kind == kLayerNorm ? 2 : 1) * (l.pass == kPostPre ? 2 : 1);
       const size_t paramBytes = static_cast<size_t>(vectors) * static_cast<size_t>(s.lanes * s.nv * vec) * sizeof(float);
       const size_t rowBytes = static_cast<size_t>(tensors) * static_cast<size_t>(s.nv) * 16 * static_cast<size_t>(ctaThreads);

@@ -31,12 +31,12 @@ __global__ void __launch_bounds__(PASS == kPre ? kForwardAheadThreads : kForward
   bool has[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) has[i] = FULL || col0 + i * apart < cols;
-  const bool token = PASS != kPre && p.gateForm == kGateToken, grouped = PASS != kPre && p.gateForm == kGateGroup;
+  const bool gated = PASS != kPre && p.gateForm != kGateNone, grouped = PASS != kPre && p.gateForm == kGateGroup;
   const unsigned int groupRows = static_cast<unsigned int>(min(p.groupRows, static_cast<int64_t>(0x7fffffff)));
 
   constexpr unsigned int perVector = (PASS == kPre ? kForwardAheadThreads : kForwardAheadPostThreads) * 16, perTensor = NV * perVector;
   constexpr unsigned int atX = PASS == kPre ? 0 : perTensor, atGate = 2 * perTensor;
-  const unsigned int used = PASS == kPre ? perTensor : token ? 3 * perTensor : 2 * perTensor;
+  const unsigned int used = PASS == kPre ? perTensor : gated ? 3 * perTensor : 2 * perTensor;
   const unsigned int slot0 = threadIdx.x * 16, slotEnd = slot0 + stages * used;
   const unsigned int slotsAt = static_cast<unsigned int>(__cvta_generic_to_shared(slots));
   auto readSlot = [&](unsigned int at) { return *reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(slots) + at); };
@@ -44,17 +44,17 @@ __global__ void __launch_bounds__(PASS == kPre ? kForwardAheadThreads : kForward
 
   auto fetch = [&](int at, unsigned int slot) {
     if (at < rows) {
-      auto vectors = [&](unsigned int where, const RowsIn &r) {
-        const char *from = static_cast<const char *>(r.base) + (static_cast<int64_t>(at) * static_cast<int>(r.ld) + col0) * EB;  // ld < 2^24
+      auto vectors = [&](unsigned int where, const RowsIn &r, int which) {
+        const char *from = static_cast<const char *>(r.base) + (static_cast<int64_t>(which) * static_cast<int>(r.ld) + col0) * EB;  // ld < 2^24
 #pragma unroll
         for (int i = 0; i < NV; ++i)
           if (has[i]) copyAhead16(slotsAt + slot + where + i * perVector, from + i * apart * EB);
       };
       if constexpr (PASS != kPre) {
-        vectors(0, p.y);
-        if (token) vectors(atGate, p.gate);
+        vectors(0, p.y, at);
+        if (gated) vectors(atGate, p.gate, grouped ? static_cast<int>(static_cast<unsigned int>(at) / groupRows) : at);
       }
-      vectors(atX, p.x);
+      vectors(atX, p.x, at);
     }
     copiesCommit();  // an empty group where there is no row: the count stays the number of rows ahead
   };
@@ -144,17 +144,14 @@ __global__ void __launch_bounds__(PASS == kPre ? kForwardAheadThreads : kForward
     storeStatistics(team, PASS == kPre ? p.statsB : p.statsA, row, mean, rstd);
     if constexpr (PASS != kPre) {
       const F2 shift = splat(-mean), r = splat(rstd), alpha = splat(p.alpha);
-      const void *gateRow = nullptr;
-      if (grouped)
-        gateRow = static_cast<const char *>(p.gate.base) + (static_cast<int64_t>(static_cast<unsigned int>(row) / groupRows) * static_cast<int>(p.gate.ld) + col0) * EB;
       char *to = rowTo(p.out);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         if (!has[i]) continue;
         normed(v[i], i, shift, r, weightA, biasA);
         F2 t[P];
-        if (token || grouped) {
-          widenPairs<ELEM>(token ? readSlot(slot + atGate + i * perVector) : *reinterpret_cast<const uint4 *>(static_cast<const char *>(gateRow) + i * apart * EB), t);
+        if (gated) {
+          widenPairs<ELEM>(readSlot(slot + atGate + i * perVector), t);
           gatePairs(t, p.gateAct);
 #pragma unroll
           for (int e = 0; e < P; ++e) v[i][e] = v[i][e] * t[e];
