@@ -111,7 +111,7 @@ struct Team {
   int half;
 };
 constexpr int kTeamValues = 3;
-constexpr int kTeamSlice = 64;  // floats per value: the CTA's warps, each team's rounded up to 16 bytes
+constexpr int kTeamSlice = 64;  // floats per value: the CTA's warps, each team's rounded up to 4, 8 or 16
 constexpr int kTeamScratchFloats = 2 * kTeamValues * kTeamSlice;
 
 __device__ __forceinline__ void teamBarrier(const Team &t) { asm volatile("bar.sync %0, %1;" ::"r"(t.index + 1), "r"(t.lanes) : "memory"); }
@@ -122,7 +122,7 @@ __device__ __forceinline__ Team makeTeam(int lanes, float *scratch) {
   t.index = static_cast<int>(threadIdx.x) / lanes;
   t.lane = static_cast<int>(threadIdx.x) - t.index * lanes;
   t.count = static_cast<int>(blockDim.x) / lanes;
-  const int slice = ((lanes >> 5) + 3) & ~3;
+  const int warps = lanes >> 5, slice = warps <= 4 ? 4 : warps <= 8 ? 8 : 16;
   t.scratch = scratch + t.index * slice;
   t.half = 0;
   if (lanes > 32) {
@@ -138,13 +138,6 @@ __device__ __forceinline__ float warpSum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
-}
-// The warps' values of one kind, four at a time.
-template <class F> __device__ __forceinline__ void eachFourWarps(const Team &t, F f) {
-  const int warps = t.lanes >> 5;
-#pragma unroll
-  for (int w = 0; w < 16; w += 4)
-    if (w < warps) f(w);
 }
 template <int N> __device__ __forceinline__ void teamSum(Team &t, float (&v)[N]) {
   static_assert(N <= kTeamValues, "the buffer holds that many values per warp");

@@ -66,37 +66,19 @@ __device__ __forceinline__ void pairStatistics(Team &team, const F2 (&v)[NV][kPa
         if (!full) buf[2 * kTeamSlice + w] = mine;
       }
       teamBarrier(team);
-      float total = 0.0f;
-      eachFourWarps(team, [&](int w) {
-        const float4 f = *reinterpret_cast<const float4 *>(buf + w);
-        total += (f.x + f.y) + (f.z + f.w);
-      });
-      mean = total * share;
-      squares = 0.0f;
-      if (full) {
-        float apart = 0.0f;  // what the warps' means differ by
-        eachFourWarps(team, [&](int w) {
-          const float4 f = *reinterpret_cast<const float4 *>(buf + w), g = *reinterpret_cast<const float4 *>(buf + kTeamSlice + w);
-          const float sums[4] = {f.x, f.y, f.z, f.w};
-          squares += (g.x + g.y) + (g.z + g.w);
+      // each warp joins the warps' sums in a shuffle tree over the next power of two of them
+      const int warps = team.lanes >> 5, tree = warps <= 2 ? 2 : warps <= 4 ? 4 : warps <= 8 ? 8 : 16;
+      const int w = threadIdx.x & (tree - 1);
+      const float sw = buf[w], count = full ? (w < warps ? static_cast<float>(NV * 32 * VEC) : 0.0f) : buf[2 * kTeamSlice + w];
+      auto treeSum = [&](float t) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float off = w + j < (team.lanes >> 5) ? fmaf(sums[j], kWhole, -mean) : 0.0f;
-            apart = fmaf(off, off, apart);
-          }
-        });
-        squares = fmaf(apart, static_cast<float>(NV * 32 * VEC), squares);
-      } else {
-        eachFourWarps(team, [&](int w) {
-          const float4 f = *reinterpret_cast<const float4 *>(buf + w), g = *reinterpret_cast<const float4 *>(buf + kTeamSlice + w),
-                       n = *reinterpret_cast<const float4 *>(buf + 2 * kTeamSlice + w);
-          auto join = [&](float sum, float square, float count) {  // the same quotient as the warp's centre
-            const float off = __fdividef(sum, fmaxf(count, 1.0f)) - mean;
-            return fmaf(count * off, off, square);
-          };
-          squares += (join(f.x, g.x, n.x) + join(f.y, g.y, n.y)) + (join(f.z, g.z, n.z) + join(f.w, g.w, n.w));
-        });
-      }
+        for (int o = 8; o > 0; o >>= 1)
+          if (o < tree) t += __shfl_xor_sync(0xffffffffu, t, o);
+        return t;
+      };
+      mean = treeSum(sw) * share;
+      const float off = (full ? sw * kWhole : __fdividef(sw, fmaxf(count, 1.0f))) - mean;  // the same quotient as the warp's centre
+      squares = treeSum(fmaf(count * off, off, buf[kTeamSlice + w]));
     }
     rstd = rsqrtf(squares * share + eps);
   }
