@@ -35,22 +35,39 @@ constexpr int kFinishThreads = 512;
 
 __device__ __forceinline__ float4 plus(const float4 &a, const float4 &b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
 
-// Four columns per thread; a CTA is blockDim.x of them by blockDim.y slots.  Adds the slots' values over each run of
-// `slots` neighbouring slots (a power of two) in a tree; the first slot of a run gets the sums.
-template <int VALUES> __device__ __forceinline__ void slotSums(float4 (&v)[VALUES], float4 (*buf)[kFinishThreads], int slots) {
-  const int s = threadIdx.y, width = blockDim.x, at = s * width + threadIdx.x;
+// Four columns per thread.  A warp is QUADS of them (lane % QUADS) by 32 / QUADS slots, a CTA 16 such warps, and slots are
+// numbered through the warps.  Adds the slots' values over each run of `slots` neighbouring slots (a power of two): shuffles
+// inside a warp, then shared memory across the run's warps.  The first slot of a run gets the sums.
+template <int VALUES, int QUADS> __device__ __forceinline__ void slotSums(float4 (&v)[VALUES], float4 (*buf)[kFinishThreads / 32 * QUADS], int slots) {
+  constexpr int kPerWarp = 32 / QUADS;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll
-  for (int k = 0; k < VALUES; ++k) buf[k][at] = v[k];
-  __syncthreads();
-  for (int o = slots / 2; o > 0; o >>= 1) {
-    if ((s & (slots - 1)) < o) {
+  for (int o = 1; o < kPerWarp; o *= 2) {
+    if (o >= slots) break;
 #pragma unroll
-      for (int k = 0; k < VALUES; ++k) buf[k][at] = plus(buf[k][at], buf[k][at + o * width]);
+    for (int k = 0; k < VALUES; ++k) {
+      float4 other;
+      other.x = __shfl_xor_sync(0xffffffffu, v[k].x, o * QUADS);
+      other.y = __shfl_xor_sync(0xffffffffu, v[k].y, o * QUADS);
+      other.z = __shfl_xor_sync(0xffffffffu, v[k].z, o * QUADS);
+      other.w = __shfl_xor_sync(0xffffffffu, v[k].w, o * QUADS);
+      v[k] = plus(v[k], other);
     }
-    __syncthreads();
   }
+  if (slots <= kPerWarp) return;
+  const int warps = slots / kPerWarp;
+  if (lane < QUADS) {
 #pragma unroll
-  for (int k = 0; k < VALUES; ++k) v[k] = buf[k][at];
+    for (int k = 0; k < VALUES; ++k) buf[k][warp * QUADS + lane] = v[k];
+  }
+  __syncthreads();
+  if (lane < QUADS && warp % warps == 0) {
+#pragma unroll
+    for (int k = 0; k < VALUES; ++k) {
+#pragma unroll 4
+      for (int w = 1; w < warps; ++w) v[k] = plus(v[k], buf[k][(warp + w) * QUADS + lane]);
+    }
+  }
   __syncthreads();
 }
 
@@ -68,12 +85,15 @@ __device__ __forceinline__ void addRows(const float *sums, int64_t sumsLd, int64
 
 // Slots share the rows of sums; the order in which they are added depends on the sizes alone.  Columns between `cols` and
 // sumsLd are read (they are in the workspace) and not stored.
-template <int VALUES> __global__ void __launch_bounds__(kFinishThreads) blockNormFinishKernel(const __grid_constant__ FinishParams p) {
+template <int VALUES, int QUADS> __global__ void __launch_bounds__(kFinishThreads) blockNormFinishKernel(const __grid_constant__ FinishParams p) {
   gridDependencyPrologue();
-  __shared__ float4 buf[VALUES][kFinishThreads];
-  const int64_t col = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * 4;
+  constexpr int allSlots = kFinishThreads / QUADS;
+  __shared__ float4 buf[VALUES][kFinishThreads / 32 * QUADS];
+  const int64_t col = (static_cast<int64_t>(blockIdx.x) * QUADS + threadIdx.x % QUADS) * 4;
   const bool live = col < p.cols;
-  const int slot = threadIdx.y, allSlots = blockDim.y;
+  const int slot = threadIdx.x / QUADS;
+  float4 next[VALUES];  // normB's, asked for before normA's are waited for
+  if (p.sumsB) addRows<VALUES>(p.sumsB + col, p.sumsLd, slot, allSlots, live ? p.teams : 0, next);
   if (p.sumsA) {
     // slots as (groups at once) x (slots per group)
     int atOnce = 1;
@@ -95,7 +115,7 @@ template <int VALUES> __global__ void __launch_bounds__(kFinishThreads) blockNor
       const bool mine = live && group < p.groups;
       float4 s[VALUES];
       addRows<VALUES>(p.sumsA + group * p.chunks * VALUES * p.sumsLd + col, p.sumsLd, slot & (perGroup - 1), perGroup, mine ? p.chunks : 0, s);
-      if (perGroup > 1) slotSums<VALUES>(s, buf, perGroup);
+      slotSums<VALUES, QUADS>(s, buf, perGroup);
       if (mine && (slot & (perGroup - 1)) == 0) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -115,7 +135,7 @@ template <int VALUES> __global__ void __launch_bounds__(kFinishThreads) blockNor
         }
       }
     }
-    if (p.groups > 1) slotSums<VALUES>(total, buf, allSlots);
+    if (p.groups > 1) slotSums<VALUES, QUADS>(total, buf, allSlots);
     if (live && slot == 0) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -128,15 +148,13 @@ template <int VALUES> __global__ void __launch_bounds__(kFinishThreads) blockNor
     }
   }
   if (p.sumsB) {
-    float4 s[VALUES];
-    addRows<VALUES>(p.sumsB + col, p.sumsLd, slot, allSlots, live ? p.teams : 0, s);
-    slotSums<VALUES>(s, buf, allSlots);
+    slotSums<VALUES, QUADS>(next, buf, allSlots);
     if (live && slot == 0) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (col + j >= p.cols) break;
-        p.nextWeight[col + j] = reinterpret_cast<const float *>(&s[0])[j];
-        if (p.nextBias) p.nextBias[col + j] = reinterpret_cast<const float *>(&s[VALUES - 1])[j];
+        p.nextWeight[col + j] = reinterpret_cast<const float *>(&next[0])[j];
+        if (p.nextBias) p.nextBias[col + j] = reinterpret_cast<const float *>(&next[VALUES - 1])[j];
       }
     }
   }
@@ -375,10 +393,11 @@ int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *
   f.dgate = static_cast<float *>(l.gateForm == kGateGroup ? l.dgate.base : nullptr);
   f.dgateLd = l.dgate.ld;
   // whole 128-byte lines of the sums (8 threads of 4 columns) for wide rows, half lines and twice the slots else
-  const int width = l.cols >= 4096 ? 8 : 4;
-  const unsigned int grid = static_cast<unsigned int>((l.cols + 4 * width - 1) / (4 * width));
-  const auto finish = f.layer ? blockNormFinishKernel<2> : blockNormFinishKernel<1>;
-  const cudaError_t e = launchDependent(finish, dim3(grid), dim3(static_cast<unsigned int>(width), static_cast<unsigned int>(kFinishThreads / width)), 0, stream, f);
+  const int quads = l.cols >= 4096 ? 8 : 4;
+  const unsigned int grid = static_cast<unsigned int>((l.cols + 4 * quads - 1) / (4 * quads));
+  const auto finish = f.layer ? (quads == 8 ? blockNormFinishKernel<2, 8> : blockNormFinishKernel<2, 4>)
+                              : (quads == 8 ? blockNormFinishKernel<1, 8> : blockNormFinishKernel<1, 4>);
+  const cudaError_t e = launchDependent(finish, dim3(grid), dim3(kFinishThreads), 0, stream, f);
   if (e == cudaSuccess && launched) *launched += 1;
   return e;
 }
