@@ -84,7 +84,9 @@ __device__ __forceinline__ void addRows(const float *sums, int64_t sumsLd, int64
 }
 
 // Slots share the rows of sums; the order in which they are added depends on the sizes alone.  Columns between `cols` and
-// sumsLd are read (they are in the workspace) and not stored.
+// sumsLd are read (they are in the workspace) and not stored.  The sums are in L2 (the row kernel has just written them) and
+// what counts is how many loads a slot has one behind the other: 148 teams' rows of 8192 columns, two norms, 8.1 us; 592
+// teams' of 1024 columns and 8 groups of gates, 13.3 us.
 template <int VALUES, int QUADS> __global__ void __launch_bounds__(kFinishThreads) blockNormFinishKernel(const __grid_constant__ FinishParams p) {
   gridDependencyPrologue();
   constexpr int allSlots = kFinishThreads / QUADS;
@@ -174,20 +176,22 @@ TeamShape shapeOf(int vec, int nv, int64_t cols) {
   return s;
 }
 
-// A team has at most 512 threads.  Few rows: one vector per thread while that is enough, for the shortest way through one
-// row; else 16 columns per thread.
-TeamShape forwardShape(int elemType, int64_t rows, int64_t cols, int smCount) {
+// A CTA per team's row.  One vector per thread while 512 threads are enough, for the shortest way through one row (296 rows of
+// 4096 bf16 behind a block: 10.4 us, 12.3 with two); 16 columns per thread where many rows have little to do each: before a
+// block (592 rows: 8.2 us, 10.3 with one vector), or in shifted pieces.
+TeamShape forwardShape(int elemType, int pass, bool vector, int64_t rows, int64_t cols, int smCount) {
   const int vec = elemType == kF32 ? 4 : 8;
-  const int64_t perThread = rows >= smCount ? 16 : vec;
+  const int64_t perThread = rows >= 2 * smCount && (pass == kPre || !vector) ? 16 : vec;
   int nv = 1;
   while (nv * vec < perThread && static_cast<int64_t>(nv) * vec * 32 < cols) nv *= 2;
   while (static_cast<int64_t>(nv) * vec * 512 < cols) nv *= 2;
   return shapeOf(vec, nv, cols);
 }
 
-// The gradient with rows fetched ahead, 512 threads per SM: two vectors per thread (one of a 16-bit layer norm, which keeps
-// twice the column sums in registers), in a team of up to 512 threads, beyond that what the width needs; fewer where
-// that makes every thread's vectors lie inside the row, which spares the kernel its tests.
+// The gradient with rows fetched ahead, 512 threads per SM: two vectors per thread, which share a row's scalars and sums (8192 x
+// 4096 f16 rms: 110 us, 136 with one), one of a 16-bit layer norm, whose column sums are twice as many registers (151 us, 712
+// with two: they spill), in a team of up to 512 threads; beyond that what the width needs; fewer where that makes every thread's
+// vectors lie inside the row, which spares the kernel its tests.
 TeamShape gradShape(int elemType, int kind, int64_t cols) {
   const int vec = elemType == kF32 ? 4 : 8;
   int nv = kind == kLayerNorm && elemType != kF32 ? 1 : 2;
@@ -223,8 +227,8 @@ GradPlan gradPlan(int elemType, int kind, int gateForm, int64_t rows, int64_t co
   const int64_t all = std::max<int64_t>(rows, 1);
   const int64_t perGroup = gateForm == kGateGroup ? std::min(groupRows, all) : all;
   const int64_t groups = gateForm == kGateGroup ? (rows + perGroup - 1) / perGroup : 1;
-  // As many teams as an SM holds: enough rows under
-  // way to cover a row's two sums, few enough that the teams' sums (f32, one or two rows each) stay small beside the rows.
+  // As many teams as an SM holds: enough rows under way to cover a row's two sums, few enough that the teams' sums (f32, one
+  // or two rows each) stay small beside the rows.
   const int64_t teams = std::max<int64_t>(1, std::min<int64_t>(rows, smCount * gradTeamsPerSm(elemType, kind, cols)));
   const int64_t wanted = std::max<int64_t>(1, groups ? teams / groups : 1);
   const int64_t chunkRows = (perGroup + wanted - 1) / wanted;
@@ -271,9 +275,11 @@ int launchBlockNorm(const BlockNormLaunch &l, cudaStream_t stream, int *launched
   int device = 0;
   if (const cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return e;
   const int sms = deviceSmCount(device);
-  // Rows fetched ahead by teams that stay, where every team gets several rows and two fit in shared memory beside the
+  // Rows fetched ahead by teams that stay, where every team gets two rows or more and two fit in shared memory beside the
   // parameters: 1024 threads per SM (64 registers each) before a block, up to 768 (80 registers) behind it, in one CTA that
-  // shares its parameters.
+  // shares its parameters.  Two rows each (888 x 4096 f16 layer, behind a block): 20.5 us, 24.6 without; eight: 41 and 67; before
+  // a block, 4096 bf16 rms, two, four and sixteen: 11.2, 18.4 and 41 us, 12.3, 20.5 and 55 without; one row each gains nothing,
+  // and few teams' set-up costs 2 us.
   if (vector) {
     TeamShape s = gradShape(l.elemType, kRmsNorm, l.cols);
     if (s.nv <= 2) {
@@ -286,7 +292,7 @@ int launchBlockNorm(const BlockNormLaunch &l, cudaStream_t stream, int *launched
       const size_t rowBytes = static_cast<size_t>(tensors) * static_cast<size_t>(s.nv) * 16 * static_cast<size_t>(ctaThreads);
       const size_t perCta = kAheadBytes / static_cast<size_t>(ctasPerSm) - 1536;
       const int stages = static_cast<int>(std::min<size_t>(4, (perCta - std::min(perCta, paramBytes)) / rowBytes));
-      if (stages >= 2 && l.rows >= static_cast<int64_t>(4) * sms * ctasPerSm * s.teamsPerCta) {
+      if (stages >= 2 && l.rows >= static_cast<int64_t>(2) * sms * ctasPerSm * s.teamsPerCta) {
         const bool full = static_cast<int64_t>(s.lanes) * s.nv * vec == l.cols;
         const ForwardAheadKernel kernel = l.elemType == kF32   ? forwardAheadKernel<kF32>(l.kind, l.pass, full, s.nv)
                                           : l.elemType == kF16 ? forwardAheadKernel<kF16>(l.kind, l.pass, full, s.nv)
@@ -300,7 +306,7 @@ int launchBlockNorm(const BlockNormLaunch &l, cudaStream_t stream, int *launched
       }
     }
   }
-  const TeamShape s = forwardShape(l.elemType, l.rows, l.cols, sms);
+  const TeamShape s = forwardShape(l.elemType, l.pass, vector, l.rows, l.cols, sms);
   const ForwardKernel kernel = l.elemType == kF32   ? forwardKernel<kF32>(l.kind, l.pass, vector, s.nv)
                                : l.elemType == kF16 ? forwardKernel<kF16>(l.kind, l.pass, vector, s.nv)
                                                     : forwardKernel<kBF16>(l.kind, l.pass, vector, s.nv);
@@ -392,7 +398,8 @@ int launchBlockNormGrad(const BlockNormGradLaunch &l, cudaStream_t stream, int *
   f.nextBias = l.db.bias;
   f.dgate = static_cast<float *>(l.gateForm == kGateGroup ? l.dgate.base : nullptr);
   f.dgateLd = l.dgate.ld;
-  // whole 128-byte lines of the sums (8 threads of 4 columns) for wide rows, half lines and twice the slots else
+  // whole 128-byte lines of the sums (8 threads of 4 columns) for wide rows, half lines, twice the slots and CTAs else (whole
+  // gradient, 8192 columns: 186 us, 189 with half lines; 1024 columns: 36 us, 40 with whole ones)
   const int quads = l.cols >= 4096 ? 8 : 4;
   const unsigned int grid = static_cast<unsigned int>((l.cols + 4 * quads - 1) / (4 * quads));
   const auto finish = f.layer ? (quads == 8 ? blockNormFinishKernel<2, 8> : blockNormFinishKernel<2, 4>)

@@ -74,13 +74,7 @@ template <int ELEM, int VEC> __device__ __forceinline__ void loadElems(const voi
   if constexpr (VEC == 1) v[0] = ElemOf<ELEM>::widen(*q);
   else unpack<ELEM, VEC>(*reinterpret_cast<const uint4 *>(q), v);
 }
-template <int ELEM, int VEC> __device__ __forceinline__ void storeElems(void *p, int64_t at, const float (&v)[VEC]) {
-  using T = typename ElemOf<ELEM>::Type;
-  T *q = static_cast<T *>(p) + at;
-  if constexpr (VEC == 1) *q = ElemOf<ELEM>::narrow(v[0]);
-  else *reinterpret_cast<uint4 *>(q) = pack<ELEM, VEC>(v);
-}
-// A parameter vector: of the rows' type or f32 (uniform over the launch); it stays in L1 from row to row.
+// A parameter vector, or one parameter: of the rows' type or f32 (uniform over the launch); it stays in L1 from row to row.
 template <int ELEM, int VEC> __device__ __forceinline__ void loadParam(const void *p, int type, int at, float (&v)[VEC]) {
   if (ELEM == kF32 || type != kF32) {
     loadElems<ELEM, VEC>(p, at, v);
@@ -103,8 +97,9 @@ template <int ELEM, int VEC> __device__ __forceinline__ void loadParam(const voi
 // `lanes` threads (a multiple of 32, at most 512) that hold one row; a CTA of up to 1024 threads has one or more of them
 // (at most 15 of more than a warp: each has a named barrier).  Sums over a team: a shuffle tree in each warp, then the
 // warps' sums through shared memory, which every thread of up to 8 warps adds up itself in the same order (a second shuffle
-// tree would be five more dependent latencies); of more warps, each warp adds them in a shuffle tree.  The two halves of the buffer alternate, so one barrier per sum is enough: whoever writes
-// a half again has passed the barrier of the sum between, which every reader of that half reached after reading.
+// tree would be five more dependent latencies); of more warps, each warp adds them in a shuffle tree.  The two halves of the
+// buffer alternate, so one barrier per sum is enough: whoever writes a half again has passed the barrier of the sum between,
+// which every reader of that half reached after reading.
 struct Team {
   int lanes, lane, index, count;  // threads in it; this thread's place; which of the CTA's; how many the CTA has
   float *scratch;                 // this team's slice of the CTA's buffer: [halves][kTeamValues][slice], zero beyond its warps
@@ -212,20 +207,17 @@ __device__ __forceinline__ float2 valuePair(unsigned int codes, float power) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
   return make_float2(f.x * power, f.y * power);
 }
-template <int VEC> __device__ __forceinline__ void valuesOfCodes(const unsigned int (&w)[VEC / 4 > 0 ? VEC / 4 : 1], float power, float (&v)[VEC]) {
-  if constexpr (VEC == 1) {
-    v[0] = valuePair(w[0] & 0xffu, power).x;
-  } else {
+template <int VEC> __device__ __forceinline__ void valuesOfCodes(const unsigned int (&w)[VEC / 4], float power, float (&v)[VEC]) {
 #pragma unroll
-    for (int i = 0; i < VEC / 4; ++i) {
-      const float2 lo = valuePair(w[i] & 0xffffu, power), hi = valuePair(w[i] >> 16, power);
-      v[4 * i] = lo.x;
-      v[4 * i + 1] = lo.y;
-      v[4 * i + 2] = hi.x;
-      v[4 * i + 3] = hi.y;
-    }
+  for (int i = 0; i < VEC / 4; ++i) {
+    const float2 lo = valuePair(w[i] & 0xffffu, power), hi = valuePair(w[i] >> 16, power);
+    v[4 * i] = lo.x;
+    v[4 * i + 1] = lo.y;
+    v[4 * i + 2] = hi.x;
+    v[4 * i + 3] = hi.y;
   }
 }
+
 // ---- the gate ---------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float gateValue(float g, int act) {
   if (act == kActSigmoid) return 1.0f / (1.0f + expf(-g));

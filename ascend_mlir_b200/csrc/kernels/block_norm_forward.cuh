@@ -65,7 +65,9 @@ __device__ __forceinline__ void storeStatistics(const Team &team, const NormStat
   if (s.mean) s.mean[row] = mean;
 }
 
-// Any width and alignment (loose.cuh).
+// Any width and alignment (loose.cuh).  Bound by instructions: the shifts, and the tests at a row's end.  8000 x 4001 bf16 rms
+// with a checkpoint 73 us (2.2 TB/s), gated f16 layer 172 us; aligned 8192 x 4096 rows take 66 us here and 37 in
+// block_norm_forward_ahead.cuh.
 template <int ELEM, int KIND, int PASS, int NV>
 __global__ void __launch_bounds__(512) blockNormForwardKernel(const __grid_constant__ BlockNormLaunch p, int teamLanes) {
   gridDependencyPrologue();

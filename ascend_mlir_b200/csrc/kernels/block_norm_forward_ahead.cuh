@@ -4,6 +4,10 @@
 // CTA) as two or three vectors do, and a kernel that starts a team for every row was bound by them.  Here a team walks
 // every teams-th row with its set-up done once, its parameters in shared memory as f32 (scale folded into normA's), and the
 // next rows arriving in slots of its threads (as in block_norm_grad_vector.cuh) while it sums.
+//
+// Measured: 8192 x 4096 bf16 rms with a checkpoint 32.7 us (168 MB, 5.1 TB/s: 78 % of a plain copy's rate; starts and last
+// rows count at this size); 16384 x 4096 f16 layer, a gate row per sequence, both norms, 121 us (537 MB, 4.4 TB/s): bound by
+// instruction issue (2.3 per cycle) and the shared memory that rows and parameters come from.
 #pragma once
 
 #include "kernels/block_norm_forward_vector.cuh"

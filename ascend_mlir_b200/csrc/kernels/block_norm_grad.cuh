@@ -33,7 +33,9 @@ struct GradPlan {
 };
 
 // Any width and alignment (loose.cuh); aligned rows too that are too wide for block_norm_grad_vector.cuh.  Elements beyond
-// the row are zeros, as are the parameters read for them, so they add nothing to a row's sums; they are not stored.
+// the row are zeros, as are the parameters read for them, so they add nothing to a row's sums; they are not stored.  A row's
+// loads are waited for one after the other and the arithmetic is not paired: 8000 x 4001 from a bf16 checkpoint 183 us (1.3
+// TB/s), gated f16 rms 435 us; aligned 8192 x 8192 rows take 677 us here, 185 with rows fetched ahead.
 template <int ELEM, int KIND, int PASS, int NV>
 __global__ void __launch_bounds__(512) blockNormGradKernel(const __grid_constant__ BlockNormGradLaunch p, const __grid_constant__ GradPlan plan,
                                                            int teamLanes) {

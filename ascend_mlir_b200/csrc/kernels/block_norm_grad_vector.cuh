@@ -3,8 +3,13 @@
 // A row of the longest form is five tensors in and three out, so a team that loads when it needs the data leaves HBM
 // idle while it sums.  Here every thread fetches its vectors two to four rows ahead into slots of its own in shared
 // memory (cp.async), so a row's sums run while the next rows arrive.  The parameter vectors are kept there too: beside the
-// rows they would not stay in what is left of the L1 (15 % hits), and every pass would wait for L2.  The arithmetic is done on pairs of f32
-// (fma.rn.f32x2): at 8192 bf16 columns the plain form needs as many issue cycles as HBM needs time.
+// rows they would not stay in what is left of the L1 (15 % hits), and every pass would wait for L2.  The arithmetic is done on
+// pairs of f32 (fma.rn.f32x2): at 8192 bf16 columns the plain form needs as many issue cycles as HBM needs time.
+//
+// Measured without the joining kernel: 8192 x 8192 bf16 rms, a gate per element, both norms 174 us (1.07 GB, 6.2 TB/s: 94 % of a
+// plain copy's rate); 8192 x 4096 bf16 rms from a checkpoint 42 us (235 MB, 5.6 TB/s); 4096 x 1024 f16 layer, a gate row per
+// sequence 21.5 us (50 MB): seven rows per team, start-up and the column sums, which are a third of the bytes;
+// 1023 x 1000 f32 layer 8.5 us.
 #pragma once
 
 #include "kernels/block_norm_grad.cuh"

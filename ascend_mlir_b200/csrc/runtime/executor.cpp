@@ -577,9 +577,12 @@ Status CudaExecutor::launchDevice(const RunRequest &req, void *workspace, size_t
     if (isOperatorClass(desc->kernelClass) && wsBytes > kWorkspaceStatusBytes)
       return Status::error("[cuda:memory] kernel '" + desc->kernel + "' needs a workspace of " + std::to_string(wsBytes) +
                            " bytes from the caller at these sizes");
-    if (Status s = ownWorkspace(wsBytes); !s) return s.withStage("cuda:memory");
-    args.workspace = workspace_.ptr;
-    args.workspaceBytes = workspace_.capacity;
+    // (forward row passes and checkpoints need none at all: nothing is allocated, so a first launch can be captured)
+    if (desc->kernelClass != KernelClass::BlockNorm && desc->kernelClass != KernelClass::Checkpoint) {
+      if (Status s = ownWorkspace(wsBytes); !s) return s.withStage("cuda:memory");
+      args.workspace = workspace_.ptr;
+      args.workspaceBytes = workspace_.capacity;
+    }
   }
   const bool trace = launchTraceEnabled();  // the environment is read once per launch
   if (trace) printLaunchTrace(req, *desc, args, device_, "device");

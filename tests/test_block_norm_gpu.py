@@ -365,6 +365,24 @@ def test_same_bits_again_and_in_a_graph(rt):
     assert all(torch.equal(outs[k], fresh[k]) for k in first)
 
 
+def test_first_launch_of_an_executor_in_a_capture(rt):
+    """A forward pass without a workspace allocates nothing, so an executor's very first launch can be captured."""
+    c = case("gated", 37, 512, "bf16", "rms", gate="token", act="sigmoid", next=True)
+    t = block_inputs(c, 9)
+    spec = descriptors.gated_residual("bf16", gate="token", gate_act="sigmoid", next_norm=True, save_stats=False)
+    want = call(rt, spec, sizes(c), t)
+    outs = outputs_for(spec, sizes(c), torch.device("cuda"), 3)
+    new = CudaRuntime()
+    new.set_device(0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a, b = arguments(spec, t, outs)
+        new.launch_device(spec.binary, spec.name, a, b, spec.pack(sizes(c)), 0, spec.magic, (0, 0), torch.cuda.current_stream().cuda_stream)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(outs[k], want[k]) for k in outs)
+
+
 def test_two_streams_at_once(rt):
     c = case("gated", 900, 2048, "bf16", "rms", gate="token", act="sigmoid", next=True)
     spec = descriptors.gated_residual_grad("bf16", gate="token", gate_act="sigmoid", next_norm=True)
