@@ -558,6 +558,8 @@ Status CudaExecutor::launchDevice(const RunRequest &req, void *workspace, size_t
   args.exchange = exchange;
   args.tableShards = tableShards;
   args.rowsPerShard = rowsPerShard;
+  args.argPtrs.reserve(static_cast<size_t>(req.numInputs + req.numOutputs));
+  args.argBytes.reserve(static_cast<size_t>(req.numInputs + req.numOutputs));
   for (int i = 0; i < req.numInputs; ++i) {
     args.argPtrs.push_back(const_cast<void *>(req.inputPtrs[i]));
     args.argBytes.push_back(req.inputBytes[i]);

@@ -43,8 +43,15 @@ def _words(n: int) -> struct.Struct:
     return struct.Struct(f"{n}Q")
 
 
-def _addresses(values: Sequence[int]) -> bytes:
-    return _words(len(values)).pack(*values)
+def _packed(args: Sequence[Tuple[int, int]]) -> Tuple[bytes, bytes]:
+    """The addresses and the sizes of (address, nbytes) pairs as two arrays of 64-bit words."""
+    if not args:
+        return b"", b""
+    addresses, sizes = zip(*args)
+    pack = _words(len(sizes)).pack
+    if None in addresses:
+        addresses = [p or 0 for p in addresses]
+    return pack(*addresses), pack(*sizes)
 
 
 @functools.lru_cache(maxsize=None)
@@ -151,9 +158,10 @@ class CudaRuntime:
             err = _error_buffer()
             binary = binary_data if type(binary_data) is bytes else bytes(binary_data or b"")
             tiling = tiling_data if type(tiling_data) is bytes else bytes(tiling_data or b"")
+            in_addresses, in_sizes = _packed(inputs)
+            out_addresses, out_sizes = _packed(outputs)
             ret = _launch_fast()(self._handle, binary or None, len(binary), function_name.encode(),
-                                 len(inputs), _addresses([p or 0 for p, _ in inputs]), _addresses([n for _, n in inputs]),
-                                 len(outputs), _addresses([p or 0 for p, _ in outputs]), _addresses([n for _, n in outputs]),
+                                 len(inputs), in_addresses, in_sizes, len(outputs), out_addresses, out_sizes,
                                  tiling or None, len(tiling), block_dim, magic,
                                  workspace[0], workspace[1], stream, err, len(err))
             if ret != 0:
