@@ -642,6 +642,48 @@ def test_rows_behind_the_last_stay(rt):
     check(dict(outs, dgate=outs["dgate"][:3]), want)
 
 
+@pytest.mark.parametrize("D,ld,first", [(64, 16384, 128), (63, 16385, 129)])
+def test_offsets_beyond_32_bits(rt, D, ld, first):
+    """Column ranges of a tensor of 2.4e9 elements: the same bits as from dense rows, and nothing beside them is written."""
+    T = 150000
+    c = case("gated", T, D, "bf16", "layer", gate="token", act="sigmoid", next=True)
+    t = block_inputs(c, 17)
+    options = dict(kind="layer", gate="token", gate_act="sigmoid", next_norm=True)
+    big, codes = torch.zeros(T, ld, dtype=torch.bfloat16, device="cuda"), torch.zeros(T, ld, dtype=torch.uint8, device="cuda")
+
+    def compare(build, names, inputs):
+        """`names`: the row tensors, each a column range of `big` (codes: of `codes`), 128 columns apart."""
+        want = call(rt, build(), sizes(c), inputs)
+        spec = build(strided=names)
+        at = {n: first + 128 * i for i, n in enumerate(names)}
+        w, outs = dict(inputs), {k: torch.full_like(v, 3) for k, v in want.items() if k != "_workspace"}
+        for n in names:
+            whole = codes if n == "codes" else big
+            whole[:, at[n]:at[n] + D] = inputs[n] if n in inputs else 3
+            (w if n in inputs else outs)[n] = whole
+        call(rt, spec, dict(sizes(c), **{f"LD_{n}": ld for n in names}, **{f"OFF_{n}": at[n] for n in names}), w, outs)
+        torch.cuda.synchronize()
+        for k in want:
+            if k != "_workspace":
+                got = outs[k][:, at[k]:at[k] + D] if k in names else outs[k]
+                assert torch.equal(got, want[k]), k
+        for n in names:
+            whole = codes if n == "codes" else big
+            assert not whole[:, at[n] + D:at[n] + 128].any() and not whole[:, at[n] - 1].any(), n
+        for n in names:
+            (codes if n == "codes" else big)[:, at[n]:at[n] + D] = 0
+        return want
+
+    done = compare(lambda **k: descriptors.gated_residual("bf16", checkpoint=True, **options, **k), ("x", "y", "gate", "out", "h", "codes"),
+                   {k: t[k] for k in ("x", "y", "gate", "weight", "bias", "scale", "next_weight", "next_bias")})
+    w = {k: t[k] for k in ("dout", "dh", "gate", "weight", "bias", "scale", "next_weight")}
+    w.update({k: done[k] for k in ("codes", "exps", "rstd", "mean", "out", "next_rstd", "next_mean")})
+    compare(lambda **k: descriptors.gated_residual_grad("bf16", checkpoint=True, **options, **k),
+            ("dout", "codes", "gate", "dh", "out", "dx", "dy", "dgate"), w)
+    compare(lambda **k: descriptors.checkpoint_pack("bf16", **k), ("x", "codes"), {"x": t["x"]})
+    compare(lambda **k: descriptors.checkpoint_restore("bf16", **k), ("codes", "x"), {k: done[k] for k in ("codes", "exps")})
+
+
 def test_current_device_and_stream_order(rt):
     """A launch on a side stream after its inputs were made there; the caller's device stays the current one."""
     c = case("norm", 2000, 512, "bf16", "rms")

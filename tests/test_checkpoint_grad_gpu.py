@@ -189,3 +189,17 @@ def test_host_path(rt):
     spec = descriptors.checkpoint_weight_grad("f16", out_dtype="f32", accumulate=True)
     with pytest.raises(ExecutorError, match="adds to its output"):
         rt.run(spec.binary, spec.name, args, [np.zeros((64, 32), np.float32)], spec.pack(s))
+
+
+def test_offsets_beyond_32_bits(rt):
+    """Codes and dy as column ranges of tensors of 2.4e9 elements: the same bits as from dense rows."""
+    T, D, N, ld = 150000, 64, 72, 16384
+    x, dy = inputs(T, D, N, "bf16", 21)
+    codes, exps = packed(rt, x, "bf16")
+    want = call(rt, descriptors.checkpoint_weight_grad("bf16", "f32"), {"T": T, "D": D, "N": N}, {"codes": codes, "exps": exps, "dy": dy})["dweight"]
+    wide_codes, wide_dy = torch.full((T, ld), 3, dtype=torch.uint8, device="cuda"), torch.full((T, ld), 3, dtype=torch.bfloat16, device="cuda")
+    wide_codes[:, 16000:16000 + D], wide_dy[:, 8000:8000 + N] = codes, dy
+    spec = descriptors.checkpoint_weight_grad("bf16", "f32", strided=("codes", "dy"))
+    got = call(rt, spec, {"T": T, "D": D, "N": N, "LD_codes": ld, "OFF_codes": 16000, "LD_dy": ld, "OFF_dy": 8000},
+               {"codes": wide_codes, "exps": exps, "dy": wide_dy}, {"dweight": torch.empty_like(want)})["dweight"]
+    assert torch.equal(got, want)
