@@ -50,7 +50,7 @@ struct BlockNormLaunch {
   NormVectors a, b;            // a: norm of y; b: norm of the stream
   int gateForm, gateAct;
   RowsIn gate;
-  int64_t groupRows;           // rows that share a gate row (kGateGroup)
+  int64_t groupRows;           // rows that share a gate row (kGateGroup), at most `rows`
   const void *scale;           // [cols] or null
   float alpha, epsA, epsB;
   RowsOut out, h;

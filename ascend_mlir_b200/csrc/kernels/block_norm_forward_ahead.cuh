@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(PASS == kPre ? kForwardAheadThreads : kForward
 #pragma unroll
   for (int i = 0; i < NV; ++i) has[i] = FULL || col0 + i * apart < cols;
   const bool gated = PASS != kPre && p.gateForm != kGateNone, grouped = PASS != kPre && p.gateForm == kGateGroup;
-  const unsigned int groupRows = static_cast<unsigned int>(min(p.groupRows, static_cast<int64_t>(0x7fffffff)));
+  const unsigned int groupRows = static_cast<unsigned int>(p.groupRows);  // at most the rows
 
   constexpr unsigned int perVector = (PASS == kPre ? kForwardAheadThreads : kForwardAheadPostThreads) * 16, perTensor = NV * perVector;
   constexpr unsigned int atX = PASS == kPre ? 0 : perTensor, atGate = 2 * perTensor;

@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(512) blockNormForwardVectorKernel(const __grid
     const bool gated = PASS != kPre && p.gateForm != kGateNone;
     int64_t gateRow = row;  // rows and groups are counted in 32 bits
     if (PASS != kPre && p.gateForm == kGateGroup)
-      gateRow = static_cast<unsigned int>(row) / static_cast<unsigned int>(min(p.groupRows, static_cast<int64_t>(0x7fffffff)));
+      gateRow = static_cast<unsigned int>(row) / static_cast<unsigned int>(p.groupRows);
 #pragma unroll
     for (int i = 0; i < NV; ++i) raw0[i] = colOf(i) < cols ? raw(first, row, i) : make_uint4(0u, 0u, 0u, 0u);
     if constexpr (PASS != kPre) {
