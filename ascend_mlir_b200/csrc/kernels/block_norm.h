@@ -109,12 +109,18 @@ struct CheckpointGradLaunch {
   RowsIn dy;
   RowsOut out;
   int accumulate;              // add to what `out` (f32) holds
-  unsigned int *status;        // device word for a pipeline wait that ran out
+  int statusWord;              // which of the device's words takes a pipeline wait that ran out
   void *workspace;
   size_t workspaceBytes;
 };
 size_t checkpointGradWorkspaceBytes(int64_t cols, int64_t outCols, int64_t rows, int smCount);
 int launchCheckpointGrad(const CheckpointGradLaunch &l, cudaStream_t stream, int *launched, char *errorText);
+
+// Words that the weight gradient reports a wait that ran out in.  They are part of the library on each device, so a launch
+// needs no memory for its word, and a graph that is replayed late writes into one that is still there.
+constexpr int kCheckpointGradStatusWords = 4096;
+// Reads one of the current device's words, and clears it.  0: no wait ran out; else the error in errorText (256 bytes).
+int checkpointGradCheckStatus(int word, char *errorText);
 
 } // namespace kernels
 } // namespace afir

@@ -19,7 +19,7 @@
 // TM = 128 * MB rows of dweight per CTA; MB = 2 halves what dy costs per flop.  One persistent CTA per SM.  Where the
 // tiles of dweight are fewer than the SMs the tokens are cut into slices whose partial tiles (f32) a second kernel adds in order.
 //
-// Every wait on an mbarrier is bounded, as in matmul_tcgen05.cu: after about 2 s a status word is set, every role leaves
+// Every wait on an mbarrier is bounded, as in matmul_tcgen05.cu: after about 2 s the launch's status word is set, every role leaves
 // its loop, copies in flight are waited for (bounded), tensor memory is freed and the kernel returns.
 #include <algorithm>
 #include <cstdio>
@@ -33,6 +33,9 @@
 namespace afir {
 namespace kernels {
 namespace {
+
+// 0, or (1 << 8) | the role whose wait ran out first.
+__device__ unsigned int checkpointGradStatusWords[kCheckpointGradStatusWords];
 
 constexpr int kTileN = 256;
 constexpr int kTokens = 64;                      // summed per stage
@@ -81,7 +84,7 @@ struct GradParams {
   int64_t splitStride;
   int accumulate;
   unsigned int idesc;
-  unsigned int *status;
+  int statusWord;
 };
 
 // 16 codes -> 16 values of the operand type, times the power (2^k as f32 bits).
@@ -149,7 +152,7 @@ checkpointGradKernel(const __grid_constant__ CUtensorMap mapDy, const __grid_con
     mbarInit(smemAddr(&ctl->tileFull), 1);
     mbarInit(smemAddr(&ctl->tileEmpty), kConvertWarps);
     ctl->abort.flag = 0;
-    ctl->abort.status = prm.status;
+    ctl->abort.status = &checkpointGradStatusWords[prm.statusWord];
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     prefetchTensorMap(&mapDy);
@@ -463,6 +466,7 @@ int launchCheckpointGrad(const CheckpointGradLaunch &l, cudaStream_t stream, int
     gradFail(errorText, "checkpoint gradient: codes, dy and dweight must be 16-byte aligned");
     return 1;
   }
+  if (l.statusWord < 0 || l.statusWord >= kCheckpointGradStatusWords) { gradFail(errorText, "checkpoint gradient: no such status word"); return 1; }
   if (l.rows >= (1ll << 31) - kTokens || l.cols >= (1ll << 30) || l.outCols >= (1ll << 30)) { gradFail(errorText, "checkpoint gradient: dimension too large"); return 1; }
   if (l.rows == 0) {  // a sum of nothing
     if (l.accumulate) return 0;
@@ -496,7 +500,7 @@ int launchCheckpointGrad(const CheckpointGradLaunch &l, cudaStream_t stream, int
   p.codesLd = l.in.codesLd;
   p.exps = l.in.exps;
   p.expsLd = l.in.expsLd;
-  p.status = l.status;
+  p.statusWord = l.statusWord;
   const bool joined = plan.splits > 1;
   p.out = joined ? l.workspace : l.out.base;
   p.outLd = joined ? l.outCols : l.out.ld;
@@ -520,6 +524,23 @@ int launchCheckpointGrad(const CheckpointGradLaunch &l, cudaStream_t stream, int
     if (rc == 0 && launched) *launched += 1;
   }
   return rc;
+}
+
+int checkpointGradCheckStatus(int word, char *errorText) {
+  unsigned int status = 0;
+  const size_t at = static_cast<size_t>(word) * sizeof(status);
+  cudaError_t e = cudaMemcpyFromSymbol(&status, checkpointGradStatusWords, sizeof(status), at);
+  if (e == cudaSuccess && status == 0) return 0;
+  if (e != cudaSuccess) {
+    if (errorText) std::snprintf(errorText, 256, "checkpoint gradient: status read failed: %s", cudaGetErrorString(e));
+    return 1;
+  }
+  const unsigned int zero = 0;
+  cudaMemcpyToSymbol(checkpointGradStatusWords, &zero, sizeof(zero), at);
+  static const char *roles[] = {"TMA producer", "MMA issuer", "output", "conversion"};
+  if (errorText)
+    std::snprintf(errorText, 256, "checkpoint gradient: %s gave up waiting on a pipeline barrier after 2 s (status 0x%x)", roles[std::min(3u, status & 0xffu)], status);
+  return 1;
 }
 
 } // namespace kernels

@@ -4,7 +4,10 @@
 
 #include "codegen/nvrtc_compile.h"
 
+#include "kernels/block_norm.h"
+
 #include <algorithm>
+#include <atomic>
 #include <cctype>
 #include <cstdio>
 #include <cstdlib>
@@ -217,6 +220,26 @@ Status CudaExecutor::validate(const RunRequest &req, CachedKernel *&kernel, std:
   return Status::success();
 }
 
+// Executors keep apart what their launches report; beyond the library's words they share the last one.
+static int nextGradientWord() {
+  static std::atomic<uint64_t> taken{0};
+  return static_cast<int>(std::min<uint64_t>(taken.fetch_add(1), kernels::kCheckpointGradStatusWords - 1));
+}
+
+void CudaExecutor::prepareGradient(const LaunchDescriptor &d, LaunchArgs &args) {
+  if (d.kernelClass != KernelClass::CheckpointGrad) return;
+  if (gradientWord_ < 0) gradientWord_ = nextGradientWord();
+  args.gradientWord = gradientWord_;
+}
+
+void CudaExecutor::noteGradient(const LaunchDescriptor &d, void *stream) {
+  if (d.kernelClass != KernelClass::CheckpointGrad) return;
+  gradientPending_ = true;
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &capture) != cudaSuccess) cudaGetLastError();
+  else if (capture != cudaStreamCaptureStatusNone) gradientCaptured_ = true;
+}
+
 // Below this size the driver's own staging of a pageable buffer is not worth replacing.
 static constexpr size_t kStagingMinBytes = 1u << 20;
 static bool stagingEnabled() {
@@ -353,6 +376,7 @@ Status CudaExecutor::runHost(const RunRequest &req) {
   if (Status s = ownWorkspace(wsBytes); !s) return s.withStage("cuda:memory");
   args.workspace = workspace_.ptr;
   args.workspaceBytes = workspace_.capacity;
+  prepareGradient(*desc, args);
   if (launchTraceEnabled()) printLaunchTrace(req, *desc, args, device_, "host");
 
   // Large runs whose work splits along the leading axis are pipelined: copies in, kernel and copies out
@@ -418,6 +442,7 @@ Status CudaExecutor::runHost(const RunRequest &req) {
   }
   if (stager_)
     if (Status fs = stager_->finishOut(); !fs) return fs;
+  noteGradient(*desc, stream_);
   statusPending_ = info.usesStatusBlock;
   statusWorkspace_ = workspace_.ptr;
   matmulPending_ = desc->kernelClass == KernelClass::Matmul;
@@ -579,21 +604,21 @@ Status CudaExecutor::launchDevice(const RunRequest &req, void *workspace, size_t
     if (isOperatorClass(desc->kernelClass) && wsBytes > kWorkspaceStatusBytes)
       return Status::error("[cuda:memory] kernel '" + desc->kernel + "' needs a workspace of " + std::to_string(wsBytes) +
                            " bytes from the caller at these sizes");
-    // (forward row passes and checkpoints need none at all: nothing is allocated, so a first launch can be captured)
-    if (desc->kernelClass != KernelClass::BlockNorm && desc->kernelClass != KernelClass::Checkpoint) {
+    // (one that needs none gets none: nothing is allocated, so a first launch can be captured)
+    if (!isOperatorClass(desc->kernelClass)) {
       if (Status s = ownWorkspace(wsBytes); !s) return s.withStage("cuda:memory");
       args.workspace = workspace_.ptr;
       args.workspaceBytes = workspace_.capacity;
     }
   }
+  prepareGradient(*desc, args);
   const bool trace = launchTraceEnabled();  // the environment is read once per launch
   if (trace) printLaunchTrace(req, *desc, args, device_, "device");
   LaunchInfo info;
   // The status words (bad gather indices, a staged reduction's time-out) accumulate over the launches queued since
   // the last synchronize: they are cleared only when nothing unread is pending on this workspace.
   const bool hasStatusWords = (desc->kernelClass == KernelClass::Gather || desc->kernelClass == KernelClass::RowReduce ||
-                               desc->kernelClass == KernelClass::Matmul || desc->kernelClass == KernelClass::Transpose ||
-                               desc->kernelClass == KernelClass::CheckpointGrad) &&
+                               desc->kernelClass == KernelClass::Matmul || desc->kernelClass == KernelClass::Transpose) &&
                               args.workspace && args.workspaceBytes >= kWorkspaceStatusBytes;
   if (hasStatusWords && !(statusPending_ && statusWorkspace_ == args.workspace)) {
     e = cudaMemsetAsync(args.workspace, 0, kWorkspaceStatusReadBytes, args.stream);
@@ -606,6 +631,7 @@ Status CudaExecutor::launchDevice(const RunRequest &req, void *workspace, size_t
   if (!ls) return launchStage(ls);
   if (trace && !info.plan.empty()) std::fprintf(stderr, "[cuda-launch] matmul plan: %s\n", info.plan.c_str());
   if (trace) std::fprintf(stderr, "[cuda-launch] code=%s kernels=%d\n", info.generated ? "generated" : "library", info.kernelsLaunched);
+  noteGradient(*desc, stream);
   statusPending_ = statusPending_ || info.usesStatusBlock;
   if (info.usesStatusBlock) statusWorkspace_ = args.workspace;
   matmulPending_ = desc->kernelClass == KernelClass::Matmul;
@@ -632,6 +658,7 @@ Status CudaExecutor::profileResident(const RunRequest &req, int repeats, double 
   }
   args.workspace = workspace_.ptr;
   args.workspaceBytes = workspace_.capacity;
+  prepareGradient(*kernel->desc, args);
   cudaEvent_t e0, e1;
   if (cudaEventCreate(&e0) != cudaSuccess || cudaEventCreate(&e1) != cudaSuccess) return Status::error("[cuda:profiling] cannot create events");
   std::vector<float> times;
@@ -680,16 +707,14 @@ Status CudaExecutor::synchronize(void *stream) {
     }
     if (static_cast<unsigned int>(words[2] & 0xffffffffull) != 0)
       return Status::error("[cuda:kernel_launch] transpose: a wait for a staged tile ran out after 2 s");
-    if (const unsigned int cg = static_cast<unsigned int>(words[2] >> 32)) {
-      static const char *roles[] = {"TMA producer", "MMA issuer", "output", "conversion"};
-      char text[160];
-      std::snprintf(text, sizeof(text), "[cuda:kernel_launch] checkpoint gradient: %s gave up waiting on a pipeline barrier after 2 s (status 0x%x)",
-                    roles[std::min(3u, cg & 0xffu)], cg);
-      return Status::error(text);
-    }
     constexpr unsigned long long kGatherTimeoutFlag = 1ull << 62;  // set by the staged gather kernel when a stage wait ran out
     if (bad & kGatherTimeoutFlag) return Status::error("[cuda:kernel_launch] gather kernel gave up waiting for a staged copy");
     if (bad) return Status::error("[cuda:kernel_launch] gather index out of range (" + std::to_string(bad) + " indices)");
+  }
+  if (gradientPending_ || gradientCaptured_) {
+    gradientPending_ = false;
+    char text[256] = {0};
+    if (kernels::checkpointGradCheckStatus(gradientWord_, text) != 0) return Status::error(std::string("[cuda:kernel_launch] ") + text);
   }
   if (reducePending_) {
     reducePending_ = false;

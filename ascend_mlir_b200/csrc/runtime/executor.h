@@ -128,6 +128,12 @@ private:
   bool matmulPending_ = false;
   bool transposePending_ = false;  // a transpose-capable launch ran without a status block: the library's own word is checked
   bool reducePending_ = false;
+  // Time-outs of the checkpoint gradient: this executor's word (taken at its first such launch), and whether it is to be read:
+  // after a launch, and always once a launch was captured, since a replay is not seen here.
+  int gradientWord_ = -1;
+  bool gradientPending_ = false, gradientCaptured_ = false;
+  void prepareGradient(const LaunchDescriptor &d, LaunchArgs &args);
+  void noteGradient(const LaunchDescriptor &d, void *stream);
 };
 
 } // namespace afir

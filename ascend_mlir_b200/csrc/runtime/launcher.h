@@ -21,7 +21,6 @@ constexpr size_t kWorkspaceStatusBytes = 256;
 constexpr size_t kWorkspaceReduceStatusOffset = 8;  // u32: a staged row-reduction kernel gave up waiting for a copy
 constexpr size_t kWorkspaceMatmulStatusOffset = 12; // u32: (1 << 8) | role of a matmul pipeline wait that ran out
 constexpr size_t kWorkspaceTransposeStatusOffset = 16;  // u32: the copy-engine transpose gave up waiting for a tile
-constexpr size_t kWorkspaceCheckpointGradStatusOffset = 20;  // u32: (1 << 8) | role of a wait of the checkpoint gradient
 constexpr size_t kWorkspaceStatusReadBytes = 24;    // what the executor reads back after a run
 
 struct LaunchArgs {
@@ -43,6 +42,7 @@ struct LaunchArgs {
   // peer-mapped).  Its entry in argPtrs is ignored (may be null); its entry in argBytes is the whole table's size.
   std::vector<const void *> tableShards;
   int64_t rowsPerShard = 0;
+  int gradientWord = 0;  // checkpoint_grad: the device's word that takes a wait that ran out (kernels/block_norm.h)
 };
 
 struct LaunchInfo {
