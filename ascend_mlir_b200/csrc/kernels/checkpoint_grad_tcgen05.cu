@@ -55,24 +55,12 @@ template <int MB> struct GradShape {
 template <int MB> struct GradControl {
   using S = GradShape<MB>;
   unsigned long long bFull[S::kBStages], bEmpty[S::kBStages], aFull[S::kATiles], aEmpty[S::kATiles];
-  unsigned long long tileFull, tileEmpty;
+  unsigned long long tileFull, tileEmpty, drained;
   unsigned int tmemBase;
   AbortState abort;
 };
 template <int MB> constexpr size_t gradSmemBytes() { return 1024 + GradShape<MB>::kControlAt + sizeof(GradControl<MB>); }
 static_assert(gradSmemBytes<1>() <= 227 * 1024 && gradSmemBytes<2>() <= 227 * 1024, "shared memory of a CTA");
-
-// Place in a ring of N and the parity of its round.
-template <int N> struct Ring {
-  int at = 0;
-  unsigned int phase = 0;
-  __device__ __forceinline__ void next() {
-    if (++at == N) {
-      at = 0;
-      phase ^= 1u;
-    }
-  }
-};
 
 struct GradParams {
   int D, N, T;
@@ -150,6 +138,7 @@ checkpointGradKernel(const __grid_constant__ CUtensorMap mapDy, const __grid_con
       mbarInit(smemAddr(&ctl->aEmpty[a]), 1);
     }
     mbarInit(smemAddr(&ctl->tileFull), 1);
+    mbarInit(smemAddr(&ctl->drained), 1);
     mbarInit(smemAddr(&ctl->tileEmpty), kConvertWarps);
     ctl->abort.flag = 0;
     ctl->abort.status = &checkpointGradStatusWords[prm.statusWord];
@@ -179,9 +168,9 @@ checkpointGradKernel(const __grid_constant__ CUtensorMap mapDy, const __grid_con
     k1 = min(prm.kBlocks, k0 + prm.kPerSplit);
   };
 
+  Ring<kBStages> ring;  // of dy's stages, the producer's
   if (warp == 0) {
     if (lane == 0) {
-      Ring<kBStages> ring;
       bool ok = true;
       for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
         int tm, tn, k0, k1, split;
@@ -192,14 +181,6 @@ checkpointGradKernel(const __grid_constant__ CUtensorMap mapDy, const __grid_con
           mbarExpectTx(full, kBStage);
 #pragma unroll
           for (int j = 0; j < 4; ++j) tmaLoad2d(to + j * kBlockBytes, &mapDy, tn * kTileN + j * 64, kb * kTokens, full);
-        }
-      }
-      if (!ok) {
-        // loads already issued still land in this CTA's shared memory: give them time before leaving
-        for (int s = 0; s < kBStages; ++s) {
-          const unsigned long long t0 = globalTimerNs();
-          while (!mbarTryWait(smemAddr(&ctl->bFull[s]), 0) && !mbarTryWait(smemAddr(&ctl->bFull[s]), 1) && globalTimerNs() - t0 < 1000000ull) {
-          }
         }
       }
     }
@@ -368,7 +349,17 @@ checkpointGradKernel(const __grid_constant__ CUtensorMap mapDy, const __grid_con
 
   tcgen05FenceBefore();
   __syncthreads();
+  // Where a wait ran out, copies may still land in this CTA's shared memory and products read it: they get time to end.
+  const bool gaveUp = abortFlag->flag != 0;
+  if (gaveUp && threadIdx.x == 0) {
+    for (int s = 0; s < kBStages; ++s) mbarDrain(smemAddr(&ctl->bFull[s]), newestFillParity(s, ring.at, ring.phase));
+  }
   if (warp == 1) {
+    if (gaveUp && lane == 0) {
+      ummaCommit(smemAddr(&ctl->drained));
+      mbarDrain(smemAddr(&ctl->drained), 0);
+    }
+    __syncwarp();
     tcgen05FenceAfter();
     tmemDealloc(tmemBase, S::kTmemCols);
   }

@@ -310,12 +310,7 @@ matmulBiasActKernel(const __grid_constant__ CUtensorMap mapA, const __grid_const
       }
       if (!ok) {
         // loads already issued still land in this CTA's shared memory: give them time before leaving
-        for (int s = 0; s < STAGES; ++s) {
-          const unsigned long long t0 = globalTimerNs();
-          while (!mbarTryWait(smemAddr(&ctl->full[s]), 0) && !mbarTryWait(smemAddr(&ctl->full[s]), 1) &&
-                 globalTimerNs() - t0 < 1000000ull) {
-          }
-        }
+        for (int s = 0; s < STAGES; ++s) mbarDrain(smemAddr(&ctl->full[s]), newestFillParity(s, static_cast<int>(it % STAGES), (it / STAGES) & 1u));
       }
     }
   } else if (warp == 1) {

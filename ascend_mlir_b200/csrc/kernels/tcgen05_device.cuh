@@ -10,6 +10,7 @@
 #include <mutex>
 
 #include "kernels/kernels.h"
+#include "kernels/ring.h"
 
 namespace afir {
 namespace kernels {
@@ -69,6 +70,12 @@ __device__ __forceinline__ bool mbarWait(unsigned int bar, unsigned int parity, 
         return false;
       }
     }
+  }
+}
+// Waits for a phase, 1 ms at most: for copies into, or products that read, memory that a CTA is about to give up.
+__device__ __forceinline__ void mbarDrain(unsigned int bar, unsigned int parity) {
+  const unsigned long long t0 = globalTimerNs();
+  while (!mbarTryWait(bar, parity) && globalTimerNs() - t0 < 1000000ull) {
   }
 }
 __device__ __forceinline__ void tmaLoad2d(unsigned int dst, const CUtensorMap *map, int x, int y, unsigned int bar) {

@@ -27,6 +27,7 @@
 #include "kernels/grid_dependency.cuh"
 #include "kernels/kernels.h"
 #include "kernels/launch_util.h"
+#include "kernels/ring.h"
 
 namespace afir {
 namespace kernels {
@@ -145,9 +146,11 @@ transposeTmaKernel(const __grid_constant__ CUtensorMap mapIn, const __grid_const
       }
       if (!ok) {
         // loads already issued still land in this CTA's shared memory: give them time before the CTA ends
+        const unsigned int next = it - 1;  // the tile that was not loaded
         for (int s = 0; s < kStages; ++s) {
+          const unsigned int parity = newestFillParity(s, static_cast<int>(next % kStages), (next / kStages) & 1u);
           const unsigned long long t0 = globalTimerNs();
-          while (!mbarTryWait(smemAddr(&full[s]), 0) && !mbarTryWait(smemAddr(&full[s]), 1) && globalTimerNs() - t0 < 1000000ull) {
+          while (!mbarTryWait(smemAddr(&full[s]), parity) && globalTimerNs() - t0 < 1000000ull) {
           }
         }
       }
