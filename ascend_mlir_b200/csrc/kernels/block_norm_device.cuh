@@ -108,17 +108,18 @@ struct Team {
 constexpr int kTeamValues = 3;
 constexpr int kTeamSlice = 64;  // floats per value: the CTA's warps, each team's rounded up to 4, 8 or 16
 constexpr int kTeamScratchFloats = 2 * kTeamValues * kTeamSlice;
+struct alignas(16) TeamScratch { float values[kTeamScratchFloats]; };  // the CTA's buffer: read 16 bytes at a time
 
 __device__ __forceinline__ void teamBarrier(const Team &t) { asm volatile("bar.sync %0, %1;" ::"r"(t.index + 1), "r"(t.lanes) : "memory"); }
 
-__device__ __forceinline__ Team makeTeam(int lanes, float *scratch) {
+__device__ __forceinline__ Team makeTeam(int lanes, TeamScratch &scratch) {
   Team t;
   t.lanes = lanes;
   t.index = static_cast<int>(threadIdx.x) / lanes;
   t.lane = static_cast<int>(threadIdx.x) - t.index * lanes;
   t.count = static_cast<int>(blockDim.x) / lanes;
   const int warps = lanes >> 5, slice = warps <= 4 ? 4 : warps <= 8 ? 8 : 16;
-  t.scratch = scratch + t.index * slice;
+  t.scratch = scratch.values + t.index * slice;
   t.half = 0;
   if (lanes > 32) {
     if (t.lane < slice) {

@@ -72,7 +72,7 @@ template <int ELEM, int KIND, int PASS, int NV>
 __global__ void __launch_bounds__(512) blockNormForwardKernel(const __grid_constant__ BlockNormLaunch p, int teamLanes) {
   gridDependencyPrologue();
   constexpr int VEC = ElemOf<ELEM>::kVec, EB = 16 / VEC;
-  __shared__ float scratch[kTeamScratchFloats];
+  __shared__ TeamScratch scratch;
   Team team = makeTeam(teamLanes, scratch);
   const int cols = static_cast<int>(p.cols);
   const int64_t step = static_cast<int64_t>(gridDim.x) * team.count;

@@ -23,7 +23,7 @@ __global__ void __launch_bounds__(PASS == kPre ? kForwardAheadThreads : kForward
   constexpr bool kLayer = KIND == kLayerNorm;
   constexpr int VEC = ElemOf<ELEM>::kVec, P = kPairs<ELEM>, EB = 16 / VEC;
   extern __shared__ uint4 slots[];  // [stages][tensors][NV][perVector / 16], then parameters
-  __shared__ float scratch[kTeamScratchFloats];
+  __shared__ TeamScratch scratch;
   Team team = makeTeam(teamLanes, scratch);
   const int cols = static_cast<int>(p.cols), rows = static_cast<int>(p.rows);
   const float share = 1.0f / static_cast<float>(cols);

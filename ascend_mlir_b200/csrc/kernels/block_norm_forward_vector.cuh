@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(512) blockNormForwardVectorKernel(const __grid
   gridDependencyPrologue();
   constexpr int VEC = ElemOf<ELEM>::kVec, P = kPairs<ELEM>;
   constexpr int kPostVectors = PASS == kPre ? 1 : NV;
-  __shared__ float scratch[kTeamScratchFloats];
+  __shared__ TeamScratch scratch;
   Team team = makeTeam(teamLanes, scratch);
   const int cols = static_cast<int>(p.cols);
   const float share = 1.0f / static_cast<float>(cols);

@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(512) blockNormGradKernel(const __grid_constant
   constexpr int VEC = ElemOf<ELEM>::kVec, EB = 16 / VEC;
   constexpr int kValues = kLayer ? 2 : 1;
   constexpr bool kPostPart = PASS != kPre, kPrePart = PASS != kPost;
-  __shared__ float scratch[kTeamScratchFloats];
+  __shared__ TeamScratch scratch;
   Team team = makeTeam(teamLanes, scratch);
   const int cols = static_cast<int>(p.cols);
   const float share = 1.0f / static_cast<float>(cols);

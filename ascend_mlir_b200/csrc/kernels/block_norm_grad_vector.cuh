@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(kGradAheadThreads) blockNormGradVectorKernel(c
   constexpr bool kPostPart = PASS != kPre, kPrePart = PASS != kPost, kToken = TOKEN;
   constexpr int VEC = ElemOf<ELEM>::kVec, P = kPairs<ELEM>, EB = 16 / VEC;
   extern __shared__ uint4 slots[];  // [stages][tensors][NV][kGradAheadThreads], then parameters
-  __shared__ float scratch[kTeamScratchFloats];
+  __shared__ TeamScratch scratch;
   Team team = makeTeam(teamLanes, scratch);
   const int cols = static_cast<int>(p.cols);
   const float share = 1.0f / static_cast<float>(cols);
