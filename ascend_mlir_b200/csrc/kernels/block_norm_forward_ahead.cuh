@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(PASS == kPre ? kForwardAheadThreads : kForward
         F2 t[P];
         if (gated) {
           widenPairs<ELEM>(readSlot(slot + atGate + i * perVector), t);
-          gatePairs(t, p.gateAct);
+          gatePairs<ELEM>(t, p.gateAct);
 #pragma unroll
           for (int e = 0; e < P; ++e) v[i][e] = v[i][e] * t[e];
         }

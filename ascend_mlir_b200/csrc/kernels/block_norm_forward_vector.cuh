@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(512) blockNormForwardVectorKernel(const __grid
         F2 t[P];
         if (gated) {
           widenPairs<ELEM>(rawGate[i], t);
-          gatePairs(t, p.gateAct);
+          gatePairs<ELEM>(t, p.gateAct);
 #pragma unroll
           for (int e = 0; e < P; ++e) v[i][e] = v[i][e] * t[e];
         }

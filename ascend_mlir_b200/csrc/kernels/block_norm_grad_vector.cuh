@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kGradAheadThreads) blockNormGradVectorKernel(c
       }
       if (gateRow >= 0) {
         loadPairs<ELEM>(p.gate.base, static_cast<int64_t>(gateRow) * p.gate.ld + col0 + i * apart, y);
-        gatePairs(y, p.gateAct);
+        gatePairs<ELEM>(y, p.gateAct);
 #pragma unroll
         for (int e = 0; e < P; ++e) x[e] = x[e] * y[e];
       }
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(kGradAheadThreads) blockNormGradVectorKernel(c
         if constexpr (kToken) {
           F2 a[P], bias[P];
           widenPairs<ELEM>(readSlot(slot + atGate + i * perVector), a);
-          gatePairs(a, p.gateAct);
+          gatePairs<ELEM>(a, p.gateAct);
           if constexpr (kLayer) readParams(biasA, i, bias);
 #pragma unroll
           for (int e = 0; e < P; ++e) {

@@ -115,17 +115,20 @@ template <int ELEM> __device__ __forceinline__ void codePairs(const uint2 &raw, 
     v[i] = pairOf(f.x, f.y) * power;
   }
 }
-// act(gate) of a vector in place; the derivative from the value.  The sigmoid takes CUDA's fast exponential and division,
-// since these kernels are bound by the instructions they issue: with their published bounds, (2 + 1.16 |g|) and 2 units in the
-// last place, it is off by less than 4e-7, and by 2.5e-6 of itself down to g = -14; beyond |g| = 87 it is 0 or 1, as
-// f32's own to 1e-37.
-__device__ __forceinline__ float sigmoidOf(float g) { return __fdividef(1.0f, 1.0f + __expf(-g)); }
-template <int N> __device__ __forceinline__ void gatePairs(F2 (&g)[N], int act) {
+// act(gate) of a vector in place; the derivative from the value.  Of f32 rows as gateValue has it.  In 16-bit rows the sigmoid takes
+// CUDA's fast exponential and division, since these kernels are bound by the instructions they issue: with their published
+// bounds, (2 + 1.16 |g|) and 2 units in the last place, it is off by less than 4e-7, and by 2.5e-6 of itself down to g = -14,
+// where the stored type's half step is 4.9e-4 (f16); beyond |g| = 87 it is 0 or 1, as f32's own to 1e-37.
+template <int ELEM> __device__ __forceinline__ float sigmoidOf(float g) {
+  if constexpr (ELEM == kF32) return gateValue(g, kActSigmoid);
+  else return __fdividef(1.0f, 1.0f + __expf(-g));
+}
+template <int ELEM> __device__ __forceinline__ void gatePairs(F2 (&g)[kPairs<ELEM>], int act) {
   if (act == kActNone) return;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
+  for (int i = 0; i < kPairs<ELEM>; ++i) {
     const float2 f = valuesOf(g[i]);
-    if (act == kActSigmoid) g[i] = pairOf(sigmoidOf(f.x), sigmoidOf(f.y));
+    if (act == kActSigmoid) g[i] = pairOf(sigmoidOf<ELEM>(f.x), sigmoidOf<ELEM>(f.y));
     else g[i] = pairOf(tanhf(f.x), tanhf(f.y));
   }
 }
