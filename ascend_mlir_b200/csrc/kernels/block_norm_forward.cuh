@@ -36,7 +36,7 @@ __device__ __forceinline__ void rowStatistics(Team &team, const float (&v)[NV][V
     }
   }
   teamSum(team, q);
-  rstd = 1.0f / sqrtf(q[0] * share + eps);
+  rstd = __frsqrt_rn(q[0] * share + eps);
 }
 
 template <int ELEM, int KIND, int NV, int VEC>

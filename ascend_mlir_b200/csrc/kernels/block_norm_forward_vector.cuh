@@ -12,6 +12,10 @@
 namespace afir {
 namespace kernels {
 
+// Of f32 rows rounded once; of 16-bit rows within two units in the last place of f32, in fewer instructions (16384 x 4096 f16
+// layer, both norms: 114 us, 121 rounded once).
+template <int ELEM> __device__ __forceinline__ float inverseRoot(float v) { return ELEM == kF32 ? __frsqrt_rn(v) : rsqrtf(v); }
+
 // Mean and 1/sqrt(variance + eps) of the row in v; what lies beyond the row is zero in v and not counted.
 template <int ELEM, int KIND, int NV>
 __device__ __forceinline__ void pairStatistics(Team &team, const F2 (&v)[NV][kPairs<ELEM>], int cols, float share, bool full, float eps, float &mean, float &rstd) {
@@ -25,7 +29,7 @@ __device__ __forceinline__ void pairStatistics(Team &team, const F2 (&v)[NV][kPa
     float s[1] = {sumOf(q)};
     teamSum(team, s);
     mean = 0.0f;
-    rstd = rsqrtf(s[0] * share + eps);
+    rstd = inverseRoot<ELEM>(s[0] * share + eps);
   } else {
     F2 sum = splat(0.0f);
 #pragma unroll
@@ -81,7 +85,7 @@ __device__ __forceinline__ void pairStatistics(Team &team, const F2 (&v)[NV][kPa
       const float off = (full ? sw * kWhole : __fdividef(sw, fmaxf(count, 1.0f))) - mean;  // the same quotient as the warp's centre
       squares = treeSum(fmaf(count * off, off, buf[kTeamSlice + w]));
     }
-    rstd = rsqrtf(squares * share + eps);
+    rstd = inverseRoot<ELEM>(squares * share + eps);
   }
 }
 

@@ -1,15 +1,17 @@
-"""Values of f32 rows that can be read off one by one: the gate's activation behind a norm that is exactly one.  The three
-kernels of each direction (few rows, many rows, rows off 16 bytes) give the same bits.
+"""Values of f32 rows that can be read off one by one: the statistics of rows whose sums are exact, and the gate's
+activation behind a norm that is exactly one.  The three kernels of each direction (few rows, many rows, rows off 16 bytes)
+give the same bits.
 
-Bounds, u = 2^-24.  The sigmoid: exp is within 2 units in the last place (4u) by
-CUDA's tables, 1 + e and the quotient one half each: 6u.  Its derivative a - a^2 takes (1 - 2a) times that, and three roundings."""
+Bounds, u = 2^-24: 1/sqrt of an exact square is rounded once (u) for f32 rows, and within 2 units in the last place (4u) by
+CUDA's tables for 16-bit ones.  The sigmoid: exp is within 2 units in the last place (4u) by them, 1 + e and the quotient one half
+each: 6u.  Its derivative a - a^2 takes (1 - 2a) times that, and three roundings."""
 import pytest
 import torch
 
 from ascend_mlir_b200 import descriptors
 from ascend_mlir_b200.runtime.executor import CudaRuntime
 
-from operator_calls import call, outputs_for
+from operator_calls import TORCH, call, outputs_for
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -38,6 +40,23 @@ def run(rt, build, which, sizes, inputs, shift):
     sizes = dict(sizes, **{f"LD_{shift}": sizes["D"] + 4, f"OFF_{shift}": 1})
     outs = outputs_for(build(()), sizes, torch.device("cuda"))
     return call(rt, build((shift,)), sizes, dict(inputs, **{shift: off_by_one(inputs[shift])}), outs)
+
+
+@pytest.mark.parametrize("which", ROWS)
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_rstd(rt, dtype, kind, which):
+    """Rows of c and -c in turn, c from 1 to 255: every sum of squares is a whole number below 2^24, and rstd = 1/c."""
+    most = (1 if dtype == "f32" else 4) * U
+    T, dt = ROWS[which], TORCH[dtype]
+    c = 1 + torch.arange(7, 7 + T, device="cuda") * 37 % 255
+    sign = 1 - 2 * (torch.arange(D, device="cuda") % 2)
+    t = {"x": (c[:, None] * sign).to(dt), "weight": torch.ones(D, device="cuda").to(dt), "bias": torch.zeros(D, device="cuda").to(dt)}
+    outs = run(rt, lambda s: descriptors.block_norm(dtype, kind=kind, eps=0.0, strided=s), which, {"T": T, "D": D}, t, "x")
+    want = 1 / c.double()
+    assert ((outs["rstd"].double() - want).abs() <= most * (1 + 2.0 ** -20) * want).all()
+    if kind == "layer":
+        assert (outs["mean"] == 0).all()
 
 
 def gates(T):
