@@ -19,7 +19,8 @@ extern "C" {
  * lib/Runtime/Execution/NativeExecutionRunner.cpp:436-476: argument list
  * [inputs..., outputs..., workspace, tiling] then rtKernelLaunch).  input_ptrs/output_ptrs are
  * DEVICE pointers on the executor's device.  workspace may be NULL (the executor then owns one;
- * that path may allocate) or a device buffer of workspace_bytes.  cuda_stream is a cudaStream_t
+ * that path may allocate; an operator kernel whose afirt_executor_workspace_bytes is more than 256
+ * needs the caller's) or a device buffer of workspace_bytes.  cuda_stream is a cudaStream_t
  * (NULL = default stream).  Returns after enqueueing; nothing is synchronised. */
 int afirt_executor_launch_device(AfirtExecutor executor, const uint8_t *binary_data, size_t binary_len,
                                  const char *function_name, int num_inputs, const void **input_ptrs,
@@ -30,7 +31,8 @@ int afirt_executor_launch_device(AfirtExecutor executor, const uint8_t *binary_d
 
 /* The wait half (reference NativeExecutionRunner.cpp:484-489, rtStreamSynchronize failure is an
  * error): waits for cuda_stream (NULL = the executor's own stream, or the device) and reports
- * device-side status words (gather index out of range, bounded-wait timeout in the matmul). */
+ * device-side status words (gather index out of range, bounded-wait timeout in the matmul, in the
+ * checkpoint gradient). */
 int afirt_executor_synchronize(AfirtExecutor executor, void *cuda_stream, char *err_buf, size_t err_len);
 
 /* Scratch bytes afirt_executor_launch_device needs for this binary at these tiling values
