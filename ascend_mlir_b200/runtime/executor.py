@@ -49,9 +49,10 @@ def _packed(args: Sequence[Tuple[int, int]]) -> Tuple[bytes, bytes]:
         return b"", b""
     addresses, sizes = zip(*args)
     pack = _words(len(sizes)).pack
-    if None in addresses:
-        addresses = [p or 0 for p in addresses]
-    return pack(*addresses), pack(*sizes)
+    try:
+        return pack(*addresses), pack(*sizes)
+    except struct.error:  # None, pointer objects, values that ctypes wraps
+        return bytes((ctypes.c_void_p * len(addresses))(*addresses)), bytes((ctypes.c_size_t * len(sizes))(*sizes))
 
 
 @functools.lru_cache(maxsize=None)
