@@ -16,6 +16,8 @@
 // Measured, 8192^3 bf16: 844 to 860 us alone (1.28 to 1.30 PFLOP/s, tensor pipe active 70 % of the time), 935 in a loop of
 // seconds under the power limit; a library product of two 16-bit tensors takes 664 and 728 there.  300 x 1024 x 1024 f16: 8.2 us, most
 // of it start-up and one tile's way through the pipeline.
+// The tensor cores cut their f32 sums off toward zero: over 8192 tokens in one slice the result is off by 3.6e-6 of itself (2-norm),
+// rounded sums by 3.6e-7; what is read has four significant bits.
 // TM = 128 * MB rows of dweight per CTA; MB = 2 halves what dy costs per flop.  One persistent CTA per SM.  Where the
 // tiles of dweight are fewer than the SMs the tokens are cut into slices whose partial tiles (f32) a second kernel adds in order.
 //

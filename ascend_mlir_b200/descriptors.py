@@ -503,8 +503,8 @@ def checkpoint_weight_grad(dtype: str = "bf16", out_dtype: Optional[str] = None,
 
     Inputs: codes, exps (made from `dtype`), dy [T, N] in `dtype` (f16 or bf16).  Outputs: dweight in `out_dtype` (f32 or
     `dtype`); with `accumulate` the product is added to what dweight holds.  The restored x is exact in `dtype`, products
-    are summed in f32.  Needs a workspace (workspace_bytes).  D a multiple of 16, N of 8, as are strided row lengths and
-    offsets."""
+    are summed in f32 by the tensor cores.  Needs a workspace where workspace_bytes says more than 256.  D a multiple of 16,
+    N of 8, as are strided row lengths and offsets."""
     _one_of("dtype", dtype, ("f16", "bf16"))
     _one_of("out_dtype", out_dtype or dtype, (dtype, "f32"))
     r = _Roles(dtype, strided).checkpoint().rows("dy", shape=("rows", "out_cols"))
