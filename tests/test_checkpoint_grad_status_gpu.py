@@ -84,9 +84,11 @@ def test_first_launch_in_a_capture_without_a_workspace(rt):
 
 def test_time_outs_reach_the_caller(tmp_path):
     """tests/cpp/checkpoint_grad_status.cu: the kernel's words set by hand, the executor's answers."""
-    lib_build.build()
     objs = [str(o) for o in sorted((ROOT / "ascend_mlir_b200" / "build").glob("*.o"))
             if not any(w in o.name for w in ("capi", "tools_", "checkpoint_grad_tcgen05"))]
+    # (not built here: the library that this process has loaded would be written anew)
+    if len(objs) != len(lib_build.CU_SOURCES) + len(lib_build.CPP_SOURCES) - 2:
+        pytest.skip("the library's objects are not all at hand")
     exe = tmp_path / "checkpoint_grad_status"
     res = subprocess.run([lib_build.NVCC, *lib_build.NVCC_FLAGS, str(ROOT / "tests" / "cpp" / "checkpoint_grad_status.cu"), *objs, "-o", str(exe),
                           "-ldl", "-lrt", "-lpthread"], capture_output=True, text=True)
