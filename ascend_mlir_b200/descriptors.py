@@ -318,7 +318,7 @@ class _Roles:
         operator = dict(operator, rows="rows", cols="cols", roles=roles)
         spec = _spec(name, kernel_class, self.dtype, len(self.inputs), len(self.outputs), [], list(dims) + self.dims,
                      {"operator": operator}, {})
-        if any("exp_cols" in r["shape"] for r in roles.values()):
+        if "exp_cols" in spec.shape_keys:
             spec.derived = {"EXP_COLS": lambda shape: -(-shape["D"] // CHECKPOINT_BLOCK)}
         return spec
 
